@@ -712,6 +712,66 @@ int mep_stamp(void* slots, int i, mep_stream_t stream);
 /* The counter's rate in kHz (hipDeviceAttributeWallClockRate of the current device), or < 0. */
 int mep_stamp_khz(void);
 
+/* ---------------------------------------------------------------- differential-attention block
+ * Operators of a block  h = N(x);  q, k = rotary(W_q h, W_k h);  a = diff_attention(q, k, v, lam);
+ * x' = scale x + gate N(W_o a);  h' = N'(x').  They have no counterpart in the reference scripts: its
+ * blocks take position tables, one softmax map and a LayerNorm behind the block.  The descriptors
+ * are passed from HOST memory by value; element types are MEP_F32 / MEP_BF16 / MEP_F16, strides
+ * count elements and are 64-bit, and all sums, statistics and angles are held in 32 bits or more. */
+#define MEP_F32 0
+#define MEP_BF16 1
+#define MEP_F16 2
+
+/* Rotary positions of up to two tensors [B, T, H, M, D] (x[1] = 0: one) with common positions.
+ * Pair i of the first `rot` channels turns by pos * freqs[i] radians and is scaled by `amplitude`;
+ * the channels behind are copied.  y is contiguous and apart from x.  inverse: by the negative angle (the gradient). */
+typedef struct {
+    uint64_t x[2], y[2];
+    int64_t  sB[2], sT[2], sH[2], sM[2];   /* of x; its channels are contiguous            */
+    int32_t  H[2], M[2];
+    uint64_t freqs;                        /* double [rot / 2], radians per position        */
+    uint64_t pos;                          /* int32, or int64 when pos64                    */
+    int64_t  pos_sB, pos_sT;
+    int32_t  B, T, D, rot;
+    int32_t  interleaved;                  /* pairs (2i, 2i + 1) instead of (i, i + rot / 2) */
+    int32_t  inverse, type, pos64;
+    float    amplitude;
+    int32_t  _pad;
+} mep_rotary_desc;
+int mep_rotary(const mep_rotary_desc* desc, mep_stream_t stream);
+
+/* The norms around a block with its gate and the residual scale, rows of D channels:
+ *   stream = scale x + gate N(y),  normed = N'(stream)
+ * kinds: 0 none, 1 rms, 2 layer (biased variance); eps under the root.  x = 0: no residual; normed = 0: no second norm;
+ * w, b, nw, nb = 0: ones / zeros.  gate_form 0 none, 1 [D], 2 [rows / T, D] (one row per sequence of T rows), 3 rows.
+ * w, b, nw, nb are of `wtype`, the gate of `gtype`: MEP_F32 or the activations' type (gate_form 3: that).  scale: a device
+ * float, or 0 with scale_value.  stream / normed / gradients are contiguous rows; the inputs have row strides. */
+#define MEP_BLOCK_NORM_MAX_D 8192
+typedef struct {
+    uint64_t y, x, gate, w, b, nw, nb, scale;
+    uint64_t stream, normed;
+    uint64_t stats;              /* fp32 [rows][4] (mean, r of y; mean, r of stream); fwd: 0 = not kept */
+    int64_t  y_ld, x_ld, g_ld;   /* g_ld: gate_form 3                                                   */
+    int64_t  rows;
+    int32_t  D, T, kind, next_kind, gate_form, type, wtype, gtype;
+    float    eps, scale_value;
+} mep_block_norm_desc;
+typedef struct {
+    mep_block_norm_desc f;
+    uint64_t dstream, dnormed;   /* upstream rows (0 = zero)                                            */
+    uint64_t dy, dx, dgate_rows; /* rows; dx, dgate_rows may be 0                                       */
+    uint64_t dw, db, dnw, dnb, dgate;   /* column sums in `wtype` / `gtype`, 0 = not wanted             */
+    uint64_t dscale;             /* fp32 [1] or 0                                                       */
+    uint64_t partial;            /* fp32 [mep_block_norm_partial][n_sums * D + 1]; 0 without sums       */
+    int64_t  ds_ld, dn_ld;
+    int32_t  n_sums;             /* of dw .. dgate wanted                                               */
+    int32_t  _pad;
+} mep_block_norm_bwd_desc;
+int mep_block_norm_fwd(const mep_block_norm_desc* desc, mep_stream_t stream);
+int mep_block_norm_bwd(const mep_block_norm_bwd_desc* desc, mep_stream_t stream);
+/* rows of the backward's workspace for this forward descriptor, or MEP_EINVAL */
+int mep_block_norm_partial(const mep_block_norm_desc* desc);
+
 /* ---------------------------------------------------------------- misc */
 int mep_abi_version(void);
 int mep_last_error(char* buf, size_t len);

@@ -264,13 +264,38 @@ class Seg(ctypes.Structure):
     _fields_ = [('offset', i64), ('length', i64)]
 
 
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [('x', u64 * 2), ('y', u64 * 2), ('sB', i64 * 2), ('sT', i64 * 2), ('sH', i64 * 2), ('sM', i64 * 2),
+                ('H', i32 * 2), ('M', i32 * 2), ('freqs', u64), ('pos', u64), ('pos_sB', i64), ('pos_sT', i64),
+                ('B', i32), ('T', i32), ('D', i32), ('rot', i32), ('interleaved', i32), ('inverse', i32),
+                ('type', i32), ('pos64', i32), ('amplitude', f32), ('_pad', i32)]
+
+
+BLOCK_NORM_MAX_D = 8192   # MEP_BLOCK_NORM_MAX_D
+
+
+class BlockNormDesc(ctypes.Structure):
+    _fields_ = [('y', u64), ('x', u64), ('gate', u64), ('w', u64), ('b', u64), ('nw', u64), ('nb', u64), ('scale', u64),
+                ('stream', u64), ('normed', u64), ('stats', u64), ('y_ld', i64), ('x_ld', i64), ('g_ld', i64),
+                ('rows', i64), ('D', i32), ('T', i32), ('kind', i32), ('next_kind', i32), ('gate_form', i32),
+                ('type', i32), ('wtype', i32), ('gtype', i32), ('eps', f32), ('scale_value', f32)]
+
+
+class BlockNormBwdDesc(ctypes.Structure):
+    _fields_ = [('f', BlockNormDesc), ('dstream', u64), ('dnormed', u64), ('dy', u64), ('dx', u64), ('dgate_rows', u64),
+                ('dw', u64), ('db', u64), ('dnw', u64), ('dnb', u64), ('dgate', u64), ('dscale', u64), ('partial', u64),
+                ('ds_ld', i64), ('dn_ld', i64), ('n_sums', i32), ('_pad', i32)]
+
+
 STRUCTS = {'mep_rows': Rows, 'mep_gemm_desc': GemmDesc, 'mep_gemm_sum_desc': GemmSumDesc, 'mep_wgrad_desc': WgradDesc,
            'mep_attn_desc': AttnDesc, 'mep_attn_bwd_desc': AttnBwdDesc, 'mep_attn_gen_desc': AttnGenDesc,
            'mep_attn_gen_bwd_desc': AttnGenBwdDesc, 'mep_epi_desc': EpiDesc,
            'mep_epi_bwd_desc': EpiBwdDesc, 'mep_ln_desc': LnDesc, 'mep_colsum_desc': ColsumDesc,
            'mep_sum_desc': SumDesc, 'mep_pool_desc': PoolDesc, 'mep_head_desc': HeadDesc, 'mep_seg': Seg,
            'mep_rf_epi_desc': RfEpiDesc, 'mep_rf_epi_bwd_desc': RfEpiBwdDesc, 'mep_rf_head_desc': RfHeadDesc,
-           'mep_sweep_desc': SweepDesc, 'mep_window_desc': WindowDesc, 'mep_wsplit_desc': WsplitDesc}
+           'mep_sweep_desc': SweepDesc, 'mep_window_desc': WindowDesc, 'mep_wsplit_desc': WsplitDesc,
+           'mep_rotary_desc': RotaryDesc, 'mep_block_norm_desc': BlockNormDesc,
+           'mep_block_norm_bwd_desc': BlockNormBwdDesc}
 
 P = ctypes.c_void_p
 # name -> argtypes (all return int)
@@ -302,6 +327,10 @@ SIGNATURES.update({
     'mep_threshold_sweep': [ctypes.POINTER(SweepDesc), P],
     'mep_assemble_windows': [ctypes.POINTER(WindowDesc), i32, P],
     'mep_tgemm': [P, i32, i32, i32, i32, P],
+    'mep_rotary': [ctypes.POINTER(RotaryDesc), P],
+    'mep_block_norm_fwd': [ctypes.POINTER(BlockNormDesc), P],
+    'mep_block_norm_bwd': [ctypes.POINTER(BlockNormBwdDesc), P],
+    'mep_block_norm_partial': [ctypes.POINTER(BlockNormDesc)],
     'mep_wgemm': [P, i32, i32, i32, P],
     'mep_attn_general_fwd': [P, i32, i32, P],
     'mep_attn_general_bwd': [P, i32, i32, i32, P],

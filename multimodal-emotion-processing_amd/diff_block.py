@@ -1,0 +1,308 @@
+"""Operators of a differential-attention block on libmep_hip, with their gradients:
+
+    h  = norm(x, w)                                       the norm before the block
+    q, k = rotary(q, k, positions=..., freqs=...)         rotary positions (rotary_frequencies makes freqs)
+    a  = diff_attention(q, k, v, lam, ...)                the difference of two softmax maps
+    x, h = norm_residual(y, x, ...)                       norm behind the block, gate, residual scale, next norm
+
+They stand beside the residual-attention blocks of the reference (its Attention_Block takes position tables, one
+softmax map and a LayerNorm behind the block, cmu-mosei/run.py:206-262) and have no counterpart there.  Each call is
+one launch (two where column sums or key splits are joined) on the current stream of its tensors' device, allocates
+nothing but its results and workspace, never synchronises, and may be captured into a graph.  float32, bfloat16 and float16
+activations; sums, statistics and angles in 32 bits or more; results do not depend on the order of atomics.
+
+Gradients come through torch.autograd.  To capture a backward pass into a graph, make the leaves it differentiates inside
+the capture (``x.detach().requires_grad_()``) and use ``torch.autograd.grad``: torch ends the process when a captured
+backward meets accumulators that an eager graph of the same leaves still holds.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._autograd import require_cuda
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MEP_F32 / MEP_BF16 / MEP_F16
+KINDS = {'none': 0, 'rms': 1, 'layer': 2}
+
+
+def _on_device(first, *others):
+    """The last check of a call's arguments: all on one GPU."""
+    for t in others:
+        if torch.is_tensor(t) and t.device != first.device:
+            raise ValueError('all tensors of a call live on one device; got %s and %s' % (first.device, t.device))
+    require_cuda(first)
+
+
+def _type_of(t, what):
+    if t.dtype not in TYPES:
+        raise ValueError('%s must be float32, bfloat16 or float16; got %s' % (what, t.dtype))
+    return TYPES[t.dtype]
+
+
+def _launch(name, desc, device):
+    """An entry point that takes its descriptor from the host, on the current stream of `device`."""
+    with torch.cuda.device(device):
+        _lib.call(name, ctypes.byref(desc))
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------------ rotary positions
+def rotary_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, original_len=None, low_turns=1.0,
+                       high_turns=32.0, device='cuda'):
+    """(freqs float64 [rot_dim / 2] in radians per position, amplitude) for rotary().
+
+    Pair i turns by base ** (-2 i / rot_dim) per position.  Contexts `factor` times as long as the trained one:
+      'linear'  every position divided by factor
+      'ntk'     the base raised to base * factor ** (rot_dim / (rot_dim - 2)): the fastest pair stays, the slowest is divided
+      'parts'   interpolated by parts: pairs that make fewer than `low_turns` turns over `original_len` positions are divided
+                by factor, pairs with more than `high_turns` stay, a linear ramp in between; amplitude 0.1 ln(factor) + 1
+    """
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError('rot_dim must be a positive even number; got %r' % (rot_dim,))
+    if not base > 0 or not factor > 0:
+        raise ValueError('base and factor must be positive')
+    if scaling not in (None, 'linear', 'ntk', 'parts'):
+        raise ValueError("scaling must be None, 'linear', 'ntk' or 'parts'; got %r" % (scaling,))
+    if scaling == 'ntk':
+        if rot_dim < 4:
+            raise ValueError("scaling 'ntk' needs rot_dim >= 4")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = torch.tensor([base ** (-i / rot_dim) for i in range(0, rot_dim, 2)], dtype=torch.float64)
+    amplitude = 1.0
+    if scaling == 'linear':
+        f = f / factor
+    elif scaling == 'parts':
+        if original_len is None or original_len < 1 or not high_turns > low_turns:
+            raise ValueError("scaling 'parts' needs original_len and high_turns > low_turns")
+        keep = ((original_len * f / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return f.to(device), amplitude
+
+
+def _rotary_launch(xs, positions, freqs, interleaved, amplitude, inverse):
+    d = _lib.RotaryDesc()
+    xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
+    ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    on = [(x, y) for x, y in zip(xs, ys) if x.numel()]
+    if not on:
+        return ys
+    for i, (x, y) in enumerate(on):
+        d.x[i], d.y[i] = x.data_ptr(), y.data_ptr()
+        d.sB[i], d.sT[i], d.sH[i] = x.stride(0), x.stride(1), x.stride(2)
+        d.H[i], d.M[i], d.sM[i] = (x.shape[2], x.shape[3], x.stride(3)) if x.dim() == 5 else (x.shape[2], 1, 0)
+    x = on[0][0]
+    d.B, d.T, d.D, d.rot = x.shape[0], x.shape[1], x.shape[-1], 2 * freqs.numel()
+    d.freqs, d.pos, d.pos64 = freqs.data_ptr(), positions.data_ptr(), int(positions.dtype == torch.int64)
+    d.pos_sB, d.pos_sT = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    d.interleaved, d.inverse, d.type, d.amplitude = int(interleaved), int(inverse), TYPES[x.dtype], amplitude
+    _launch('mep_rotary', d, x.device)
+    return ys
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, positions, freqs, interleaved, amplitude, *xs):
+        ctx.save_for_backward(positions, freqs)
+        ctx.meta = (interleaved, amplitude)
+        ctx.set_materialize_grads(False)
+        return tuple(_rotary_launch(list(xs), positions, freqs, interleaved, amplitude, False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *gs):
+        positions, freqs = ctx.saved_tensors
+        interleaved, amplitude = ctx.meta
+        on = [i for i, g in enumerate(gs) if g is not None and ctx.needs_input_grad[4 + i]]
+        out = [None] * len(gs)
+        if on:
+            for i, y in zip(on, _rotary_launch([gs[i] for i in on], positions, freqs, interleaved, amplitude, True)):
+                out[i] = y
+        return (None, None, None, None, *out)
+
+
+def rotary(q, k=None, *, positions, freqs, layout='half', amplitude=1.0):
+    """Rotary positions of q, or of q and k in one launch; returns what it was given, contiguous.
+
+    q, k [B, T, heads, D] or [B, T, heads, maps, D] (any strides), of one type; positions int32 / int64 [T] or [B, T];
+    freqs float64 [r / 2] (rotary_frequencies): the first r channels of each head are turned, the rest copied.
+    layout 'half' pairs channels (i, i + r / 2), 'interleaved' pairs (2i, 2i + 1).  The angles are formed in 64 bits.
+    """
+    xs = [q] if k is None else [q, k]
+    _type_of(q, 'q')
+    for x in xs:
+        if x.dim() not in (4, 5) or x.shape[:2] != q.shape[:2] or x.shape[-1] != q.shape[-1] or x.dtype != q.dtype:
+            raise ValueError('q and k must be [batch, time, heads, (maps,) channels] of one type, batch, time and channels; got %s'
+                             % ', '.join('%s %s' % (tuple(x.shape), x.dtype) for x in xs))
+    B, T, D = q.shape[0], q.shape[1], q.shape[-1]
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 1 <= freqs.numel() <= D // 2:
+        raise ValueError('freqs must be contiguous float64 [r / 2] with 2 <= r <= channels; got %s %s' % (tuple(freqs.shape), freqs.dtype))
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((T,), (B, T)):
+        raise ValueError('positions must be int32 or int64 [time] or [batch, time]; got %s %s' % (tuple(positions.shape), positions.dtype))
+    if layout not in ('half', 'interleaved'):
+        raise ValueError("layout must be 'half' or 'interleaved'; got %r" % (layout,))
+    _on_device(q, k, positions, freqs)
+    out = _RotaryFn.apply(positions, freqs, layout == 'interleaved', float(amplitude), *xs)
+    return out[0] if k is None else out
+
+
+# ------------------------------------------------------------------ the norms around a block
+def _rows(t, D):
+    """(2-D row view, row stride) of [..., D]; a copy only where the rows have no common stride"""
+    t = t.reshape(-1, D)
+    if D > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+class _NormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cfg, y, x, w, b, gate, scale, nw, nb):
+        kind, next_kind, gate_form, T, eps, scale_value = cfg
+        D = y.shape[-1]
+        dev = y.device
+        y2, y_ld = _rows(y, D)
+        x2, x_ld = _rows(x, D) if x is not None else (None, 0)
+        g2, g_ld = _rows(gate, D) if gate_form == 3 else (gate.contiguous() if gate is not None else None, 0)
+        w, b, nw, nb = (None if t is None else t.contiguous() for t in (w, b, nw, nb))
+        n = y2.shape[0]
+        stream = torch.empty(y.shape, dtype=y.dtype, device=dev)
+        normed = torch.empty(y.shape, dtype=y.dtype, device=dev) if next_kind else None
+        keep = any(ctx.needs_input_grad)
+        stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if keep else None
+        params = [t for t in (w, b, nw, nb) if t is not None]
+        d = _lib.BlockNormDesc(y=_ptr(y2), x=_ptr(x2), gate=_ptr(g2), w=_ptr(w), b=_ptr(b), nw=_ptr(nw), nb=_ptr(nb),
+                               scale=_ptr(scale), stream=_ptr(stream), normed=_ptr(normed), stats=_ptr(stats), y_ld=y_ld, x_ld=x_ld,
+                               g_ld=g_ld, rows=n, D=D, T=T, kind=kind, next_kind=next_kind, gate_form=gate_form,
+                               type=TYPES[y.dtype], wtype=TYPES[params[0].dtype] if params else 0,
+                               gtype=TYPES[gate.dtype] if gate is not None else 0, eps=eps, scale_value=scale_value)
+        if n:
+            _launch('mep_block_norm_fwd', d, dev)
+        if keep:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(y2, x2, g2, w, b, scale, nw, nb, stats)
+            ctx.shapes = (y.shape, None if gate is None else gate.shape, None if scale is None else scale.shape)
+            # the backward reads the forward's inputs by address, and asks of its results only which there were
+            ctx.desc = d
+        return (stream, normed) if next_kind else stream
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dstream, dnormed=None):
+        y2, x2, g2, w, b, scale, nw, nb, stats = ctx.saved_tensors
+        none = (None,) * 9
+        if dstream is None and dnormed is None:
+            return none
+        need = ctx.needs_input_grad
+        shape, gate_shape, scale_shape = ctx.shapes
+        n, D = y2.shape
+        dev = y2.device
+        d = ctx.desc
+        rows = lambda on: torch.empty(shape, dtype=y2.dtype, device=dev) if on else None  # noqa: E731
+        like = lambda t, on: torch.empty_like(t) if t is not None and on else None  # noqa: E731
+        dy, dx = rows(True), rows(x2 is not None and need[2])
+        dw, db, dgate, dscale, dnw, dnb = (like(t, need[i]) for t, i in ((w, 3), (b, 4), (g2, 5), (scale, 6), (nw, 7), (nb, 8)))
+        if d.gate_form == 3 and dgate is not None:
+            dgate = rows(True)
+        if dnormed is None:    # the second norm took no part
+            for t in (dnw, dnb):
+                if t is not None:
+                    t.zero_()
+        if n == 0:
+            for t in (dw, db, dnw, dnb, dscale, dgate):
+                if t is not None:
+                    t.zero_()
+        else:
+            ds2, ds_ld = _rows(dstream, D) if dstream is not None else (None, 0)
+            dn2, dn_ld = _rows(dnormed, D) if dnormed is not None else (None, 0)
+            sums = [t for t in (dw, db, dnw if dn2 is not None else None, dnb if dn2 is not None else None,
+                                dgate if d.gate_form != 3 else None) if t is not None]
+            partial = None
+            if sums or dscale is not None:
+                p = _lib.lib().mep_block_norm_partial(ctypes.byref(d))
+                if p < 0:
+                    _lib.check(p, 'mep_block_norm_partial')
+                partial = torch.empty(p * (len(sums) * D + 1), dtype=torch.float32, device=dev)
+            bd = _lib.BlockNormBwdDesc(f=d, dstream=_ptr(ds2), dnormed=_ptr(dn2), dy=_ptr(dy), dx=_ptr(dx),
+                                       dgate_rows=_ptr(dgate) if d.gate_form == 3 else 0, dw=_ptr(dw), db=_ptr(db),
+                                       dnw=_ptr(dnw) if dn2 is not None else 0, dnb=_ptr(dnb) if dn2 is not None else 0,
+                                       dgate=_ptr(dgate) if d.gate_form != 3 else 0, dscale=_ptr(dscale),
+                                       partial=_ptr(partial), ds_ld=ds_ld, dn_ld=dn_ld, n_sums=len(sums))
+            _launch('mep_block_norm_bwd', bd, dev)
+        if dgate is not None:
+            dgate = dgate.reshape(gate_shape)
+        if dscale is not None:
+            dscale = dscale.reshape(scale_shape)
+        return (None, dy if need[1] else None, dx, dw, db, dgate, dscale, dnw, dnb)
+
+
+def _affine_ok(w, b, D, what):
+    for t, n in ((w, 'weight'), (b, 'bias')):
+        if t is not None and (tuple(t.shape) != (D,) or t.dtype not in TYPES):
+            raise ValueError('%s%s must be a [%d] tensor of a floating type; got %s %s' % (what, n, D, tuple(t.shape), t.dtype))
+
+
+def norm_residual(y, residual, weight=None, bias=None, *, kind='rms', gate=None, scale=1.0, next_kind='none',
+                  next_weight=None, next_bias=None, eps=1e-6):
+    """stream = scale * residual + gate * N(y) and, with a next_kind, normed = N'(stream), in one pass over the rows.
+
+    y, residual [..., D] of one type, D <= 8192.  kind / next_kind: 'rms', 'layer' (biased variance) or 'none'.  weight, bias,
+    next_weight, next_bias [D] in float32 or y's type (all the same).  gate: None, [D] (learned per channel),
+    [B, D] or [B, 1, D] for y [B, T, D] (one row per sequence), or y's shape; float32 or y's type, y's type for the last.
+    scale: a number, or a one-element float32 tensor that is learned.  Returns stream, or (stream, normed).
+    """
+    _type_of(y, 'y')
+    if y.dim() < 1 or not 1 <= y.shape[-1] <= _lib.BLOCK_NORM_MAX_D:
+        raise ValueError('rows must have 1 to %d channels; got %s' % (_lib.BLOCK_NORM_MAX_D, tuple(y.shape)))
+    D = y.shape[-1]
+    if residual is not None and (residual.shape != y.shape or residual.dtype != y.dtype):
+        raise ValueError('residual must have the shape and type of y; got %s %s' % (tuple(residual.shape), residual.dtype))
+    for k in (kind, next_kind):
+        if k not in KINDS:
+            raise ValueError("kinds are 'rms', 'layer' and 'none'; got %r" % (k,))
+    if (kind == 'none' and (weight is not None or bias is not None)) or \
+            (next_kind == 'none' and (next_weight is not None or next_bias is not None)):
+        raise ValueError("a norm of kind 'none' has no weight and no bias")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError('eps must be finite and not negative; got %r' % (eps,))
+    _affine_ok(weight, bias, D, '')
+    _affine_ok(next_weight, next_bias, D, 'next_')
+    types = {t.dtype for t in (weight, bias, next_weight, next_bias) if t is not None}
+    if len(types) > 1 or not types <= {torch.float32, y.dtype}:
+        raise ValueError('weights and biases must all be float32 or all of the type of y')
+    form, T = 0, 1
+    if gate is not None:
+        if gate.dtype not in (torch.float32, y.dtype):
+            raise ValueError('gate must be float32 or of the type of y; got %s' % gate.dtype)
+        per_seq = y.dim() == 3 and tuple(gate.shape) in ((y.shape[0], D), (y.shape[0], 1, D))
+        if gate.shape == y.shape and gate.dtype == y.dtype:
+            form = 3
+        elif tuple(gate.shape) == (D,):
+            form = 1
+        elif per_seq and y.shape[0] <= 65000:
+            form, T = 2, max(1, y.shape[1])
+        else:
+            raise ValueError('gate must be [D], [B, D] or [B, 1, D] for y [B, T, D] with B <= 65000, or of the shape and type of y; '
+                             'got %s %s for %s' % (tuple(gate.shape), gate.dtype, tuple(y.shape)))
+    st, sv = None, 1.0
+    if torch.is_tensor(scale):
+        if scale.numel() != 1 or scale.dtype != torch.float32:
+            raise ValueError('a learned scale is a one-element float32 tensor; got %s %s' % (tuple(scale.shape), scale.dtype))
+        st = scale
+    else:
+        sv = float(scale)
+    _on_device(y, residual, weight, bias, gate, next_weight, next_bias, st)
+    cfg = (KINDS[kind], KINDS[next_kind], form, T, float(eps), sv)
+    return _NormFn.apply(cfg, y, residual, weight, bias, gate, st, next_weight, next_bias)
+
+
+def norm(x, weight=None, bias=None, *, kind='rms', eps=1e-6):
+    """N(x) over the last dimension: the norm before a block, or of each head's row.  As norm_residual without its residual."""
+    if kind not in ('rms', 'layer'):
+        raise ValueError("kind must be 'rms' or 'layer'; got %r" % (kind,))
+    return norm_residual(x, None, weight, bias, kind=kind, eps=eps)
