@@ -772,6 +772,41 @@ int mep_block_norm_bwd(const mep_block_norm_bwd_desc* desc, mep_stream_t stream)
 /* rows of the backward's workspace for this forward descriptor, or MEP_EINVAL */
 int mep_block_norm_partial(const mep_block_norm_desc* desc);
 
+/* Differential attention: out = (A_1 - lam A_2) v, A_m = softmax over the allowed keys of scale q_m k_m^T.
+ * q [B, Tq, H, 2, d], k [B, Tk, G, 2, d], v [B, Tk, G, dv] (strides given, channels contiguous), head h reads key head
+ * h / (H / G); lam fp32 by strides (0: shared).  A key is allowed when it is below lengths[b] (int32; 0 = Tk), when causal
+ * at most q_start[b] + query (int32; 0 = Tk - Tq), and when the mask holds a value other than 0 for it (mask_form 1: [B, Tk],
+ * 2: [B, Tq, Tk]).  A row without an allowed key is 0 and gives no gradient.  Keys past the lengths, past every query's
+ * causal reach, and of a zero in a form-1 mask never enter a result, whatever they hold. */
+#define MEP_DIFF_ATTN_MAX_D 128
+#define MEP_DIFF_ATTN_MAX_DV 256
+typedef struct {
+    uint64_t q, k, v, lam;
+    uint64_t out;                /* [B, Tq, H, dv] contiguous                                     */
+    uint64_t stats;              /* fp32 [B, H, Tq, 4], what the backward needs, or 0             */
+    int64_t  q_sB, q_sT, q_sH, q_sM, k_sB, k_sT, k_sH, k_sM, v_sB, v_sT, v_sH;
+    int64_t  lam_sB, lam_sT, lam_sH;
+    uint64_t mask;               /* bytes, or fp32 when mask_float                                */
+    int64_t  m_sB, m_sQ, m_sK;
+    uint64_t lengths, q_start;
+    int32_t  B, Tq, Tk, H, G, d, dv, type;
+    int32_t  causal, mask_form, mask_float;
+    float    scale;
+    int32_t  vec;                /* set by the library                                            */
+    int32_t  _pad;
+} mep_diff_attn_desc;
+typedef struct {
+    mep_diff_attn_desc f;
+    uint64_t dout;               /* [B, Tq, H, dv] by strides                                     */
+    int64_t  o_sB, o_sT, o_sH;
+    uint64_t dq, dk, dv;         /* contiguous, as q, k, v; dq may be 0, dk and dv both           */
+    uint64_t dlam;               /* fp32 [H] for a lam shared by batch and queries, or 0          */
+    uint64_t dlam_rows;          /* fp32 [B, Tq, H], or 0                                         */
+    uint64_t delta;              /* workspace, fp32 [B, H, Tq, 2]                                 */
+} mep_diff_attn_bwd_desc;
+int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t stream);
+int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_t stream);
+
 /* ---------------------------------------------------------------- misc */
 int mep_abi_version(void);
 int mep_last_error(char* buf, size_t len);

@@ -287,6 +287,22 @@ class BlockNormBwdDesc(ctypes.Structure):
                 ('ds_ld', i64), ('dn_ld', i64), ('n_sums', i32), ('_pad', i32)]
 
 
+class DiffAttnDesc(ctypes.Structure):
+    _fields_ = [('q', u64), ('k', u64), ('v', u64), ('lam', u64), ('out', u64), ('stats', u64),
+                ('q_sB', i64), ('q_sT', i64), ('q_sH', i64), ('q_sM', i64), ('k_sB', i64), ('k_sT', i64), ('k_sH', i64),
+                ('k_sM', i64), ('v_sB', i64), ('v_sT', i64), ('v_sH', i64), ('lam_sB', i64), ('lam_sT', i64), ('lam_sH', i64),
+                ('mask', u64), ('m_sB', i64), ('m_sQ', i64), ('m_sK', i64), ('lengths', u64), ('q_start', u64),
+                ('B', i32), ('Tq', i32), ('Tk', i32), ('H', i32), ('G', i32), ('d', i32), ('dv', i32), ('type', i32),
+                ('causal', i32), ('mask_form', i32), ('mask_float', i32), ('scale', f32), ('vec', i32), ('_pad', i32)]
+
+
+class DiffAttnBwdDesc(ctypes.Structure):
+    _fields_ = [('f', DiffAttnDesc), ('dout', u64), ('o_sB', i64), ('o_sT', i64), ('o_sH', i64), ('dq', u64), ('dk', u64),
+                ('dv', u64), ('dlam', u64), ('dlam_rows', u64), ('delta', u64)]
+
+
+DIFF_ATTN_MAX_D, DIFF_ATTN_MAX_DV = 128, 256   # MEP_DIFF_ATTN_MAX_*
+
 STRUCTS = {'mep_rows': Rows, 'mep_gemm_desc': GemmDesc, 'mep_gemm_sum_desc': GemmSumDesc, 'mep_wgrad_desc': WgradDesc,
            'mep_attn_desc': AttnDesc, 'mep_attn_bwd_desc': AttnBwdDesc, 'mep_attn_gen_desc': AttnGenDesc,
            'mep_attn_gen_bwd_desc': AttnGenBwdDesc, 'mep_epi_desc': EpiDesc,
@@ -295,7 +311,8 @@ STRUCTS = {'mep_rows': Rows, 'mep_gemm_desc': GemmDesc, 'mep_gemm_sum_desc': Gem
            'mep_rf_epi_desc': RfEpiDesc, 'mep_rf_epi_bwd_desc': RfEpiBwdDesc, 'mep_rf_head_desc': RfHeadDesc,
            'mep_sweep_desc': SweepDesc, 'mep_window_desc': WindowDesc, 'mep_wsplit_desc': WsplitDesc,
            'mep_rotary_desc': RotaryDesc, 'mep_block_norm_desc': BlockNormDesc,
-           'mep_block_norm_bwd_desc': BlockNormBwdDesc}
+           'mep_block_norm_bwd_desc': BlockNormBwdDesc, 'mep_diff_attn_desc': DiffAttnDesc,
+           'mep_diff_attn_bwd_desc': DiffAttnBwdDesc}
 
 P = ctypes.c_void_p
 # name -> argtypes (all return int)
@@ -327,6 +344,8 @@ SIGNATURES.update({
     'mep_threshold_sweep': [ctypes.POINTER(SweepDesc), P],
     'mep_assemble_windows': [ctypes.POINTER(WindowDesc), i32, P],
     'mep_tgemm': [P, i32, i32, i32, i32, P],
+    'mep_diff_attn_fwd': [ctypes.POINTER(DiffAttnDesc), P],
+    'mep_diff_attn_bwd': [ctypes.POINTER(DiffAttnBwdDesc), P],
     'mep_rotary': [ctypes.POINTER(RotaryDesc), P],
     'mep_block_norm_fwd': [ctypes.POINTER(BlockNormDesc), P],
     'mep_block_norm_bwd': [ctypes.POINTER(BlockNormBwdDesc), P],

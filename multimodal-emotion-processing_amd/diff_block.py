@@ -306,3 +306,102 @@ def norm(x, weight=None, bias=None, *, kind='rms', eps=1e-6):
     if kind not in ('rms', 'layer'):
         raise ValueError("kind must be 'rms' or 'layer'; got %r" % (kind,))
     return norm_residual(x, None, weight, bias, kind=kind, eps=eps)
+
+
+# ------------------------------------------------------------------ differential attention
+class _DiffAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cfg, mask, lengths, q_start, q, k, v, lam):
+        causal, scale = cfg
+        q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+        B, Tq, H, _, hd = q.shape
+        Tk, G, dv = k.shape[1], k.shape[2], v.shape[3]
+        dev = q.device
+        out = torch.empty(B, Tq, H, dv, dtype=q.dtype, device=dev)
+        keep = any(ctx.needs_input_grad)
+        stats = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev) if keep else None
+        ls = (0, 0, lam.stride(0)) if lam.dim() == 1 else lam.stride()
+        m = (0, 0, 0)
+        if mask is not None:
+            m = (mask.stride(0), 0, mask.stride(1)) if mask.dim() == 2 else mask.stride()
+        d = _lib.DiffAttnDesc(q=_ptr(q), k=_ptr(k), v=_ptr(v), lam=_ptr(lam), out=_ptr(out), stats=_ptr(stats),
+                              q_sB=q.stride(0), q_sT=q.stride(1), q_sH=q.stride(2), q_sM=q.stride(3),
+                              k_sB=k.stride(0), k_sT=k.stride(1), k_sH=k.stride(2), k_sM=k.stride(3),
+                              v_sB=v.stride(0), v_sT=v.stride(1), v_sH=v.stride(2), lam_sB=ls[0], lam_sT=ls[1], lam_sH=ls[2],
+                              mask=_ptr(mask), m_sB=m[0], m_sQ=m[1], m_sK=m[2], lengths=_ptr(lengths), q_start=_ptr(q_start),
+                              B=B, Tq=Tq, Tk=Tk, H=H, G=G, d=hd, dv=dv, type=TYPES[q.dtype], causal=int(causal),
+                              mask_form=0 if mask is None else mask.dim() - 1,
+                              mask_float=int(mask is not None and mask.dtype == torch.float32), scale=scale)
+        _launch('mep_diff_attn_fwd', d, dev)
+        if keep:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(mask, lengths, q_start, q, k, v, lam, stats)
+            ctx.desc = d
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        if dout is None:
+            return (None,) * 8
+        mask, lengths, q_start, q, k, v, lam, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if dout.stride(-1) != 1:
+            dout = dout.contiguous()
+        B, Tq, H, _, _ = q.shape
+        dev = q.device
+        like = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
+        dq = like(q) if need[4] else None
+        dk, dv = (like(k), like(v)) if need[5] or need[6] else (None, None)
+        dlam = like(lam) if need[7] else None
+        delta = torch.empty(B, H, Tq, 2, dtype=torch.float32, device=dev)
+        shared = lam.dim() == 1
+        bd = _lib.DiffAttnBwdDesc(f=ctx.desc, dout=_ptr(dout), o_sB=dout.stride(0), o_sT=dout.stride(1), o_sH=dout.stride(2),
+                                  dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlam=_ptr(dlam) if shared else 0,
+                                  dlam_rows=0 if shared else _ptr(dlam), delta=_ptr(delta))
+        _launch('mep_diff_attn_bwd', bd, dev)
+        return (None, None, None, None, dq, dk if need[5] else None, dv if need[6] else None, dlam)
+
+
+def diff_attention(q, k, v, lam, *, mask=None, lengths=None, causal=False, q_start=None, scale=None):
+    """The difference of two softmax maps, applied to the values: out = (A_1 - lam A_2) v [B, Tq, H, dv], with
+    A_m = softmax(scale q_m k_m^T) over the keys that a query may see; a query that sees none gives zeros.
+
+    q [B, Tq, H, 2, d], k [B, Tk, G, 2, d], v [B, Tk, G, dv] (any strides) of one type, d <= 128, dv <= 256; H a multiple of G:
+    head h reads key head h // (H // G).  lam float32 [H] (learned per head) or [B, Tq, H] (per query).  scale: 1 / sqrt(d).
+    What a query sees:
+      mask      [B, Tk] or [B, Tq, Tk], bool, uint8 or float32: nonzero keeps a key (the loaders' masks of ones and zeros)
+      lengths   int32 [B]: the keys at and behind it are not there (a padded batch, a cache)
+      causal    query t of row b sees the keys up to q_start[b] + t; q_start int32 [B], Tk - Tq without it
+    Keys past the lengths, past every query's causal reach or of a zero in a [B, Tk] mask never enter a result, whatever they
+    hold; the keys that only some queries may see must be finite.
+    """
+    _type_of(q, 'q')
+    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4 or q.shape[3] != 2 or k.shape[3] != 2 or q.shape[4] != k.shape[4] or \
+            not q.shape[0] == k.shape[0] == v.shape[0] or k.shape[1:3] != v.shape[1:3]:
+        raise ValueError('q, k, v must be [B, Tq, H, 2, d], [B, Tk, G, 2, d], [B, Tk, G, dv]; got %s, %s, %s'
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    B, Tq, H, _, hd = q.shape
+    Tk, G, dv = k.shape[1], k.shape[2], v.shape[3]
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('q, k and v must be of one type; got %s, %s, %s' % (q.dtype, k.dtype, v.dtype))
+    if not 1 <= hd <= _lib.DIFF_ATTN_MAX_D or not 1 <= dv <= _lib.DIFF_ATTN_MAX_DV:
+        raise ValueError('head widths up to %d (q, k) and %d (v); got %d and %d'
+                         % (_lib.DIFF_ATTN_MAX_D, _lib.DIFF_ATTN_MAX_DV, hd, dv))
+    if G < 1 or H < 1 or H % G:
+        raise ValueError('the query heads must be a multiple of the key heads; got %d and %d' % (H, G))
+    if lam.dtype != torch.float32 or tuple(lam.shape) not in ((H,), (B, Tq, H)):
+        raise ValueError('lam must be float32 [H] or [B, Tq, H]; got %s %s' % (tuple(lam.shape), lam.dtype))
+    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8, torch.float32) or
+                             tuple(mask.shape) not in ((B, Tk), (B, Tq, Tk))):
+        raise ValueError('mask must be bool, uint8 or float32 [B, Tk] or [B, Tq, Tk]; got %s %s' % (tuple(mask.shape), mask.dtype))
+    for t, n in ((lengths, 'lengths'), (q_start, 'q_start')):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+            raise ValueError('%s must be contiguous int32 [B]; got %s %s' % (n, tuple(t.shape), t.dtype))
+    if q_start is not None and not causal:
+        raise ValueError('q_start places the queries of a causal call; causal is False')
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e6:
+        raise ValueError('scale must be positive and at most 1e6; got %r' % (scale,))
+    _on_device(q, k, v, lam, mask, lengths, q_start)
+    return _DiffAttnFn.apply((bool(causal), scale), mask, lengths, q_start, q, k, v, lam)
