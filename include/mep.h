@@ -777,13 +777,17 @@ int mep_block_norm_partial(const mep_block_norm_desc* desc);
  * h / (H / G); lam fp32 by strides (0: shared).  A key is allowed when it is below lengths[b] (int32; 0 = Tk), when causal
  * at most q_start[b] + query (int32; 0 = Tk - Tq), and when the mask holds a value other than 0 for it (mask_form 1: [B, Tk],
  * 2: [B, Tq, Tk]).  A row without an allowed key is 0 and gives no gradient.  Keys past the lengths, past every query's
- * causal reach, and of a zero in a form-1 mask never enter a result, whatever they hold. */
+ * causal reach, and of a zero in a form-1 mask never enter a result, whatever they hold.
+ * q, k, v and dout are read 16 bytes at a time: their bases and strides are multiples of that, their rows hold zeros from d
+ * (dv) to the next multiple, and 64 time steps with all heads of a key head span under 2^30 elements; mep_pack_rows makes such rows
+ * of any others.  MEP_EINVAL otherwise. */
 #define MEP_DIFF_ATTN_MAX_D 128
 #define MEP_DIFF_ATTN_MAX_DV 256
 typedef struct {
     uint64_t q, k, v, lam;
     uint64_t out;                /* [B, Tq, H, dv] contiguous                                     */
-    uint64_t stats;              /* fp32 [B, H, Tq, 4], what the backward needs, or 0             */
+    uint64_t stats;              /* fp32 [B, H, Tq, 4] (max, 1 / sum of each map), for the backward, or 0 */
+    uint64_t second;             /* [B, Tq, H, dv] A_2 v, rounded to the type, with stats         */
     int64_t  q_sB, q_sT, q_sH, q_sM, k_sB, k_sT, k_sH, k_sM, v_sB, v_sT, v_sH;
     int64_t  lam_sB, lam_sT, lam_sH;
     uint64_t mask;               /* bytes, or fp32 when mask_float                                */
@@ -792,8 +796,6 @@ typedef struct {
     int32_t  B, Tq, Tk, H, G, d, dv, type;
     int32_t  causal, mask_form, mask_float;
     float    scale;
-    int32_t  vec;                /* set by the library                                            */
-    int32_t  _pad;
 } mep_diff_attn_desc;
 typedef struct {
     mep_diff_attn_desc f;
@@ -802,9 +804,16 @@ typedef struct {
     uint64_t dq, dk, dv;         /* contiguous, as q, k, v; dq may be 0, dk and dv both           */
     uint64_t dlam;               /* fp32 [H] for a lam shared by batch and queries, or 0          */
     uint64_t dlam_rows;          /* fp32 [B, Tq, H], or 0                                         */
-    uint64_t delta;              /* workspace, fp32 [B, H, Tq, 2]                                 */
+    uint64_t delta;              /* workspace, fp32 [B, H, Tq, 4]                                 */
 } mep_diff_attn_bwd_desc;
 int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t stream);
+/* y [B, T, H, M, n rounded up to 16 bytes] = x [B, T, H, M, n] of any strides (sN: of the channels), zeros behind n */
+typedef struct {
+    uint64_t x, y;
+    int64_t  sB, sT, sH, sM, sN;
+    int32_t  B, T, H, M, n, type;
+} mep_pack_rows_desc;
+int mep_pack_rows(const mep_pack_rows_desc* desc, mep_stream_t stream);
 int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_t stream);
 
 /* ---------------------------------------------------------------- misc */

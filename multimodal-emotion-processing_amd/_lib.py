@@ -288,17 +288,22 @@ class BlockNormBwdDesc(ctypes.Structure):
 
 
 class DiffAttnDesc(ctypes.Structure):
-    _fields_ = [('q', u64), ('k', u64), ('v', u64), ('lam', u64), ('out', u64), ('stats', u64),
+    _fields_ = [('q', u64), ('k', u64), ('v', u64), ('lam', u64), ('out', u64), ('stats', u64), ('second', u64),
                 ('q_sB', i64), ('q_sT', i64), ('q_sH', i64), ('q_sM', i64), ('k_sB', i64), ('k_sT', i64), ('k_sH', i64),
                 ('k_sM', i64), ('v_sB', i64), ('v_sT', i64), ('v_sH', i64), ('lam_sB', i64), ('lam_sT', i64), ('lam_sH', i64),
                 ('mask', u64), ('m_sB', i64), ('m_sQ', i64), ('m_sK', i64), ('lengths', u64), ('q_start', u64),
                 ('B', i32), ('Tq', i32), ('Tk', i32), ('H', i32), ('G', i32), ('d', i32), ('dv', i32), ('type', i32),
-                ('causal', i32), ('mask_form', i32), ('mask_float', i32), ('scale', f32), ('vec', i32), ('_pad', i32)]
+                ('causal', i32), ('mask_form', i32), ('mask_float', i32), ('scale', f32)]
 
 
 class DiffAttnBwdDesc(ctypes.Structure):
     _fields_ = [('f', DiffAttnDesc), ('dout', u64), ('o_sB', i64), ('o_sT', i64), ('o_sH', i64), ('dq', u64), ('dk', u64),
                 ('dv', u64), ('dlam', u64), ('dlam_rows', u64), ('delta', u64)]
+
+
+class PackRowsDesc(ctypes.Structure):
+    _fields_ = [('x', u64), ('y', u64), ('sB', i64), ('sT', i64), ('sH', i64), ('sM', i64), ('sN', i64),
+                ('B', i32), ('T', i32), ('H', i32), ('M', i32), ('n', i32), ('type', i32)]
 
 
 DIFF_ATTN_MAX_D, DIFF_ATTN_MAX_DV = 128, 256   # MEP_DIFF_ATTN_MAX_*
@@ -312,7 +317,7 @@ STRUCTS = {'mep_rows': Rows, 'mep_gemm_desc': GemmDesc, 'mep_gemm_sum_desc': Gem
            'mep_sweep_desc': SweepDesc, 'mep_window_desc': WindowDesc, 'mep_wsplit_desc': WsplitDesc,
            'mep_rotary_desc': RotaryDesc, 'mep_block_norm_desc': BlockNormDesc,
            'mep_block_norm_bwd_desc': BlockNormBwdDesc, 'mep_diff_attn_desc': DiffAttnDesc,
-           'mep_diff_attn_bwd_desc': DiffAttnBwdDesc}
+           'mep_diff_attn_bwd_desc': DiffAttnBwdDesc, 'mep_pack_rows_desc': PackRowsDesc}
 
 P = ctypes.c_void_p
 # name -> argtypes (all return int)
@@ -346,6 +351,7 @@ SIGNATURES.update({
     'mep_tgemm': [P, i32, i32, i32, i32, P],
     'mep_diff_attn_fwd': [ctypes.POINTER(DiffAttnDesc), P],
     'mep_diff_attn_bwd': [ctypes.POINTER(DiffAttnBwdDesc), P],
+    'mep_pack_rows': [ctypes.POINTER(PackRowsDesc), P],
     'mep_rotary': [ctypes.POINTER(RotaryDesc), P],
     'mep_block_norm_fwd': [ctypes.POINTER(BlockNormDesc), P],
     'mep_block_norm_bwd': [ctypes.POINTER(BlockNormBwdDesc), P],

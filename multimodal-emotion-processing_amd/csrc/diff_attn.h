@@ -1,0 +1,867 @@
+// Differential attention on the matrix cores (instantiated per element type in diff_attn_*.hip, entry points in diff_attn.hip).
+// With s_m = scale q_m k_m^T over the allowed keys (m = 1, 2),
+//   A_m = softmax(s_m) (a row without an allowed key: zeros),  P = A_1 - lam A_2,  out = P v
+// and backward with dP = dO v^T, D_m = sum_k A_m dP = dO . (A_m v):
+//   dS_1 = A_1 (dP - D_1), dS_2 = -lam A_2 (dP - D_2), dq_m = scale dS_m k_m, dk_m = scale dS_m^T q_m, dv = P^T dO, dlam = -D_2.
+//
+// The rows of a (batch, key head) are its Tq queries times the H / G heads that share the key head, query-major: row r is
+// query r / n of head n * g + r % n, so shared heads read one copy of the keys and their gradients are summed in registers.
+//
+// The difference is formed before anything is rounded to 16 bits: two nearly equal maps cancel, and rounding each of them
+// first would leave an error of 2^-9 of the parts in a difference of a few hundredths.  See k_diff_fwd for how one pass over the
+// keys does that.  Scores, statistics and accumulators are fp32; P and dS are rounded once, as operands of the second products.
+//
+// Products on v_mfma_f32_32x32x16 (fp32: 32x32x2).  Scores are formed transposed (keys x rows): a lane holds one row and 16
+// keys, the row statistics are lane-local, and the accumulator registers are the second product's operand as they are
+// when its sum runs over the keys in the order {4h .. 4h+3, 8+4h .. 8+4h+3} of lane half h; the other operand (V^T, K^T, Q^T,
+// dO^T) is read transposed from LDS by ds_read_b64_tr_b16 in that order.
+//
+// Tiles of 64 keys (32 in fp32) go to LDS by DMA, 16 bytes a lane, one tile ahead of the products, and are stored as 16-byte chunks
+// whose place in the row is xor-ed with the row (Lay): both kinds of reads touch every bank equally often.
+#pragma once
+#include <climits>
+#include <type_traits>
+
+#include "elem.h"
+
+namespace mep {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int DA_THREADS = 256, DA_WAVES = 4, DA_ROWS = 32 * DA_WAVES;
+constexpr float DA_LOG2E = 1.4426950408889634f;
+constexpr float DA_MIN = -1.0e30f;      // the running maximum's start: finite, so that masked scores (-inf) give 2^-inf = 0
+constexpr unsigned DA_NOWHERE = 0x80000000u, DA_SPAN = 0x7fffffffu;   // a DMA offset behind the span reads zeros
+enum { DA_FWD, DA_BWD_Q, DA_BWD_KV };
+
+// One 16-byte operand of a lane: E consecutive k of a 2 E step
+template <int TYPE> struct Mat;
+template <> struct Mat<MEP_BF16> {
+    typedef __bf16 T;
+    typedef __bf16 Frag __attribute__((ext_vector_type(8)));
+    static constexpr int KS = 16, E = 8;
+    static MEP_DEV floatx16 mma(Frag a, Frag b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<MEP_F16> {
+    typedef _Float16 T;
+    typedef _Float16 Frag __attribute__((ext_vector_type(8)));
+    static constexpr int KS = 16, E = 8;
+    static MEP_DEV floatx16 mma(Frag a, Frag b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<MEP_F32> {
+    typedef float T;
+    typedef f32x4 Frag;
+    static constexpr int KS = 8, E = 4;
+    static MEP_DEV floatx16 mma(Frag a, Frag b, floatx16 c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = mfma32(a[j], b[j], c);
+        return c;
+    }
+};
+
+// A tile of rows of COLS elements in LDS: chunk c (16 bytes) of row r lies at place c ^ sw(r) of the row.  sw differs over any
+// 8 consecutive rows (first-product operands: the same chunk of 32 rows), and in pairs over any 4 (transposed reads:
+// 2 neighbouring chunks of 4 rows).  Rows of 4 chunks share 128 bytes with their neighbour.
+template <class M, int COLS>
+struct Lay {
+    static constexpr int CH = COLS / M::E;
+    static_assert(CH == 4 || CH % 8 == 0, "row width");
+    static MEP_DEV int sw(int r) { return CH >= 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1); }
+    static MEP_DEV int at(int r, int c) { return (r * CH + (c ^ sw(r))) * M::E; }
+};
+
+// Geometry of an instance: head widths padded to DK (each map) and DV
+template <int TYPE, int DK, int DV>
+struct Geo {
+    typedef Mat<TYPE> M;
+    typedef typename M::T T;
+    typedef typename M::Frag Frag;
+    static constexpr int KT = TYPE == MEP_F32 ? 32 : 64;      // keys (or rows) of a staged tile
+    static constexpr int NK = DK / M::KS, NV = DV / M::KS;    // operands along the head widths
+    static constexpr int NP = 32 / M::KS;                     // operands of 32 keys
+    static constexpr int KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;      // elements of a tile's keys, and of a tile
+    static constexpr int OUT = DA_ROWS * ((DK > DV ? DK : DV) + M::E);  // the results pass through the tiles
+    static constexpr int BUF = 2 * TSZ > OUT ? 2 * TSZ : OUT;
+};
+
+template <class M>
+MEP_DEV typename M::Frag zero_frag() {
+    typename M::Frag f;
+#pragma unroll
+    for (int j = 0; j < M::E; ++j) f[j] = (typename M::T)0.f;
+    return f;
+}
+
+// E elements at column c of a row of n (rows are padded to whole operands with zeros)
+template <class M>
+MEP_DEV typename M::Frag row_frag(const MEP_G typename M::T* row, int c, int n, bool live) {
+    return live && c < n ? *reinterpret_cast<const MEP_G typename M::Frag*>(row + c) : zero_frag<M>();
+}
+
+typedef __attribute__((address_space(3))) void da_lds_void;
+
+// ROWS x COLS of LDS from rows of global memory, by DMA.  where(r, c, off): whether chunk c of tile row r is there, at element
+// base + off; zeros otherwise.  Masked rows are never loaded: their contents, NaN too, never enter a product.
+template <class M, int ROWS, int COLS, class F>
+MEP_DEV void stage(typename M::T* dst, const MEP_G typename M::T* base, F where) {
+    typedef Lay<M, COLS> L;
+    constexpr int N = ROWS * L::CH / 64;                 // images of 64 chunks, one instruction of a wave each
+    static_assert(N * 64 == ROWS * L::CH && N % DA_WAVES == 0, "tile");
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, DA_SPAN, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < N / DA_WAVES; ++i) {
+        const int img = i * DA_WAVES + wave, pos = img * 64 + lane, r = pos / L::CH, c = (pos % L::CH) ^ L::sw(r);
+        unsigned off;
+        const bool on = where(r, c, off);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (da_lds_void*)(dst + img * 64 * M::E), 16,
+                                                 on ? off * (unsigned)sizeof(typename M::T) : DA_NOWHERE, 0, 0, 0);
+    }
+}
+
+// every wave's DMA and LDS accesses done, then the workgroup barrier
+MEP_DEV void tile_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// first-product operand i: row r0 + (lane & 31), chunk c0 + 2 i + h
+template <class M, int COLS>
+MEP_DEV typename M::Frag lds_frag(const typename M::T* tile, int r0, int c0, int i) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const typename M::Frag*>(tile + Lay<M, COLS>::at(r0 + (lane & 31), c0 + 2 * i + (lane >> 5)));
+}
+
+// second-product operand: column col0 + (lane & 31) of the tile, rows r0 + KS i .. in accumulator order
+template <class M, int COLS>
+MEP_DEV typename M::Frag lds_frag_t(const typename M::T* tile, int r0, int col0, int i) {
+    typedef Lay<M, COLS> L;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (M::KS == 8) {
+        typename M::Frag f;
+        const int col = col0 + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = tile[L::at(r0 + 8 * i + 4 * h + j, col / M::E) + col % M::E];
+        return f;
+    } else {
+        // the 16 lanes of a group read 4 rows x 16 columns and get a column's 4 rows each
+        const int r = r0 + 16 * i + 4 * h + ((lane & 15) >> 2), c = (col0 + (lane & 16)) / M::E + ((lane & 3) >> 1);
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + L::at(r, c) + 4 * (lane & 1)));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + L::at(r + 8, c) + 4 * (lane & 1)));
+        return __builtin_bit_cast(typename M::Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+// an accumulator tile as operand i of the next product, rounded to the tensors' type
+template <class M>
+MEP_DEV typename M::Frag acc_frag(const floatx16& p, int i) {
+    typename M::Frag f;
+#pragma unroll
+    for (int j = 0; j < M::E; ++j) f[j] = (typename M::T)p[M::E * i + j];
+    return f;
+}
+
+MEP_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// v over both lane halves of a row: lo and hi, each in every lane
+MEP_DEV void both_halves(float v, float& lo, float& hi) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned a = r[0], b = r[1];
+    lo = __builtin_bit_cast(float, a);
+    hi = __builtin_bit_cast(float, b);
+}
+MEP_DEV float half_sum(float v) {
+    float lo, hi;
+    both_halves(v, lo, hi);
+    return lo + hi;
+}
+MEP_DEV float half_max(float v) {
+    float lo, hi;
+    both_halves(v, lo, hi);
+    return fmaxf(lo, hi);
+}
+MEP_DEV float max16(const floatx16& s) {
+    float m = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) m = fmaxf(m, s[r]);
+    return m;
+}
+
+// what a workgroup works on, and its keys
+struct Job {
+    int b, g, block, n;          // batch row, key head, block of rows or keys, heads per key head
+    int rows, len, first;        // Tq n; allowed keys are below len; causal: key <= first + query
+};
+// Workgroups go round the 8 XCDs by their index; where the (batch, key head) pairs divide evenly over them, a pair's blocks
+// stay on one XCD (or on a few, in turn), so that its keys are read into one L2.
+MEP_DEV Job make_job(const mep_diff_attn_desc& d, int blocks, bool reverse) {
+    Job j;
+    const int x = blockIdx.x, bgs = d.B * d.G;
+    int bg;
+    if (bgs % 8 == 0) {
+        const int s = x >> 3, q = s / blocks;
+        bg = q * 8 + (x & 7);
+        j.block = s - q * blocks;
+    } else if (8 % bgs == 0 && blocks % (8 / bgs) == 0) {
+        const int per = 8 / bgs;
+        bg = (x & 7) / per;
+        j.block = (x >> 3) * per + (x & 7) % per;
+    } else {
+        bg = x / blocks;
+        j.block = x - bg * blocks;
+    }
+    if (reverse) j.block = blocks - 1 - j.block;      // causal: the longest blocks start first
+    j.b = bg / d.G;
+    j.g = bg - j.b * d.G;
+    j.n = d.H / d.G;
+    j.rows = d.Tq * j.n;
+    j.len = d.Tk;
+    if (d.lengths) j.len = max(0, min(j.len, G<const int>(d.lengths)[j.b]));
+    j.first = d.Tk - d.Tq;
+    if (d.q_start) j.first = max(-(1 << 30), min(1 << 30, G<const int>(d.q_start)[j.b]));
+    if (d.causal) j.len = max(0, min(j.len, j.first + d.Tq));     // what no query sees is never read
+    return j;
+}
+// keys that any of the queries up to t may see
+MEP_DEV int key_end(const mep_diff_attn_desc& d, const Job& j, int t) {
+    return d.causal ? max(0, min(j.len, j.first + t + 1)) : j.len;
+}
+
+MEP_DEV bool mask_at(const mep_diff_attn_desc& d, int64_t o) {
+    return d.mask_float ? G<const float>(d.mask)[o] != 0.f : G<const uint8_t>(d.mask)[o] != 0;
+}
+// The [B, Tk] mask's value for key k0 + lane, as it lies in memory (loaded a tile ahead of its use), and the tile's key bits:
+// bit i: key k0 + i is there and not masked for every query
+MEP_DEV unsigned key_raw(const mep_diff_attn_desc& d, const Job& j, int k0) {
+    const int k = k0 + (int)(threadIdx.x & 63);
+    if (d.mask_form != 1 || k >= j.len) return 2u;
+    const int64_t o = (int64_t)j.b * d.m_sB + (int64_t)k * d.m_sK;
+    return d.mask_float ? G<const uint32_t>(d.mask)[o] : (unsigned)G<const uint8_t>(d.mask)[o];
+}
+MEP_DEV unsigned long long key_bits(const mep_diff_attn_desc& d, const Job& j, int k0, int n, unsigned raw) {
+    const int i = threadIdx.x & 63;
+    return __ballot(i < n && k0 + i < j.len && (d.mask_float ? raw << 1 : raw) != 0);      // -0.0 is zero
+}
+// a tile position in accumulator order: acc_row(r, lane) = acc_off(r) + 4 h
+MEP_DEV constexpr int acc_off(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// scores of keys k0 .. k0 + 31 (rows of the accumulator) against this lane's query t: masked ones to -inf
+MEP_DEV void mask_keys(const mep_diff_attn_desc& d, const Job& j, int k0, unsigned bits, int t, floatx16& s1, floatx16& s2) {
+    const int h = (threadIdx.x & 63) >> 5;
+    unsigned on = bits >> (4 * h);
+    if (d.causal) {      // keys up to first + t
+        const int last = j.first + t - k0 - 4 * h;
+        on &= last < 0 ? 0u : last > 30 ? ~0u : (2u << last) - 1u;
+    }
+    if (d.mask_form == 2) {      // all 16 at once; keys past the end read the last one's
+        const int64_t o = (int64_t)j.b * d.m_sB + (int64_t)t * d.m_sQ;
+        unsigned keep = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            keep |= (mask_at(d, o + (int64_t)min(k0 + 4 * h + acc_off(r), d.Tk - 1) * d.m_sK) ? 1u : 0u) << acc_off(r);
+        on &= keep;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const bool ok = on >> acc_off(r) & 1;
+        s1[r] = ok ? s1[r] : -INFINITY;
+        s2[r] = ok ? s2[r] : -INFINITY;
+    }
+}
+
+// The keys and values of a (batch, key head), tile by tile
+template <int TYPE, int DK, int DV>
+struct KeyTiles {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef typename Ge::M M;
+    typedef typename Ge::T T;
+    const mep_diff_attn_desc& d;
+    const MEP_G T* kp;
+    const MEP_G T* vp;
+    MEP_DEV KeyTiles(const mep_diff_attn_desc& desc, const Job& j) : d(desc) {
+        kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
+        vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
+    }
+    MEP_DEV void load(T* tile, int k0, unsigned long long bits) const {
+        constexpr int CK = DK / M::E;
+        const unsigned sK = (unsigned)d.k_sT, sV = (unsigned)d.v_sT, sM = (unsigned)d.k_sM;
+        stage<M, Ge::KT, 2 * DK>(tile, kp + k0 * d.k_sT, [&](int r, int c, unsigned& off) {
+            const int m = c >= CK, col = (c - m * CK) * M::E;
+            off = r * sK + col + (m ? sM : 0u);
+            return col < d.d && (bits >> r & 1);
+        });
+        stage<M, Ge::KT, DV>(tile + Ge::KSZ, vp + k0 * d.v_sT, [&](int r, int c, unsigned& off) {
+            off = r * sV + c * M::E;
+            return c * M::E < d.dv && (bits >> r & 1);
+        });
+    }
+};
+
+// the rows of a wave: lane's row, its query and head, and what the wave's keys are
+struct Rows32 {
+    int row0, row, t, head, wend, wfull;
+    bool live;
+    MEP_DEV Rows32(const mep_diff_attn_desc& d, const Job& j) {
+        row0 = j.block * DA_ROWS + (threadIdx.x >> 6) * 32;
+        row = row0 + (threadIdx.x & 31);
+        live = row < j.rows;
+        const int rr = live ? row : j.rows - 1;
+        t = rr / j.n;
+        head = j.g * j.n + rr - t * j.n;
+        wend = row0 < j.rows ? key_end(d, j, (min(j.rows, row0 + 32) - 1) / j.n) : 0;
+        wfull = d.causal ? j.first + row0 / j.n + 1 : INT_MAX;         // keys below are causal for all the wave's rows
+    }
+};
+
+// A wave's accumulators (32 rows or keys x 32 N channels, transposed) times f, rounded, to rows of global memory: through LDS
+// (a wave's own 32 x (32 N + E) elements), so that a row's channels are written together.  row_at(r): the row's first element, or null.
+template <class M, int N, class F>
+MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, int n, F row_at) {
+    typedef typename M::T T;
+    constexpr int LD = 32 * N + M::E;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            typename VecOf<T, 4>::type v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][r + e] * f);
+            *reinterpret_cast<typename VecOf<T, 4>::type*>(buf + (lane & 31) * LD + 32 * i + acc_off(r) + 4 * h) = v;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // this wave's own writes
+    constexpr int CH = 32 * N / M::E;
+    const bool whole = n % M::E == 0;
+#pragma unroll 1
+    for (int i = lane; i < 32 * CH; i += 64) {
+        const int r = i / CH, col = i % CH * M::E;
+        MEP_G T* p = row_at(r);
+        if (!p || col >= n) continue;
+        const typename M::Frag v = *reinterpret_cast<const typename M::Frag*>(buf + r * LD + col);
+        if (whole) {
+            *reinterpret_cast<MEP_G typename M::Frag*>(p + col) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < M::E; ++e) if (col + e < n) p[col + e] = v[e];
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next one is written
+}
+
+// ------------------------------------------------------------------ forward
+// One pass over the keys.  With e_m = 2^(s_m c - m_m) and l_m = sum e_m, out = E_1 / l_1 - lam E_2 / l_2 for E_m = sum e_m v.
+// The accumulators hold X = sum round(f1 e_1 - f2 e_2) v and Y = sum round(e_2) v with f2 / f1 = rho, an estimate of
+// lam l_1 / l_2 from the keys seen so far, max(f1, |f2|) = 1; at the end
+//   out = X / (f1 l_1) + (f2 / (f1 l_1) - lam / l_2) Y.
+// What is rounded is the difference itself, up to the estimate's error: where the maps cancel, l_1 / l_2 hardly changes along the
+// keys and Y's factor vanishes.  rho is renewed, by X' = f1' (X + f2 Y) / f1 - f2' Y, at every rescaling and whenever it is
+// off the sums so far (these keys' own among them) by a quarter: a few times a row, and neither operand is ever of a size
+// that the row's weights do not have.
+// The maxima m_m are renewed only when a score exceeds one by 8 (e <= 256: the sums are as exact), the lanes of a row agree on them, and
+// the sums l_m stay lane-local to the end.
+template <int TYPE, int DK, int DV>
+__global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks) {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef typename Ge::M M;
+    typedef typename Ge::T T;
+    typedef typename Ge::Frag Frag;
+    constexpr int KT = Ge::KT;
+    __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
+    const Job j = make_job(d, blocks, d.causal);
+    const int h = (threadIdx.x & 63) >> 5;
+    const Rows32 w(d, j);
+    const KeyTiles<TYPE, DK, DV> keys(d, j);
+    const float c = d.scale * DA_LOG2E;
+    const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
+
+    unsigned raw = key_raw(d, j, 0);
+    unsigned long long bits = key_bits(d, j, 0, KT, raw);
+    if (end > 0) keys.load(Buf, 0, bits);
+    raw = key_raw(d, j, KT);
+    Frag q[2][Ge::NK];
+    {
+        const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < Ge::NK; ++i)
+                q[m][i] = row_frag<M>(qp + m * d.q_sM, M::KS * i + M::E * h, d.d, w.live);
+    }
+    const float lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
+
+    float m1 = mul_rn(DA_MIN, c), m2 = m1, l1 = 0.f, l2 = 0.f, top1 = DA_MIN, top2 = DA_MIN, f1 = 1.f, f2 = 0.f;
+    floatx16 x[DV / 32], y[DV / 32];
+#pragma unroll
+    for (int n = 0; n < DV / 32; ++n) x[n] = y[n] = zero16();
+    for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+        tile_sync();
+        const unsigned long long now = bits;
+        if (k0 + KT < end) {
+            bits = key_bits(d, j, k0 + KT, KT, raw);
+            keys.load(Buf + (buf ^ 1) * Ge::TSZ, k0 + KT, bits);
+            raw = key_raw(d, j, k0 + 2 * KT);
+        }
+        const T* kt = Buf + buf * Ge::TSZ;
+        const T* vt = kt + Ge::KSZ;
+#pragma unroll 1
+        for (int sub = 0; sub < KT / 32; ++sub) {
+            const int ks = k0 + 32 * sub;
+            const unsigned on = (unsigned)(now >> (32 * sub));
+            if (ks >= w.wend || !on) continue;
+            floatx16 s1 = zero16(), s2 = zero16();
+#pragma unroll
+            for (int i = 0; i < Ge::NK; ++i) {
+                s1 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, 0, i), q[0][i], s1);
+                s2 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, DK / M::E, i), q[1][i], s2);
+            }
+            if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
+            const float a1 = max16(s1), a2 = max16(s2);
+            top1 = fmaxf(top1, a1);
+            top2 = fmaxf(top2, a2);
+            if (__ballot(a1 * c > m1 + 8.f || a2 * c > m2 + 8.f)) {
+                const float n1 = fmaxf(m1, mul_rn(half_max(top1), c)), n2 = fmaxf(m2, mul_rn(half_max(top2), c));
+                const float g1 = exp2_fast(m1 - n1), g2 = exp2_fast(m2 - n2);
+                l1 *= g1;
+                l2 *= g2;
+                m1 = n1;
+                m2 = n2;
+#pragma unroll
+                for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        x[n][r] = fmaf(f2, y[n][r], x[n][r]) * g1;      // f1 E_1 alone: g2 may be 0
+                        y[n][r] *= g2;
+                    }
+                f2 = 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s1[r] = exp2_fast(fmaf(s1[r], c, -m1));
+                s2[r] = exp2_fast(fmaf(s2[r], c, -m2));
+                l1 += s1[r];
+                l2 += s2[r];
+            }
+            const float t1 = lam * half_sum(l1), t2 = half_sum(l2);
+            if (__ballot(fabsf(t1 * f1 - t2 * f2) > 0.25f * fabsf(t1 * f1))) {
+                const float rho = t2 > 0.f ? t1 / t2 : 0.f, h1 = 1.f / fmaxf(1.f, fabsf(rho)), h2 = rho * h1;
+                const float u = h1 / f1, v = u * f2 - h2;
+#pragma unroll
+                for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[n][r] = fmaf(x[n][r], u, y[n][r] * v);
+                f1 = h1;
+                f2 = h2;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s1[r] = fmaf(s1[r], f1, -f2 * s2[r]);
+#pragma unroll
+            for (int i = 0; i < Ge::NP; ++i) {
+                const Frag p = acc_frag<M>(s1, i), e = acc_frag<M>(s2, i);
+#pragma unroll
+                for (int n = 0; n < DV / 32; ++n) {
+                    const Frag v = lds_frag_t<M, DV>(vt, 32 * sub, 32 * n, i);
+                    x[n] = M::mma(v, p, x[n]);
+                    y[n] = M::mma(v, e, y[n]);
+                }
+            }
+        }
+    }
+    // the row's sums over both lane halves, and its true maxima (the backward's e_m are then at most 1)
+    l1 = half_sum(l1);
+    l2 = half_sum(l2);
+    const float i1 = l1 > 0.f ? 1.f / l1 : l1, i2 = l2 > 0.f ? 1.f / l2 : l2;
+    // one rounding each, as m1 and m2 have: without keys the differences below are 0
+    const float n1 = mul_rn(half_max(top1), c), n2 = mul_rn(half_max(top2), c);
+    if (d.stats && w.live && h == 0)
+        *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) =
+            f32x4{n1, i1 * exp2_fast(n1 - m1), n2, i2 * exp2_fast(n2 - m2)};
+    const float fx = i1 / f1, fy = fx * f2 - lam * i2;
+    tile_sync();                             // the tiles are free
+    const int64_t first = (int64_t)j.b * d.Tq * d.H * d.dv;
+    auto row_at = [&](uint64_t p, int r) -> MEP_G T* {
+        const int row = w.row0 + r;
+        if (row >= j.rows) return nullptr;
+        const int t = row / j.n;
+        return G<T>(p) + first + ((int64_t)t * d.H + j.g * j.n + row - t * j.n) * d.dv;
+    };
+    T* mine = Buf + (threadIdx.x >> 6) * 32 * (DV + M::E);
+#pragma unroll
+    for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[n][r] = fmaf(x[n][r], fx, y[n][r] * fy);
+    write_rows<M>(mine, x, 1.f, d.dv, [&](int r) { return row_at(d.out, r); });
+    if (d.second) write_rows<M>(mine, y, i2, d.dv, [&](int r) { return row_at(d.second, r); });
+}
+
+// ------------------------------------------------------------------ backward: D and dq
+// D_m = dO . (A_m v) is known from the forward's out and second = A_2 v only up to their roundings, which would be an error of
+// the size of dS where few keys carry a row.  So dS is formed with that estimate, the row sums of A_m dP are formed beside it
+// without any rounding to 16 bits, and their difference is put right at the end: dq_m -= (D_m - estimate) A_m k_m, for which
+// E_m k_m is summed too (CORR; in fp32 the estimate is as good as the sum).  The sums are also lam's gradient and what dk needs.
+template <int TYPE, int DK, int DV>
+__global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef typename Ge::M M;
+    typedef typename Ge::T T;
+    typedef typename Ge::Frag Frag;
+    constexpr int KT = Ge::KT;
+    const mep_diff_attn_desc& d = bd.f;
+    __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
+    const Job j = make_job(d, blocks, d.causal);
+    const int h = (threadIdx.x & 63) >> 5;
+    const Rows32 w(d, j);
+    const KeyTiles<TYPE, DK, DV> keys(d, j);
+    const float c = d.scale * DA_LOG2E;
+    const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
+
+    unsigned raw = key_raw(d, j, 0);
+    unsigned long long bits = key_bits(d, j, 0, KT, raw);
+    if (end > 0) keys.load(Buf, 0, bits);
+    raw = key_raw(d, j, KT);
+    Frag q[2][Ge::NK], g[Ge::NV];
+    float d1 = 0.f, d2 = 0.f;              // the estimates
+    {
+        const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
+        const MEP_G T* gp = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)w.t * bd.o_sT + (int64_t)w.head * bd.o_sH;
+        const int64_t at = (((int64_t)j.b * d.Tq + w.t) * d.H + w.head) * d.dv;
+        const MEP_G T* o = G<const T>(d.out) + at;
+        const MEP_G T* o2 = G<const T>(d.second) + at;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < Ge::NK; ++i)
+                q[m][i] = row_frag<M>(qp + m * d.q_sM, M::KS * i + M::E * h, d.d, w.live);
+#pragma unroll
+        for (int i = 0; i < Ge::NV; ++i) {
+            const int col = M::KS * i + M::E * h;
+            g[i] = row_frag<M>(gp, col, d.dv, w.live);
+            if (d.dv % M::E == 0) {
+                const Frag a = row_frag<M>(o, col, d.dv, true), b = row_frag<M>(o2, col, d.dv, true);
+#pragma unroll
+                for (int e = 0; e < M::E; ++e) {
+                    d1 = fmaf((float)g[i][e], (float)a[e], d1);
+                    d2 = fmaf((float)g[i][e], (float)b[e], d2);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < M::E; ++e)
+                    if (col + e < d.dv) {
+                        d1 = fmaf((float)g[i][e], (float)o[col + e], d1);
+                        d2 = fmaf((float)g[i][e], (float)o2[col + e], d2);
+                    }
+            }
+        }
+        d1 = half_sum(d1);
+        d2 = half_sum(d2);
+    }
+    const float lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
+    d1 = fmaf(lam, d2, d1);                     // out = A_1 v - lam A_2 v
+    const int64_t srow = ((int64_t)j.b * d.H + w.head) * d.Tq + w.t;
+    const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * srow);      // m1, 1 / l1, m2, 1 / l2
+
+    constexpr bool CORR = TYPE != MEP_F32;
+    float sum1 = 0.f, sum2 = 0.f;
+    floatx16 a1[DK / 32], a2[DK / 32], k1[CORR ? DK / 32 : 1], k2[CORR ? DK / 32 : 1];
+#pragma unroll
+    for (int n = 0; n < DK / 32; ++n) {
+        a1[n] = a2[n] = zero16();
+        if constexpr (CORR) k1[n] = k2[n] = zero16();
+    }
+    for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+        tile_sync();
+        const unsigned long long now = bits;
+        if (k0 + KT < end) {
+            bits = key_bits(d, j, k0 + KT, KT, raw);
+            keys.load(Buf + (buf ^ 1) * Ge::TSZ, k0 + KT, bits);
+            raw = key_raw(d, j, k0 + 2 * KT);
+        }
+        const T* kt = Buf + buf * Ge::TSZ;
+        const T* vt = kt + Ge::KSZ;
+#pragma unroll 1
+        for (int sub = 0; sub < KT / 32; ++sub) {
+            const int ks = k0 + 32 * sub;
+            const unsigned on = (unsigned)(now >> (32 * sub));
+            if (ks >= w.wend || !on) continue;
+            floatx16 s1 = zero16(), s2 = zero16(), dp = zero16();
+#pragma unroll
+            for (int i = 0; i < Ge::NK; ++i) {
+                s1 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, 0, i), q[0][i], s1);
+                s2 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, DK / M::E, i), q[1][i], s2);
+            }
+#pragma unroll
+            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(lds_frag<M, DV>(vt, 32 * sub, 0, i), g[i], dp);
+            if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s1[r] = exp2_fast(fmaf(s1[r], c, -st[0]));
+                s2[r] = exp2_fast(fmaf(s2[r], c, -st[2]));
+                sum1 = fmaf(s1[r], dp[r], sum1);
+                sum2 = fmaf(s2[r], dp[r], sum2);
+            }
+            Frag e1[CORR ? Ge::NP : 1], e2[CORR ? Ge::NP : 1];
+            if constexpr (CORR) {
+#pragma unroll
+                for (int i = 0; i < Ge::NP; ++i) {
+                    e1[i] = acc_frag<M>(s1, i);
+                    e2[i] = acc_frag<M>(s2, i);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {      // dS_m without the row's factors 1 / l1, -lam / l2
+                s1[r] *= dp[r] - d1;
+                s2[r] *= dp[r] - d2;
+            }
+#pragma unroll
+            for (int i = 0; i < Ge::NP; ++i) {
+                const Frag p1 = acc_frag<M>(s1, i), p2 = acc_frag<M>(s2, i);
+#pragma unroll
+                for (int n = 0; n < DK / 32; ++n) {
+                    const Frag f1 = lds_frag_t<M, 2 * DK>(kt, 32 * sub, 32 * n, i), f2 = lds_frag_t<M, 2 * DK>(kt, 32 * sub, DK + 32 * n, i);
+                    a1[n] = M::mma(f1, p1, a1[n]);
+                    a2[n] = M::mma(f2, p2, a2[n]);
+                    if constexpr (CORR) {
+                        k1[n] = M::mma(f1, e1[i], k1[n]);
+                        k2[n] = M::mma(f2, e2[i], k2[n]);
+                    }
+                }
+            }
+        }
+    }
+    sum1 = half_sum(sum1) * st[1];
+    sum2 = half_sum(sum2) * st[3];
+    if (w.live && h == 0) {
+        *reinterpret_cast<MEP_G f32x4*>(G<float>(bd.delta) + 4 * srow) = f32x4{sum1, sum2, 0.f, 0.f};
+        if (bd.dlam_rows) G<float>(bd.dlam_rows)[((int64_t)j.b * d.Tq + w.t) * d.H + w.head] = -sum2;
+    }
+    if (!bd.dq) return;
+    tile_sync();                             // the tiles are free
+    if constexpr (CORR) {
+#pragma unroll
+        for (int n = 0; n < DK / 32; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                a1[n][r] = fmaf(k1[n][r], d1 - sum1, a1[n][r]);
+                a2[n][r] = fmaf(k2[n][r], d2 - sum2, a2[n][r]);
+            }
+    }
+    const int64_t first = (int64_t)j.b * d.Tq * d.H * 2 * d.d;
+    auto row_at = [&](int m, int r) -> MEP_G T* {
+        const int row = w.row0 + r;
+        if (row >= j.rows) return nullptr;
+        const int t = row / j.n;
+        return G<T>(bd.dq) + first + (((int64_t)t * d.H + j.g * j.n + row - t * j.n) * 2 + m) * d.d;
+    };
+    T* mine = Buf + (threadIdx.x >> 6) * 32 * (DK + M::E);
+    write_rows<M>(mine, a1, st[1] * d.scale, d.d, [&](int r) { return row_at(0, r); });
+    write_rows<M>(mine, a2, -lam * st[3] * d.scale, d.d, [&](int r) { return row_at(1, r); });
+}
+
+// ------------------------------------------------------------------ backward: dk and dv
+// A wave owns 32 keys (an accumulator column each) and walks the rows; KREG: its K and V operands stay in registers.
+template <int TYPE, int DK, int DV, bool KREG>
+__global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks) {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef typename Ge::M M;
+    typedef typename Ge::T T;
+    typedef typename Ge::Frag Frag;
+    constexpr int RT = Ge::KT;
+    const mep_diff_attn_desc& d = bd.f;
+    __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their queries, then their upstream gradients
+    __shared__ __align__(16) float Rs[2][6][RT];      // a row's m1, m2, i1, lam i2, i1 D1, lam i2 D2
+    __shared__ int Ts[2][RT];                         // and its query
+    const Job j = make_job(d, blocks, false);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int key0 = j.block * DA_ROWS + wave * 32, key = key0 + (lane & 31);
+    const float c = d.scale * DA_LOG2E;
+    // rows that see any of the block's / the wave's keys; every one of the wave's keys: from row wfull on
+    const int bstart = d.causal ? max(0, min(d.Tq, j.block * DA_ROWS - j.first)) * j.n : 0;
+    const int wstart = d.causal ? max(0, min(d.Tq, key0 - j.first)) * j.n : 0;
+    const int wfull = d.causal ? max(0, min(d.Tq, key0 + 31 - j.first)) * j.n : 0;
+    const int rmin = d.causal ? max(0, min(d.Tq, key - j.first)) * j.n : 0;      // the lane's key's first row
+    const int rend = j.block * DA_ROWS < j.len ? j.rows : 0;
+
+    const MEP_G T* qb = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)j.g * j.n * d.q_sH;
+    const MEP_G T* ob = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
+    auto load_rows = [&](int buf, int r0) {
+        const int t0 = r0 / j.n, x0 = r0 - t0 * j.n;      // the tile's first query and its first head there
+        auto place = [&](int r, int& t, int& x) {
+            t = 0;
+            x = 0;
+            if (j.n == 1) t = r;
+            else {
+                const unsigned y = (unsigned)(x0 + r);
+                t = (int)(y / (unsigned)j.n);
+                x = (int)y - t * j.n;
+            }
+        };
+        constexpr int CK = DK / M::E;
+        stage<M, RT, 2 * DK>(Buf + buf * Ge::TSZ, qb + (int64_t)t0 * d.q_sT, [&](int r, int ch, unsigned& off) {
+            const int m = ch >= CK, col = (ch - m * CK) * M::E;
+            int t, x;
+            place(r, t, x);
+            off = (unsigned)t * (unsigned)d.q_sT + (unsigned)x * (unsigned)d.q_sH + col + (m ? (unsigned)d.q_sM : 0u);
+            return col < d.d && r0 + r < j.rows;
+        });
+        stage<M, RT, DV>(Buf + buf * Ge::TSZ + Ge::KSZ, ob + (int64_t)t0 * bd.o_sT, [&](int r, int ch, unsigned& off) {
+            int t, x;
+            place(r, t, x);
+            off = (unsigned)t * (unsigned)bd.o_sT + (unsigned)x * (unsigned)bd.o_sH + ch * M::E;
+            return ch * M::E < d.dv && r0 + r < j.rows;
+        });
+    };
+    f32x4 sv = {0.f, 0.f, 0.f, 0.f}, dv4 = sv;      // a row's statistics on their way to LDS: past the end A = 0
+    float lv = 0.f;
+    int tv = 0;
+    auto fetch_stats = [&](int r0) {
+        const int row = r0 + threadIdx.x;
+        sv = dv4 = f32x4{0.f, 0.f, 0.f, 0.f};
+        lv = 0.f;
+        tv = 0;
+        if (threadIdx.x < RT && row < j.rows) {
+            tv = row / j.n;
+            const int head = j.g * j.n + row - tv * j.n;
+            const int64_t srow = ((int64_t)j.b * d.H + head) * d.Tq + tv;
+            sv = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * srow);
+            dv4 = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(bd.delta) + 4 * srow);
+            lv = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)tv * d.lam_sT + (int64_t)head * d.lam_sH];
+        }
+    };
+    auto put_stats = [&](int buf) {
+        if (threadIdx.x < RT) {
+            const int i = threadIdx.x;
+            Rs[buf][0][i] = sv[0];
+            Rs[buf][1][i] = sv[2];
+            Rs[buf][2][i] = sv[1];
+            Rs[buf][3][i] = lv * sv[3];
+            Rs[buf][4][i] = sv[1] * dv4[0];
+            Rs[buf][5][i] = lv * sv[3] * dv4[1];
+            Ts[buf][i] = tv;
+        }
+    };
+    const int rbeg = bstart / RT * RT;
+    if (rbeg < rend) {
+        load_rows(0, rbeg);
+        fetch_stats(rbeg);
+    }
+    bool on = key < j.len;
+    if (on && d.mask_form == 1) on = mask_at(d, (int64_t)j.b * d.m_sB + (int64_t)key * d.m_sK);
+    const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH + (int64_t)(on ? key : 0) * d.k_sT;
+    const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH + (int64_t)(on ? key : 0) * d.v_sT;
+    auto load_k = [&](int m, int i) { return row_frag<M>(kp + m * d.k_sM, M::KS * i + M::E * h, d.d, on); };
+    auto load_v = [&](int i) { return row_frag<M>(vp, M::KS * i + M::E * h, d.dv, on); };
+    Frag kr[2][KREG ? Ge::NK : 1], vr[KREG ? Ge::NV : 1];
+    if constexpr (KREG) {
+#pragma unroll
+        for (int i = 0; i < Ge::NK; ++i) { kr[0][i] = load_k(0, i); kr[1][i] = load_k(1, i); }
+#pragma unroll
+        for (int i = 0; i < Ge::NV; ++i) vr[i] = load_v(i);
+    }
+    floatx16 ak1[DK / 32], ak2[DK / 32], av[DV / 32];
+#pragma unroll
+    for (int n = 0; n < DK / 32; ++n) ak1[n] = ak2[n] = zero16();
+#pragma unroll
+    for (int n = 0; n < DV / 32; ++n) av[n] = zero16();
+    const bool wave_on = __ballot(on) != 0, all_on = __ballot(on) == ~0ull;
+    if (rbeg < rend) put_stats(0);
+
+    for (int r0 = rbeg, buf = 0; r0 < rend; r0 += RT, buf ^= 1) {
+        tile_sync();
+        const bool more = r0 + RT < rend;
+        if (more) {
+            load_rows(buf ^ 1, r0 + RT);
+            fetch_stats(r0 + RT);
+        }
+        const T* qt = Buf + buf * Ge::TSZ;
+        const T* ot = qt + Ge::KSZ;
+#pragma unroll 1
+        for (int sub = 0; sub < RT / 32; ++sub) {
+            const int rs = r0 + 32 * sub;
+            if (!wave_on || rs >= j.rows || rs + 32 <= wstart) continue;
+            floatx16 s1 = zero16(), s2 = zero16(), dp = zero16();
+#pragma unroll
+            for (int i = 0; i < Ge::NK; ++i) {
+                const Frag k1 = KREG ? kr[0][KREG ? i : 0] : load_k(0, i), k2 = KREG ? kr[1][KREG ? i : 0] : load_k(1, i);
+                s1 = M::mma(lds_frag<M, 2 * DK>(qt, 32 * sub, 0, i), k1, s1);
+                s2 = M::mma(lds_frag<M, 2 * DK>(qt, 32 * sub, DK / M::E, i), k2, s2);
+            }
+#pragma unroll
+            for (int i = 0; i < Ge::NV; ++i) {
+                const Frag v = KREG ? vr[KREG ? i : 0] : load_v(i);
+                dp = M::mma(lds_frag<M, DV>(ot, 32 * sub, 0, i), v, dp);
+            }
+            if (!all_on || rs < wfull || d.mask_form == 2) {      // rows that see this lane's key: those from rmin on
+                const int least = rmin - rs - 4 * h;
+                unsigned ok = !on || least > 31 ? 0u : least > 0 ? ~0u << least : ~0u;
+                if (d.mask_form == 2) {
+                    const int64_t o = (int64_t)j.b * d.m_sB + (int64_t)min(key, d.Tk - 1) * d.m_sK;
+                    unsigned keep = 0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        keep |= (mask_at(d, o + (int64_t)Ts[buf][32 * sub + acc_off(r) + 4 * h] * d.m_sQ) ? 1u : 0u) << acc_off(r);
+                    ok &= keep;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s1[r] = ok >> acc_off(r) & 1 ? s1[r] : -INFINITY;
+                    s2[r] = ok >> acc_off(r) & 1 ? s2[r] : -INFINITY;
+                }
+            }
+            floatx16 p;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int lr = 32 * sub + acc_off(r) + 4 * h;
+                const float x1 = exp2_fast(fmaf(s1[r], c, -Rs[buf][0][lr])), x2 = exp2_fast(fmaf(s2[r], c, -Rs[buf][1][lr]));
+                p[r] = x1 * Rs[buf][2][lr] - x2 * Rs[buf][3][lr];
+                s1[r] = x1 * fmaf(dp[r], Rs[buf][2][lr], -Rs[buf][4][lr]);
+                s2[r] = x2 * fmaf(dp[r], -Rs[buf][3][lr], Rs[buf][5][lr]);
+            }
+#pragma unroll
+            for (int i = 0; i < Ge::NP; ++i) {
+                const Frag fp = acc_frag<M>(p, i), f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
+#pragma unroll
+                for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(lds_frag_t<M, DV>(ot, 32 * sub, 32 * n, i), fp, av[n]);
+#pragma unroll
+                for (int n = 0; n < DK / 32; ++n) {
+                    ak1[n] = M::mma(lds_frag_t<M, 2 * DK>(qt, 32 * sub, 32 * n, i), f1, ak1[n]);
+                    ak2[n] = M::mma(lds_frag_t<M, 2 * DK>(qt, 32 * sub, DK + 32 * n, i), f2, ak2[n]);
+                }
+            }
+        }
+        if (more) put_stats(buf ^ 1);
+    }
+    tile_sync();                             // the tiles are free
+    // masked keys and keys past the lengths get zeros
+    const int64_t first = (int64_t)j.b * d.Tk * d.G + j.g;
+    auto key_at = [&](uint64_t p, int r, int64_t width) -> MEP_G T* {
+        return key0 + r < d.Tk ? G<T>(p) + (first + (int64_t)(key0 + r) * d.G) * width : nullptr;
+    };
+    T* mine = Buf + wave * 32 * ((DK > DV ? DK : DV) + M::E);
+    write_rows<M>(mine, ak1, d.scale, d.d, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
+    write_rows<M>(mine, ak2, d.scale, d.d, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
+    write_rows<M>(mine, av, 1.f, d.dv, [&](int r) { return key_at(bd.dv, r, d.dv); });
+}
+
+// ------------------------------------------------------------------ instances
+template <int TYPE, int DK, int DV>
+void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
+    // fp32 keys of 128 + 128 + 256 channels beside their gradients' accumulators would need more than the register file
+    constexpr bool KREG = !(TYPE == MEP_F32 && DK >= 128);
+    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks);
+    else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+    else hipLaunchKernelGGL((k_diff_bwd_kv<TYPE, DK, DV, KREG>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+}
+
+// the smallest instance that holds the head widths
+template <int TYPE>
+void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
+    if (d.d <= 32 && d.dv <= 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, st);
+    else if (d.d <= 32 && d.dv <= 64) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, st);
+    else if (d.d <= 64 && d.dv <= 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, st);
+    else if (d.d <= 64 && d.dv <= 128) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, st);
+    else if (d.dv <= 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, st);
+    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, st);
+}
+
+void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st);
+void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st);
+void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st);
+
+}  // namespace mep

@@ -309,25 +309,43 @@ def norm(x, weight=None, bias=None, *, kind='rms', eps=1e-6):
 
 
 # ------------------------------------------------------------------ differential attention
+def _packed(t, heads=1):
+    """t [B, T, H, (2,) n] as the attention kernels read it: 16 bytes at a time, 64 time steps within 2^30 elements; a copy with
+    rows padded by zeros (mep_pack_rows) where it does not lie so."""
+    V = 16 // t.element_size()
+    st = t.stride()
+    sM = st[3] if t.dim() == 5 else 0
+    if st[-1] == 1 and t.shape[-1] % V == 0 and t.data_ptr() % 16 == 0 and not any(s % V for s in st[:-1]) and \
+            st[1] < 1 << 23 and sM < 1 << 28 and st[2] * heads < 1 << 28:
+        return t
+    n = t.shape[-1]
+    y = torch.empty(*t.shape[:-1], -(-n // V) * V, dtype=t.dtype, device=t.device)
+    if t.numel():
+        _launch('mep_pack_rows', _lib.PackRowsDesc(x=_ptr(t), y=_ptr(y), sB=st[0], sT=st[1], sH=st[2], sM=sM, sN=st[-1], B=t.shape[0], T=t.shape[1],
+                                                   H=t.shape[2], M=t.shape[3] if t.dim() == 5 else 1, n=n, type=TYPES[t.dtype]), t.device)
+    return y
+
+
 class _DiffAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, mask, lengths, q_start, q, k, v, lam):
         causal, scale = cfg
-        q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
         B, Tq, H, _, hd = q.shape
         Tk, G, dv = k.shape[1], k.shape[2], v.shape[3]
         dev = q.device
+        qp, kp, vp = _packed(q, H // G), _packed(k), _packed(v)
         out = torch.empty(B, Tq, H, dv, dtype=q.dtype, device=dev)
         keep = any(ctx.needs_input_grad)
         stats = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev) if keep else None
+        second = torch.empty_like(out) if keep else None
         ls = (0, 0, lam.stride(0)) if lam.dim() == 1 else lam.stride()
         m = (0, 0, 0)
         if mask is not None:
             m = (mask.stride(0), 0, mask.stride(1)) if mask.dim() == 2 else mask.stride()
-        d = _lib.DiffAttnDesc(q=_ptr(q), k=_ptr(k), v=_ptr(v), lam=_ptr(lam), out=_ptr(out), stats=_ptr(stats),
-                              q_sB=q.stride(0), q_sT=q.stride(1), q_sH=q.stride(2), q_sM=q.stride(3),
-                              k_sB=k.stride(0), k_sT=k.stride(1), k_sH=k.stride(2), k_sM=k.stride(3),
-                              v_sB=v.stride(0), v_sT=v.stride(1), v_sH=v.stride(2), lam_sB=ls[0], lam_sT=ls[1], lam_sH=ls[2],
+        qs, ks, vs = qp.stride(), kp.stride(), vp.stride()
+        d = _lib.DiffAttnDesc(q=_ptr(qp), k=_ptr(kp), v=_ptr(vp), lam=_ptr(lam), out=_ptr(out), stats=_ptr(stats), second=_ptr(second),
+                              q_sB=qs[0], q_sT=qs[1], q_sH=qs[2], q_sM=qs[3], k_sB=ks[0], k_sT=ks[1], k_sH=ks[2], k_sM=ks[3],
+                              v_sB=vs[0], v_sT=vs[1], v_sH=vs[2], lam_sB=ls[0], lam_sT=ls[1], lam_sH=ls[2],
                               mask=_ptr(mask), m_sB=m[0], m_sQ=m[1], m_sK=m[2], lengths=_ptr(lengths), q_start=_ptr(q_start),
                               B=B, Tq=Tq, Tk=Tk, H=H, G=G, d=hd, dv=dv, type=TYPES[q.dtype], causal=int(causal),
                               mask_form=0 if mask is None else mask.dim() - 1,
@@ -335,7 +353,8 @@ class _DiffAttnFn(torch.autograd.Function):
         _launch('mep_diff_attn_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
-            ctx.save_for_backward(mask, lengths, q_start, q, k, v, lam, stats)
+            # the packed copies too: the descriptor holds their addresses
+            ctx.save_for_backward(mask, lengths, q_start, q, k, v, lam, stats, second, out, qp, kp, vp)
             ctx.desc = d
         return out
 
@@ -344,17 +363,16 @@ class _DiffAttnFn(torch.autograd.Function):
     def backward(ctx, dout):
         if dout is None:
             return (None,) * 8
-        mask, lengths, q_start, q, k, v, lam, stats = ctx.saved_tensors
+        q, k, v, lam = ctx.saved_tensors[3:7]
         need = ctx.needs_input_grad
-        if dout.stride(-1) != 1:
-            dout = dout.contiguous()
         B, Tq, H, _, _ = q.shape
         dev = q.device
+        dout = _packed(dout, H // k.shape[2])
         like = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
         dq = like(q) if need[4] else None
         dk, dv = (like(k), like(v)) if need[5] or need[6] else (None, None)
         dlam = like(lam) if need[7] else None
-        delta = torch.empty(B, H, Tq, 2, dtype=torch.float32, device=dev)
+        delta = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev)
         shared = lam.dim() == 1
         bd = _lib.DiffAttnBwdDesc(f=ctx.desc, dout=_ptr(dout), o_sB=dout.stride(0), o_sT=dout.stride(1), o_sH=dout.stride(2),
                                   dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlam=_ptr(dlam) if shared else 0,

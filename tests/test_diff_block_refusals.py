@@ -134,5 +134,10 @@ def test_descriptors_refused_before_any_launch():
                dict(k=0), dict(lam=0), dict(out=0), dict(Tk=1 << 30), dict(Tq=1 << 30), dict(B=1 << 20, Tq=1 << 20)):
         assert _refused('mep_diff_attn_fwd', attn(**kw)), kw
         assert _refused('mep_diff_attn_bwd', _lib.DiffAttnBwdDesc(f=attn(**kw), dout=16, delta=16)), kw
-    for kw in (dict(), dict(dout=16), dict(dout=16, delta=16, dk=16)):
-        assert _refused('mep_diff_attn_bwd', _lib.DiffAttnBwdDesc(f=attn(stats=16), **kw)), kw
+    for kw in (dict(q=8), dict(k=2), dict(v=4), dict(q_sT=4), dict(k_sM=2), dict(v_sH=1), dict(q_sT=1 << 23), dict(k_sM=1 << 28),
+               dict(k_sT=-8), dict(q_sH=1 << 28), dict(stats=16), dict(second=16)):
+        assert _refused('mep_diff_attn_fwd', attn(type=1, **kw)), kw
+    for kw in (dict(), dict(x=16), dict(x=16, y=8), dict(x=16, y=16, n=0), dict(x=16, y=16, type=3), dict(x=16, y=16, B=-1), dict(x=16, y=16, M=0)):
+        assert _refused('mep_pack_rows', _lib.PackRowsDesc(**dict(dict(B=1, T=1, H=1, M=1, n=8), **kw))), kw
+    for kw in (dict(), dict(dout=16), dict(dout=16, delta=16, dk=16), dict(dout=8, delta=16)):
+        assert _refused('mep_diff_attn_bwd', _lib.DiffAttnBwdDesc(f=attn(stats=16, second=16), **kw)), kw

@@ -21,7 +21,7 @@ def case(B, Tq, Tk, H, G, d, dv, dtype, lam='head', seed=1, std=1.0):
     return q, k, v, l
 
 
-def check(q, k, v, lam, grads=True, dout=None, scale=None, **masks):
+def check(q, k, v, lam, grads=True, dout=None, scale=None, same_maps=False, **masks):
     """Errors counted where they arise.  A score's 2^(s c - m) is off by its rounding and by |s| roundings of fp32 (both of the sum
     over d and of the exponent): `terms` of them at the products' magnitudes.  P and dS are rounded once to the type (half a step each);
     the output or gradient once more (ref.close counts that one).  An operand of P or dS below the type's smallest normal number lies
@@ -50,6 +50,9 @@ def check(q, k, v, lam, grads=True, dout=None, scale=None, **masks):
         lamb = w[3].expand(B, Tq, H).permute(0, 2, 1)[..., None].abs()
         both = a[:, :, 0] + lamb * a[:, :, 1]
         diff = (a[:, :, 0] - lamb * a[:, :, 1]).abs()
+        upto = lambda x: x.cumsum(-1)[..., [min(32 * (i // 32) + 31, Tk - 1) for i in range(Tk)]] if Tk else x  # noqa: E731
+        late = upto(a[:, :, 0]) / upto(a[:, :, 1]).clamp_min(1e-300)
+        fwd = diff if same_maps else a[:, :, 0] + lamb * a[:, :, 1] * (1.25 * late + 0.25)
     half = ref.half_step(q.dtype) if q.dtype != torch.float32 else 0.0
     terms = 64 + 16 * big + Tk / 8      # the exponents, and the sums over keys
     low = torch.finfo(q.dtype).smallest_normal * half
@@ -59,7 +62,7 @@ def check(q, k, v, lam, grads=True, dout=None, scale=None, **masks):
         """fp32 roundings at the sum of absolute terms, half a step of the type per rounded operand, and its subnormals'"""
         return terms * ref.U * sum_abs + half * rounded + low * other
 
-    tout = tol(torch.einsum('bhts,bshe->bthe', both, vv.abs()), torch.einsum('bhts,bshe->bthe', diff, vv.abs()),
+    tout = tol(torch.einsum('bhts,bshe->bthe', both, vv.abs()), torch.einsum('bhts,bshe->bthe', fwd, vv.abs()),
                torch.einsum('bhts,bshe->bthe', pairs, vv.abs()))
     ref.close(out, want, tout / ref.U, 1, 'out')
     assert torch.equal(out[~ok.any(-1).cuda()], torch.zeros_like(out[~ok.any(-1).cuda()])), 'empty rows'
@@ -187,7 +190,7 @@ def test_large_scores_and_equal_maps(cuda):
             q[..., 1, :] = q[..., 0, :]
             k[..., 1, :] = k[..., 0, :]
             lam.fill_(0.96875)
-        check(q, k, v, lam)
+        check(q, k, v, lam, same_maps=True)
 
 
 def test_scale(cuda):
