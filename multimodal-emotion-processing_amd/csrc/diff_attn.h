@@ -98,57 +98,126 @@ MEP_DEV typename M::Frag row_frag(const MEP_G typename M::T* row, int c, int n, 
     return live && c < n ? *reinterpret_cast<const MEP_G typename M::Frag*>(row + c) : zero_frag<M>();
 }
 
-typedef __attribute__((address_space(3))) void da_lds_void;
+typedef __attribute__((address_space(3))) char da_lds_char;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// ROWS x COLS of LDS from rows of global memory, by DMA.  where(r, c, off): whether chunk c of tile row r is there, at element
-// base + off; zeros otherwise.  Masked rows are never loaded: their contents, NaN too, never enter a product.
-template <class M, int ROWS, int COLS, class F>
-MEP_DEV void stage(typename M::T* dst, const MEP_G typename M::T* base, F where) {
-    typedef Lay<M, COLS> L;
-    constexpr int N = ROWS * L::CH / 64;                 // images of 64 chunks, one instruction of a wave each
-    static_assert(N * 64 == ROWS * L::CH && N % DA_WAVES == 0, "tile");
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, DA_SPAN, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < N / DA_WAVES; ++i) {
-        const int img = i * DA_WAVES + wave, pos = img * 64 + lane, r = pos / L::CH, c = (pos % L::CH) ^ L::sw(r);
-        unsigned off;
-        const bool on = where(r, c, off);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (da_lds_void*)(dst + img * 64 * M::E), 16,
-                                                 on ? off * (unsigned)sizeof(typename M::T) : DA_NOWHERE, 0, 0, 0);
-    }
+// 16 bytes a lane from the buffer `rs` at off + soff to LDS at `dst` + 16 lane (dst of the wave).  In inline assembly, since the
+// compiler would wait for every load in flight before the next LDS read, which is of the other tile; nothing but tile_sync
+// waits for these.  The loads return no registers; m0 has no other user in these kernels.
+MEP_DEV void dma16(const void* dst, unsigned off, i32x4 rs, unsigned soff) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const da_lds_char*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(off), "s"(rs), "s"(soff) : "memory");
 }
+// a raw buffer of DA_SPAN bytes from p on
+MEP_DEV i32x4 da_buffer(const MEP_G void* p) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)), (int)DA_SPAN, 0x00020000};
+}
+
+// ROWS x COLS of LDS from rows of global memory, by DMA: an instruction of a wave fills 64 chunks, and instruction i of a
+// lane takes chunk `chunk(i)` of row `row + i STEP`.  The chunk does not depend on i (but for rows of 64 chunks, on its
+// parity), so neither does the lane's offset, and a tile costs no address arithmetic: the row steps are the scalar offset.
+template <class M, int ROWS, int COLS>
+struct Stager {
+    typedef Lay<M, COLS> L;
+    typedef typename M::T T;
+    static constexpr int STEP = DA_THREADS / L::CH, N = ROWS / STEP, NO = L::CH > 32 ? 2 : 1;
+    static_assert(STEP >= 4 && ROWS % STEP == 0, "tile");
+    int row;
+    unsigned off[NO];                // byte offset of the lane's chunk in row `row`, or DA_NOWHERE
+    static MEP_DEV int chunk(int i) {
+        const int pos = threadIdx.x;
+        return (pos % L::CH) ^ L::sw(pos / L::CH + i * STEP);
+    }
+    // where(c): element offset of chunk c within its row, or -1 where there is none
+    template <class F>
+    MEP_DEV Stager(unsigned stride, F where) {
+        row = threadIdx.x / L::CH;
+#pragma unroll
+        for (int i = 0; i < NO; ++i) {
+            const int o = where(chunk(i));
+            off[i] = o < 0 ? DA_NOWHERE : (unsigned)(row * stride + o) * (unsigned)sizeof(T);
+        }
+    }
+    // rows of the tile with their bit set, `stride` elements apart from base on; zeros in the others.  Masked rows are never loaded:
+    // their contents, NaN too, never enter a product.
+    MEP_DEV void load(T* dst, const MEP_G T* base, unsigned stride, unsigned long long bits) const {
+        const i32x4 rs = da_buffer(base);
+        const bool full = bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1);
+        T* mine = dst + (threadIdx.x >> 6) * 64 * M::E;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            unsigned o = off[i % NO];
+            if (!full && !(bits >> (row + i * STEP) & 1)) o = DA_NOWHERE;
+            dma16(mine + i * DA_THREADS * M::E, o, rs, i * STEP * stride * (unsigned)sizeof(T));
+        }
+    }
+    // rows at any places: at(r): element offset of tile row r, or -1
+    template <class F>
+    MEP_DEV void gather(T* dst, const MEP_G T* base, unsigned stride, F at) const {
+        const i32x4 rs = da_buffer(base);
+        T* mine = dst + (threadIdx.x >> 6) * 64 * M::E;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int o = at(row + i * STEP);
+            const unsigned c = off[i % NO];
+            dma16(mine + i * DA_THREADS * M::E, o < 0 || c == DA_NOWHERE ? DA_NOWHERE : c + (unsigned)(o - row * (int)stride) * (unsigned)sizeof(T), rs, 0);
+        }
+    }
+};
 
 // every wave's DMA and LDS accesses done, then the workgroup barrier
-MEP_DEV void tile_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-// first-product operand i: row r0 + (lane & 31), chunk c0 + 2 i + h
-template <class M, int COLS>
-MEP_DEV typename M::Frag lds_frag(const typename M::T* tile, int r0, int c0, int i) {
-    const int lane = threadIdx.x & 63;
-    return *reinterpret_cast<const typename M::Frag*>(tile + Lay<M, COLS>::at(r0 + (lane & 31), c0 + 2 * i + (lane >> 5)));
+// (vmcnt = lgkmcnt = 0, by the builtin: the compiler then knows that nothing loaded before needs a wait behind it)
+MEP_DEV void tile_sync() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-// second-product operand: column col0 + (lane & 31) of the tile, rows r0 + KS i .. in accumulator order
+// A lane's places in a tile.  a[j]: first-product operand, chunk 2 j + h of row lane & 31 (j = 0 .. 3 of a group of 8 chunks); the
+// other rows and groups are constants away.  t[n]: second-product operand, in the rows of accumulator order and columns
+// 32 n + (lane & 31), n = 0, 1; likewise.
 template <class M, int COLS>
-MEP_DEV typename M::Frag lds_frag_t(const typename M::T* tile, int r0, int col0, int i) {
+struct Reader {
     typedef Lay<M, COLS> L;
-    const int lane = threadIdx.x & 63, h = lane >> 5;
-    if constexpr (M::KS == 8) {
-        typename M::Frag f;
-        const int col = col0 + (lane & 31);
+    typedef typename M::T T;
+    typedef typename M::Frag Frag;
+    static constexpr int NA = L::CH >= 8 ? 4 : 2, NT = L::CH >= 8 && M::KS == 16 ? 2 : 1;
+    int a[NA], t[NT];                // elements
+    MEP_DEV Reader() {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = tile[L::at(r0 + 8 * i + 4 * h + j, col / M::E) + col % M::E];
-        return f;
-    } else {
-        // the 16 lanes of a group read 4 rows x 16 columns and get a column's 4 rows each
-        const int r = r0 + 16 * i + 4 * h + ((lane & 15) >> 2), c = (col0 + (lane & 16)) / M::E + ((lane & 3) >> 1);
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + L::at(r, c) + 4 * (lane & 1)));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + L::at(r + 8, c) + 4 * (lane & 1)));
-        return __builtin_bit_cast(typename M::Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        for (int j = 0; j < NA; ++j) a[j] = L::at(lane & 31, 2 * j + h);
+        if constexpr (M::KS == 16) {     // the 16 lanes of a group read 4 rows x 16 columns and get a column's 4 rows each
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                t[n] = L::at(4 * h + ((lane & 15) >> 2), (32 * n + (lane & 16)) / M::E + ((lane & 3) >> 1)) + 4 * (lane & 1);
+        } else {
+            t[0] = 0;
+        }
     }
-}
+    // operand i (of all COLS) of the rows from r0 on
+    MEP_DEV Frag rows(const T* tile, int r0, int i) const {
+        return *reinterpret_cast<const Frag*>(tile + a[i % NA] + (r0 * L::CH + i / NA * 2 * NA) * M::E);
+    }
+    // step i of the rows from r0 on, columns col0 (a multiple of 32) ..
+    MEP_DEV Frag cols(const T* tile, int r0, int col0, int i) const {
+        if constexpr (M::KS == 8) {
+            Frag f;
+            const int lane = threadIdx.x & 63, col = col0 + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = tile[L::at(r0 + 8 * i + 4 * (lane >> 5) + j, col / M::E) + col % M::E];
+            return f;
+        } else {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const T* p = tile + t[col0 / 32 % NT] + ((r0 + 16 * i) * L::CH + col0 / (32 * NT) * (4 * NT)) * M::E;
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * L::CH * M::E));
+            return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
 
 // an accumulator tile as operand i of the next product, rounded to the tensors' type
 template <class M>
@@ -276,22 +345,21 @@ struct KeyTiles {
     const mep_diff_attn_desc& d;
     const MEP_G T* kp;
     const MEP_G T* vp;
-    MEP_DEV KeyTiles(const mep_diff_attn_desc& desc, const Job& j) : d(desc) {
+    Stager<M, Ge::KT, 2 * DK> ks;
+    Stager<M, Ge::KT, DV> vs;
+    MEP_DEV KeyTiles(const mep_diff_attn_desc& desc, const Job& j)
+        : d(desc),
+          ks((unsigned)desc.k_sT, [&](int c) {
+              const int m = c >= DK / M::E, col = c * M::E - m * DK;
+              return col < desc.d ? col + (m ? (int)desc.k_sM : 0) : -1;
+          }),
+          vs((unsigned)desc.v_sT, [&](int c) { return c * M::E < desc.dv ? c * M::E : -1; }) {
         kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
         vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
     }
     MEP_DEV void load(T* tile, int k0, unsigned long long bits) const {
-        constexpr int CK = DK / M::E;
-        const unsigned sK = (unsigned)d.k_sT, sV = (unsigned)d.v_sT, sM = (unsigned)d.k_sM;
-        stage<M, Ge::KT, 2 * DK>(tile, kp + k0 * d.k_sT, [&](int r, int c, unsigned& off) {
-            const int m = c >= CK, col = (c - m * CK) * M::E;
-            off = r * sK + col + (m ? sM : 0u);
-            return col < d.d && (bits >> r & 1);
-        });
-        stage<M, Ge::KT, DV>(tile + Ge::KSZ, vp + k0 * d.v_sT, [&](int r, int c, unsigned& off) {
-            off = r * sV + c * M::E;
-            return c * M::E < d.dv && (bits >> r & 1);
-        });
+        ks.load(tile, kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
+        vs.load(tile + Ge::KSZ, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
     }
 };
 
@@ -369,6 +437,8 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
     const int h = (threadIdx.x & 63) >> 5;
     const Rows32 w(d, j);
     const KeyTiles<TYPE, DK, DV> keys(d, j);
+    const Reader<M, 2 * DK> kread;
+    const Reader<M, DV> vread;
     const float c = d.scale * DA_LOG2E;
     const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
 
@@ -409,8 +479,8 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
             floatx16 s1 = zero16(), s2 = zero16();
 #pragma unroll
             for (int i = 0; i < Ge::NK; ++i) {
-                s1 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, 0, i), q[0][i], s1);
-                s2 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, DK / M::E, i), q[1][i], s2);
+                s1 = M::mma(kread.rows(kt, 32 * sub, i), q[0][i], s1);
+                s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q[1][i], s2);
             }
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
             const float a1 = max16(s1), a2 = max16(s2);
@@ -457,7 +527,7 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
                 const Frag p = acc_frag<M>(s1, i), e = acc_frag<M>(s2, i);
 #pragma unroll
                 for (int n = 0; n < DV / 32; ++n) {
-                    const Frag v = lds_frag_t<M, DV>(vt, 32 * sub, 32 * n, i);
+                    const Frag v = vread.cols(vt, 32 * sub, 32 * n, i);
                     x[n] = M::mma(v, p, x[n]);
                     y[n] = M::mma(v, e, y[n]);
                 }
@@ -509,6 +579,8 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
     const int h = (threadIdx.x & 63) >> 5;
     const Rows32 w(d, j);
     const KeyTiles<TYPE, DK, DV> keys(d, j);
+    const Reader<M, 2 * DK> kread;
+    const Reader<M, DV> vread;
     const float c = d.scale * DA_LOG2E;
     const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
 
@@ -583,11 +655,11 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
             floatx16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
             for (int i = 0; i < Ge::NK; ++i) {
-                s1 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, 0, i), q[0][i], s1);
-                s2 = M::mma(lds_frag<M, 2 * DK>(kt, 32 * sub, DK / M::E, i), q[1][i], s2);
+                s1 = M::mma(kread.rows(kt, 32 * sub, i), q[0][i], s1);
+                s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q[1][i], s2);
             }
 #pragma unroll
-            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(lds_frag<M, DV>(vt, 32 * sub, 0, i), g[i], dp);
+            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g[i], dp);
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -614,7 +686,7 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
                 const Frag p1 = acc_frag<M>(s1, i), p2 = acc_frag<M>(s2, i);
 #pragma unroll
                 for (int n = 0; n < DK / 32; ++n) {
-                    const Frag f1 = lds_frag_t<M, 2 * DK>(kt, 32 * sub, 32 * n, i), f2 = lds_frag_t<M, 2 * DK>(kt, 32 * sub, DK + 32 * n, i);
+                    const Frag f1 = kread.cols(kt, 32 * sub, 32 * n, i), f2 = kread.cols(kt, 32 * sub, DK + 32 * n, i);
                     a1[n] = M::mma(f1, p1, a1[n]);
                     a2[n] = M::mma(f2, p2, a2[n]);
                     if constexpr (CORR) {
@@ -680,32 +752,29 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_d
 
     const MEP_G T* qb = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)j.g * j.n * d.q_sH;
     const MEP_G T* ob = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
+    const Reader<M, 2 * DK> qread;
+    const Reader<M, DV> oread;
+    const Stager<M, RT, 2 * DK> qs((unsigned)d.q_sT, [&](int ch) {
+        const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
+        return col < d.d ? col + (m ? (int)d.q_sM : 0) : -1;
+    });
+    const Stager<M, RT, DV> os((unsigned)bd.o_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
     auto load_rows = [&](int buf, int r0) {
-        const int t0 = r0 / j.n, x0 = r0 - t0 * j.n;      // the tile's first query and its first head there
-        auto place = [&](int r, int& t, int& x) {
-            t = 0;
-            x = 0;
-            if (j.n == 1) t = r;
-            else {
-                const unsigned y = (unsigned)(x0 + r);
-                t = (int)(y / (unsigned)j.n);
-                x = (int)y - t * j.n;
-            }
-        };
-        constexpr int CK = DK / M::E;
-        stage<M, RT, 2 * DK>(Buf + buf * Ge::TSZ, qb + (int64_t)t0 * d.q_sT, [&](int r, int ch, unsigned& off) {
-            const int m = ch >= CK, col = (ch - m * CK) * M::E;
-            int t, x;
-            place(r, t, x);
-            off = (unsigned)t * (unsigned)d.q_sT + (unsigned)x * (unsigned)d.q_sH + col + (m ? (unsigned)d.q_sM : 0u);
-            return col < d.d && r0 + r < j.rows;
-        });
-        stage<M, RT, DV>(Buf + buf * Ge::TSZ + Ge::KSZ, ob + (int64_t)t0 * bd.o_sT, [&](int r, int ch, unsigned& off) {
-            int t, x;
-            place(r, t, x);
-            off = (unsigned)t * (unsigned)bd.o_sT + (unsigned)x * (unsigned)bd.o_sH + ch * M::E;
-            return ch * M::E < d.dv && r0 + r < j.rows;
-        });
+        T* tile = Buf + buf * Ge::TSZ;
+        if (j.n == 1) {
+            const int left = j.rows - r0;
+            const unsigned long long bits = left >= 64 ? ~0ull : (1ull << left) - 1;
+            qs.load(tile, qb + r0 * d.q_sT, (unsigned)d.q_sT, RT == 64 ? bits : bits & 0xffffffffull);
+            os.load(tile + Ge::KSZ, ob + r0 * bd.o_sT, (unsigned)bd.o_sT, RT == 64 ? bits : bits & 0xffffffffull);
+        } else {      // shared heads: a tile's rows are some heads of some queries
+            const int t0 = r0 / j.n, x0 = r0 - t0 * j.n;
+            auto at = [&](int r, int64_t sT, int64_t sH) {
+                const unsigned y = (unsigned)(x0 + r), t = y / (unsigned)j.n;
+                return r0 + r < j.rows ? (int)(t * (unsigned)sT + (y - t * (unsigned)j.n) * (unsigned)sH) : -1;
+            };
+            qs.gather(tile, qb + t0 * d.q_sT, (unsigned)d.q_sT, [&](int r) { return at(r, d.q_sT, d.q_sH); });
+            os.gather(tile + Ge::KSZ, ob + t0 * bd.o_sT, (unsigned)bd.o_sT, [&](int r) { return at(r, bd.o_sT, bd.o_sH); });
+        }
     };
     f32x4 sv = {0.f, 0.f, 0.f, 0.f}, dv4 = sv;      // a row's statistics on their way to LDS: past the end A = 0
     float lv = 0.f;
@@ -779,13 +848,13 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_d
 #pragma unroll
             for (int i = 0; i < Ge::NK; ++i) {
                 const Frag k1 = KREG ? kr[0][KREG ? i : 0] : load_k(0, i), k2 = KREG ? kr[1][KREG ? i : 0] : load_k(1, i);
-                s1 = M::mma(lds_frag<M, 2 * DK>(qt, 32 * sub, 0, i), k1, s1);
-                s2 = M::mma(lds_frag<M, 2 * DK>(qt, 32 * sub, DK / M::E, i), k2, s2);
+                s1 = M::mma(qread.rows(qt, 32 * sub, i), k1, s1);
+                s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), k2, s2);
             }
 #pragma unroll
             for (int i = 0; i < Ge::NV; ++i) {
                 const Frag v = KREG ? vr[KREG ? i : 0] : load_v(i);
-                dp = M::mma(lds_frag<M, DV>(ot, 32 * sub, 0, i), v, dp);
+                dp = M::mma(oread.rows(ot, 32 * sub, i), v, dp);
             }
             if (!all_on || rs < wfull || d.mask_form == 2) {      // rows that see this lane's key: those from rmin on
                 const int least = rmin - rs - 4 * h;
@@ -817,11 +886,11 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_d
             for (int i = 0; i < Ge::NP; ++i) {
                 const Frag fp = acc_frag<M>(p, i), f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
 #pragma unroll
-                for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(lds_frag_t<M, DV>(ot, 32 * sub, 32 * n, i), fp, av[n]);
+                for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), fp, av[n]);
 #pragma unroll
                 for (int n = 0; n < DK / 32; ++n) {
-                    ak1[n] = M::mma(lds_frag_t<M, 2 * DK>(qt, 32 * sub, 32 * n, i), f1, ak1[n]);
-                    ak2[n] = M::mma(lds_frag_t<M, 2 * DK>(qt, 32 * sub, DK + 32 * n, i), f2, ak2[n]);
+                    ak1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, ak1[n]);
+                    ak2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, ak2[n]);
                 }
             }
         }
