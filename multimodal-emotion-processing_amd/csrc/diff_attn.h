@@ -106,7 +106,9 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // waits for these.  The loads return no registers; m0 has no other user in these kernels.
 MEP_DEV void dma16(const void* dst, unsigned off, i32x4 rs, unsigned soff) {
     const unsigned at = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const da_lds_char*)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(off), "s"(rs), "s"(soff) : "memory");
+    soff = __builtin_amdgcn_readfirstlane((int)soff);
+    // 5 wait states between a readfirstlane and a memory instruction that reads its result, 1 behind m0
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(off), "s"(rs), "s"(soff) : "memory");
 }
 // a raw buffer of DA_SPAN bytes from p on
 MEP_DEV i32x4 da_buffer(const MEP_G void* p) {
@@ -115,13 +117,14 @@ MEP_DEV i32x4 da_buffer(const MEP_G void* p) {
 }
 
 // ROWS x COLS of LDS from rows of global memory, by DMA: an instruction of a wave fills 64 chunks, and instruction i of a
-// lane takes chunk `chunk(i)` of row `row + i STEP`.  The chunk does not depend on i (but for rows of 64 chunks, on its
-// parity), so neither does the lane's offset, and a tile costs no address arithmetic: the row steps are the scalar offset.
-template <class M, int ROWS, int COLS>
+// lane takes chunk `chunk(i)` of row `row + i STEP`.  The chunk does not depend on i (with 4 rows a step, on its
+// parity alone), so neither does the lane's offset, and a tile costs no address arithmetic: the row steps are the scalar offset.
+template <class M, int ROWS, int COLS, int THREADS = DA_THREADS>
 struct Stager {
     typedef Lay<M, COLS> L;
     typedef typename M::T T;
-    static constexpr int STEP = DA_THREADS / L::CH, N = ROWS / STEP, NO = L::CH > 32 ? 2 : 1;
+    static constexpr int STEP = THREADS / L::CH < ROWS ? THREADS / L::CH : ROWS, N = ROWS / STEP, NO = STEP % 8 ? 2 : 1;
+    static constexpr bool ALL = STEP * L::CH == THREADS;      // else only the first waves load
     static_assert(STEP >= 4 && ROWS % STEP == 0, "tile");
     int row;
     unsigned off[NO];                // byte offset of the lane's chunk in row `row`, or DA_NOWHERE
@@ -143,25 +146,27 @@ struct Stager {
     // their contents, NaN too, never enter a product.
     MEP_DEV void load(T* dst, const MEP_G T* base, unsigned stride, unsigned long long bits) const {
         const i32x4 rs = da_buffer(base);
+        if (!ALL && threadIdx.x >= STEP * L::CH) return;
         const bool full = bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1);
         T* mine = dst + (threadIdx.x >> 6) * 64 * M::E;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             unsigned o = off[i % NO];
             if (!full && !(bits >> (row + i * STEP) & 1)) o = DA_NOWHERE;
-            dma16(mine + i * DA_THREADS * M::E, o, rs, i * STEP * stride * (unsigned)sizeof(T));
+            dma16(mine + i * THREADS * M::E, o, rs, i * STEP * stride * (unsigned)sizeof(T));
         }
     }
     // rows at any places: at(r): element offset of tile row r, or -1
     template <class F>
     MEP_DEV void gather(T* dst, const MEP_G T* base, unsigned stride, F at) const {
+        if (!ALL && threadIdx.x >= STEP * L::CH) return;
         const i32x4 rs = da_buffer(base);
         T* mine = dst + (threadIdx.x >> 6) * 64 * M::E;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int o = at(row + i * STEP);
             const unsigned c = off[i % NO];
-            dma16(mine + i * DA_THREADS * M::E, o < 0 || c == DA_NOWHERE ? DA_NOWHERE : c + (unsigned)(o - row * (int)stride) * (unsigned)sizeof(T), rs, 0);
+            dma16(mine + i * THREADS * M::E, o < 0 || c == DA_NOWHERE ? DA_NOWHERE : c + (unsigned)(o - row * (int)stride) * (unsigned)sizeof(T), rs, 0);
         }
     }
 };
@@ -457,7 +462,9 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
     }
     const float lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
 
-    float m1 = mul_rn(DA_MIN, c), m2 = m1, l1 = 0.f, l2 = 0.f, top1 = DA_MIN, top2 = DA_MIN, f1 = 1.f, f2 = 0.f;
+    // The backward's e_m are to be at most 1: it gets maxima 8 up, or in float16, whose subnormals begin at 2^-14, the true ones
+    constexpr bool TOP = TYPE == MEP_F16;
+    float m1 = mul_rn(DA_MIN, c), m2 = m1, l1 = 0.f, l2 = 0.f, f1 = 1.f, f2 = 0.f, top1 = DA_MIN, top2 = DA_MIN;
     floatx16 x[DV / 32], y[DV / 32];
 #pragma unroll
     for (int n = 0; n < DV / 32; ++n) x[n] = y[n] = zero16();
@@ -484,10 +491,12 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
             }
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
             const float a1 = max16(s1), a2 = max16(s2);
-            top1 = fmaxf(top1, a1);
-            top2 = fmaxf(top2, a2);
+            if constexpr (TOP) {
+                top1 = fmaxf(top1, a1);
+                top2 = fmaxf(top2, a2);
+            }
             if (__ballot(a1 * c > m1 + 8.f || a2 * c > m2 + 8.f)) {
-                const float n1 = fmaxf(m1, mul_rn(half_max(top1), c)), n2 = fmaxf(m2, mul_rn(half_max(top2), c));
+                const float n1 = fmaxf(m1, mul_rn(half_max(a1), c)), n2 = fmaxf(m2, mul_rn(half_max(a2), c));
                 const float g1 = exp2_fast(m1 - n1), g2 = exp2_fast(m2 - n2);
                 l1 *= g1;
                 l2 *= g2;
@@ -534,12 +543,11 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
             }
         }
     }
-    // the row's sums over both lane halves, and its true maxima (the backward's e_m are then at most 1)
     l1 = half_sum(l1);
     l2 = half_sum(l2);
     const float i1 = l1 > 0.f ? 1.f / l1 : l1, i2 = l2 > 0.f ? 1.f / l2 : l2;
-    // one rounding each, as m1 and m2 have: without keys the differences below are 0
-    const float n1 = mul_rn(half_max(top1), c), n2 = mul_rn(half_max(top2), c);
+    // (one rounding, as m1 and m2 have: without keys the differences are 0)
+    const float n1 = TOP ? mul_rn(half_max(top1), c) : m1 + 8.f, n2 = TOP ? mul_rn(half_max(top2), c) : m2 + 8.f;
     if (d.stats && w.live && h == 0)
         *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) =
             f32x4{n1, i1 * exp2_fast(n1 - m1), n2, i2 * exp2_fast(n2 - m2)};
@@ -562,12 +570,14 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
 }
 
 // ------------------------------------------------------------------ backward: D and dq
-// D_m = dO . (A_m v) is known from the forward's out and second = A_2 v only up to their roundings, which would be an error of
-// the size of dS where few keys carry a row.  So dS is formed with that estimate, the row sums of A_m dP are formed beside it
-// without any rounding to 16 bits, and their difference is put right at the end: dq_m -= (D_m - estimate) A_m k_m, for which
-// E_m k_m is summed too (CORR; in fp32 the estimate is as good as the sum).  The sums are also lam's gradient and what dk needs.
+// D_m = dO . (A_m v) is known beforehand only up to the roundings of the forward's out and second = A_2 v.  That error is some
+// 2^-9 of the sum of A_m^2 of the row in dP's units: nothing beside dS's own rounding where many keys carry the row, but all of dS
+// where one does.  So the row sums of A_m dP are formed beside dS without any rounding to 16 bits, and where a row of the
+// workgroup rests on fewer than 16 keys (sum A_m^2 > 1 / 16), a second pass over the keys forms A_m k_m and puts their difference
+// right: dq_m -= (D_m - estimate) A_m k_m.  (In fp32 the estimate is as good as the sum.)  The sums are also lam's gradient and
+// what dk needs.
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
+__global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
@@ -630,13 +640,10 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
     const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * srow);      // m1, 1 / l1, m2, 1 / l2
 
     constexpr bool CORR = TYPE != MEP_F32;
-    float sum1 = 0.f, sum2 = 0.f;
-    floatx16 a1[DK / 32], a2[DK / 32], k1[CORR ? DK / 32 : 1], k2[CORR ? DK / 32 : 1];
+    float sum1 = 0.f, sum2 = 0.f, sq1 = 0.f, sq2 = 0.f;
+    floatx16 a1[DK / 32], a2[DK / 32];
 #pragma unroll
-    for (int n = 0; n < DK / 32; ++n) {
-        a1[n] = a2[n] = zero16();
-        if constexpr (CORR) k1[n] = k2[n] = zero16();
-    }
+    for (int n = 0; n < DK / 32; ++n) a1[n] = a2[n] = zero16();
     for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
         tile_sync();
         const unsigned long long now = bits;
@@ -662,37 +669,24 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
             for (int i = 0; i < Ge::NV; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g[i], dp);
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s1[r] = exp2_fast(fmaf(s1[r], c, -st[0]));
-                s2[r] = exp2_fast(fmaf(s2[r], c, -st[2]));
-                sum1 = fmaf(s1[r], dp[r], sum1);
-                sum2 = fmaf(s2[r], dp[r], sum2);
-            }
-            Frag e1[CORR ? Ge::NP : 1], e2[CORR ? Ge::NP : 1];
-            if constexpr (CORR) {
-#pragma unroll
-                for (int i = 0; i < Ge::NP; ++i) {
-                    e1[i] = acc_frag<M>(s1, i);
-                    e2[i] = acc_frag<M>(s2, i);
+            for (int r = 0; r < 16; ++r) {      // e_m, the row sums, and dS_m without the row's factors 1 / l1, -lam / l2
+                const float e1 = exp2_fast(fmaf(s1[r], c, -st[0])), e2 = exp2_fast(fmaf(s2[r], c, -st[2]));
+                sum1 = fmaf(e1, dp[r], sum1);
+                sum2 = fmaf(e2, dp[r], sum2);
+                if constexpr (CORR) {
+                    sq1 = fmaf(e1, e1, sq1);
+                    sq2 = fmaf(e2, e2, sq2);
                 }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {      // dS_m without the row's factors 1 / l1, -lam / l2
-                s1[r] *= dp[r] - d1;
-                s2[r] *= dp[r] - d2;
+                s1[r] = e1 * (dp[r] - d1);
+                s2[r] = e2 * (dp[r] - d2);
             }
 #pragma unroll
             for (int i = 0; i < Ge::NP; ++i) {
                 const Frag p1 = acc_frag<M>(s1, i), p2 = acc_frag<M>(s2, i);
 #pragma unroll
                 for (int n = 0; n < DK / 32; ++n) {
-                    const Frag f1 = kread.cols(kt, 32 * sub, 32 * n, i), f2 = kread.cols(kt, 32 * sub, DK + 32 * n, i);
-                    a1[n] = M::mma(f1, p1, a1[n]);
-                    a2[n] = M::mma(f2, p2, a2[n]);
-                    if constexpr (CORR) {
-                        k1[n] = M::mma(f1, e1[i], k1[n]);
-                        k2[n] = M::mma(f2, e2[i], k2[n]);
-                    }
+                    a1[n] = M::mma(kread.cols(kt, 32 * sub, 32 * n, i), p1, a1[n]);
+                    a2[n] = M::mma(kread.cols(kt, 32 * sub, DK + 32 * n, i), p2, a2[n]);
                 }
             }
         }
@@ -704,16 +698,55 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
         if (bd.dlam_rows) G<float>(bd.dlam_rows)[((int64_t)j.b * d.Tq + w.t) * d.H + w.head] = -sum2;
     }
     if (!bd.dq) return;
-    tile_sync();                             // the tiles are free
     if constexpr (CORR) {
+        const bool few = w.live && fmaxf(half_sum(sq1) * st[1] * st[1], half_sum(sq2) * st[3] * st[3]) > 0.0625f;
+        if (__syncthreads_or(few)) {
+            floatx16 k1[DK / 32], k2[DK / 32];
 #pragma unroll
-        for (int n = 0; n < DK / 32; ++n)
+            for (int n = 0; n < DK / 32; ++n) k1[n] = k2[n] = zero16();
+            for (int k0 = 0; k0 < end; k0 += KT) {      // one buffer: this pass is the rare one
+                bits = key_bits(d, j, k0, KT, key_raw(d, j, k0));
+                tile_sync();
+                keys.ks.load(Buf, keys.kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
+                tile_sync();
+#pragma unroll 1
+                for (int sub = 0; sub < KT / 32; ++sub) {
+                    const int ks = k0 + 32 * sub;
+                    const unsigned on = (unsigned)(bits >> (32 * sub));
+                    if (ks >= w.wend || !on) continue;
+                    floatx16 s1 = zero16(), s2 = zero16();
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                a1[n][r] = fmaf(k1[n][r], d1 - sum1, a1[n][r]);
-                a2[n][r] = fmaf(k2[n][r], d2 - sum2, a2[n][r]);
+                    for (int i = 0; i < Ge::NK; ++i) {
+                        s1 = M::mma(kread.rows(Buf, 32 * sub, i), q[0][i], s1);
+                        s2 = M::mma(kread.rows(Buf, 32 * sub, Ge::NK + i), q[1][i], s2);
+                    }
+                    if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s1[r] = exp2_fast(fmaf(s1[r], c, -st[0]));
+                        s2[r] = exp2_fast(fmaf(s2[r], c, -st[2]));
+                    }
+#pragma unroll
+                    for (int i = 0; i < Ge::NP; ++i) {
+                        const Frag p1 = acc_frag<M>(s1, i), p2 = acc_frag<M>(s2, i);
+#pragma unroll
+                        for (int n = 0; n < DK / 32; ++n) {
+                            k1[n] = M::mma(kread.cols(Buf, 32 * sub, 32 * n, i), p1, k1[n]);
+                            k2[n] = M::mma(kread.cols(Buf, 32 * sub, DK + 32 * n, i), p2, k2[n]);
+                        }
+                    }
+                }
             }
+#pragma unroll
+            for (int n = 0; n < DK / 32; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    a1[n][r] = fmaf(k1[n][r], d1 - sum1, a1[n][r]);
+                    a2[n][r] = fmaf(k2[n][r], d2 - sum2, a2[n][r]);
+                }
+        }
     }
+    tile_sync();                             // the tiles are free
     const int64_t first = (int64_t)j.b * d.Tq * d.H * 2 * d.d;
     auto row_at = [&](int m, int r) -> MEP_G T* {
         const int row = w.row0 + r;
@@ -727,45 +760,88 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
 }
 
 // ------------------------------------------------------------------ backward: dk and dv
-// A wave owns 32 keys (an accumulator column each) and walks the rows; KREG: its K and V operands stay in registers.
-template <int TYPE, int DK, int DV, bool KREG>
-__global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks) {
+// A workgroup walks the rows of 32 KW keys.  Of its 2 KW waves one half forms dv (an accumulator column per key), the other dk: each
+// needs the scores, but so neither holds more than 256 registers and two waves share a SIMD (in one wave, the accumulators of
+// both pass through the accumulation registers and back for every tile: 335 us against 241 at B 2, T 4096, 8 heads, 64 / 128, causal).
+//
+// The scores lie rows x keys here, so a row's statistics are not a lane's.  They come in as a product: the accumulator starts
+// at X 1 with X the row's value in three bf16 parts (24 bits) against a column of ones, one instruction for 16 registers.  With
+//   s' = s - lse_m / c, lse_1 = m_1 + log2 l_1, lse_2 = m_2 + log2 l_2 - log2 |lam|:   2^(c s') = A_1, |lam| A_2
+//   dP' = dP - D_1, and D_1 - D_2 added for the second map
+// the rest is a product and an exponential each.  (lse_m folds a sum into the maximum: its last bits are below those that s has.)
+template <int KW, int TYPE, int DK, int DV>
+struct KvShape {
     typedef Geo<TYPE, DK, DV> Ge;
+    static constexpr int THREADS = 128 * KW, KEYS = 32 * KW;
+    static constexpr int OUT = KEYS * (DK + DV + 2 * Ge::M::E), BUF = 2 * Ge::TSZ > OUT ? 2 * Ge::TSZ : OUT;
+};
+
+typedef __bf16 bf16x8_da __attribute__((ext_vector_type(8)));
+enum { X_LSE1, X_LSE2, X_D1, X_D12, X_SIGN, X_COUNT };
+
+// -v, in three parts that sum to it to 24 bits, as the k = 0, 1, 2 of an operand
+MEP_DEV bf16x8_da parts3(float v) {
+    bf16x8_da x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (__bf16)0.f;
+    v = -v;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        x[i] = (__bf16)v;
+        v = sub_rn(v, (float)x[i]);
+    }
+    return x;
+}
+// the 32 rows' values x[0 .. 31], each in its row of an accumulator
+MEP_DEV floatx16 row_values(const bf16x8_da* x) {
+    const int lane = threadIdx.x & 63;
+    bf16x8_da ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)(i < 3 && lane < 32 ? 1.f : 0.f);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[lane & 31], ones, zero16(), 0, 0, 0);
+}
+
+template <int KW, int TYPE, int DK, int DV>
+__global__ __launch_bounds__(128 * KW, KW / 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks) {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef KvShape<KW, TYPE, DK, DV> Sh;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
     typedef typename Ge::Frag Frag;
-    constexpr int RT = Ge::KT;
+    constexpr int RT = Ge::KT, THREADS = Sh::THREADS;
     const mep_diff_attn_desc& d = bd.f;
-    __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their queries, then their upstream gradients
-    __shared__ __align__(16) float Rs[2][6][RT];      // a row's m1, m2, i1, lam i2, i1 D1, lam i2 D2
-    __shared__ int Ts[2][RT];                         // and its query
+    __shared__ __align__(16) T Buf[Sh::BUF];      // two tiles: their queries, then their upstream gradients
+    __shared__ bf16x8_da Xs[2][X_COUNT][RT];      // and their rows' values
+    __shared__ int Ts[2][RT];                     // and queries
+    __shared__ int Neg[2];                        // whether any lam of the tile is negative
     const Job j = make_job(d, blocks, false);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int key0 = j.block * DA_ROWS + wave * 32, key = key0 + (lane & 31);
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+    const bool for_v = wave < KW;
+    const int key0 = j.block * Sh::KEYS + wave % KW * 32, key = key0 + (lane & 31);
     const float c = d.scale * DA_LOG2E;
-    // rows that see any of the block's / the wave's keys; every one of the wave's keys: from row wfull on
-    const int bstart = d.causal ? max(0, min(d.Tq, j.block * DA_ROWS - j.first)) * j.n : 0;
+    // rows that see any of the block's / the wave's keys; every one of the wave's keys: from row wfull on; the lane's key: from rmin on
+    const int bstart = d.causal ? max(0, min(d.Tq, j.block * Sh::KEYS - j.first)) * j.n : 0;
     const int wstart = d.causal ? max(0, min(d.Tq, key0 - j.first)) * j.n : 0;
     const int wfull = d.causal ? max(0, min(d.Tq, key0 + 31 - j.first)) * j.n : 0;
-    const int rmin = d.causal ? max(0, min(d.Tq, key - j.first)) * j.n : 0;      // the lane's key's first row
-    const int rend = j.block * DA_ROWS < j.len ? j.rows : 0;
+    const int rmin = d.causal ? max(0, min(d.Tq, key - j.first)) * j.n : 0;
+    const int rend = j.block * Sh::KEYS < j.len ? j.rows : 0;
 
     const MEP_G T* qb = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)j.g * j.n * d.q_sH;
     const MEP_G T* ob = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
     const Reader<M, 2 * DK> qread;
     const Reader<M, DV> oread;
-    const Stager<M, RT, 2 * DK> qs((unsigned)d.q_sT, [&](int ch) {
+    const Stager<M, RT, 2 * DK, THREADS> qs((unsigned)d.q_sT, [&](int ch) {
         const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
         return col < d.d ? col + (m ? (int)d.q_sM : 0) : -1;
     });
-    const Stager<M, RT, DV> os((unsigned)bd.o_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
+    const Stager<M, RT, DV, THREADS> os((unsigned)bd.o_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
     auto load_rows = [&](int buf, int r0) {
         T* tile = Buf + buf * Ge::TSZ;
         if (j.n == 1) {
             const int left = j.rows - r0;
-            const unsigned long long bits = left >= 64 ? ~0ull : (1ull << left) - 1;
-            qs.load(tile, qb + r0 * d.q_sT, (unsigned)d.q_sT, RT == 64 ? bits : bits & 0xffffffffull);
-            os.load(tile + Ge::KSZ, ob + r0 * bd.o_sT, (unsigned)bd.o_sT, RT == 64 ? bits : bits & 0xffffffffull);
+            const unsigned long long bits = left >= RT ? (RT == 64 ? ~0ull : 0xffffffffull) : (1ull << left) - 1;
+            qs.load(tile, qb + r0 * d.q_sT, (unsigned)d.q_sT, bits);
+            os.load(tile + Ge::KSZ, ob + r0 * bd.o_sT, (unsigned)bd.o_sT, bits);
         } else {      // shared heads: a tile's rows are some heads of some queries
             const int t0 = r0 / j.n, x0 = r0 - t0 * j.n;
             auto at = [&](int r, int64_t sT, int64_t sH) {
@@ -776,9 +852,10 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_d
             os.gather(tile + Ge::KSZ, ob + t0 * bd.o_sT, (unsigned)bd.o_sT, [&](int r) { return at(r, bd.o_sT, bd.o_sH); });
         }
     };
-    f32x4 sv = {0.f, 0.f, 0.f, 0.f}, dv4 = sv;      // a row's statistics on their way to LDS: past the end A = 0
-    float lv = 0.f;
-    int tv = 0;
+    // the rows' statistics on their way to LDS, a row per thread of the first wave
+    f32x4 sv, dv4;
+    float lv;
+    int tv;
     auto fetch_stats = [&](int r0) {
         const int row = r0 + threadIdx.x;
         sv = dv4 = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -794,15 +871,20 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_d
         }
     };
     auto put_stats = [&](int buf) {
-        if (threadIdx.x < RT) {
+        if (threadIdx.x < 64) {
+            const bool neg = __ballot(threadIdx.x < RT && lv < 0.f) != 0;
             const int i = threadIdx.x;
-            Rs[buf][0][i] = sv[0];
-            Rs[buf][1][i] = sv[2];
-            Rs[buf][2][i] = sv[1];
-            Rs[buf][3][i] = lv * sv[3];
-            Rs[buf][4][i] = sv[1] * dv4[0];
-            Rs[buf][5][i] = lv * sv[3] * dv4[1];
-            Ts[buf][i] = tv;
+            if (i < RT) {
+                // without keys, past the end (1 / l = 0) and for lam = 0: A = 0
+                const float al = fabsf(lv) * sv[3];
+                Xs[buf][X_LSE1][i] = parts3(sv[1] > 0.f || sv[1] != sv[1] ? (sv[0] - __log2f(sv[1])) / c : -DA_MIN);
+                Xs[buf][X_LSE2][i] = parts3(al > 0.f || al != al ? (sv[2] - __log2f(al)) / c : -DA_MIN);
+                Xs[buf][X_D1][i] = parts3(dv4[0]);
+                Xs[buf][X_D12][i] = parts3(dv4[1] - dv4[0]);
+                if (neg) Xs[buf][X_SIGN][i] = parts3(lv < 0.f ? 1.f : -1.f);
+                Ts[buf][i] = tv;
+            }
+            if (i == 0) Neg[buf] = neg;
         }
     };
     const int rbeg = bstart / RT * RT;
@@ -812,113 +894,144 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 128 || DK >= 64 ? 1 : 2) void k_d
     }
     bool on = key < j.len;
     if (on && d.mask_form == 1) on = mask_at(d, (int64_t)j.b * d.m_sB + (int64_t)key * d.m_sK);
-    const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH + (int64_t)(on ? key : 0) * d.k_sT;
-    const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH + (int64_t)(on ? key : 0) * d.v_sT;
-    auto load_k = [&](int m, int i) { return row_frag<M>(kp + m * d.k_sM, M::KS * i + M::E * h, d.d, on); };
-    auto load_v = [&](int i) { return row_frag<M>(vp, M::KS * i + M::E * h, d.dv, on); };
-    Frag kr[2][KREG ? Ge::NK : 1], vr[KREG ? Ge::NV : 1];
-    if constexpr (KREG) {
+    const int64_t krow = on ? key : 0;
+    const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH + krow * d.k_sT;
+    const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH + krow * d.v_sT;
+    Frag kr[2][Ge::NK];
 #pragma unroll
-        for (int i = 0; i < Ge::NK; ++i) { kr[0][i] = load_k(0, i); kr[1][i] = load_k(1, i); }
-#pragma unroll
-        for (int i = 0; i < Ge::NV; ++i) vr[i] = load_v(i);
+    for (int i = 0; i < Ge::NK; ++i) {
+        kr[0][i] = row_frag<M>(kp, M::KS * i + M::E * h, d.d, on);
+        kr[1][i] = row_frag<M>(kp + d.k_sM, M::KS * i + M::E * h, d.d, on);
     }
-    floatx16 ak1[DK / 32], ak2[DK / 32], av[DV / 32];
-#pragma unroll
-    for (int n = 0; n < DK / 32; ++n) ak1[n] = ak2[n] = zero16();
-#pragma unroll
-    for (int n = 0; n < DV / 32; ++n) av[n] = zero16();
     const bool wave_on = __ballot(on) != 0, all_on = __ballot(on) == ~0ull;
     if (rbeg < rend) put_stats(0);
 
-    for (int r0 = rbeg, buf = 0; r0 < rend; r0 += RT, buf ^= 1) {
-        tile_sync();
-        const bool more = r0 + RT < rend;
-        if (more) {
-            load_rows(buf ^ 1, r0 + RT);
-            fetch_stats(r0 + RT);
-        }
+    // A_1 and lam A_2 of the rows from rs on
+    auto maps = [&](int buf, int sub, int rs, floatx16& s1, floatx16& s2) {
         const T* qt = Buf + buf * Ge::TSZ;
-        const T* ot = qt + Ge::KSZ;
-#pragma unroll 1
-        for (int sub = 0; sub < RT / 32; ++sub) {
-            const int rs = r0 + 32 * sub;
-            if (!wave_on || rs >= j.rows || rs + 32 <= wstart) continue;
-            floatx16 s1 = zero16(), s2 = zero16(), dp = zero16();
+        s1 = row_values(Xs[buf][X_LSE1] + 32 * sub);
+        s2 = row_values(Xs[buf][X_LSE2] + 32 * sub);
 #pragma unroll
-            for (int i = 0; i < Ge::NK; ++i) {
-                const Frag k1 = KREG ? kr[0][KREG ? i : 0] : load_k(0, i), k2 = KREG ? kr[1][KREG ? i : 0] : load_k(1, i);
-                s1 = M::mma(qread.rows(qt, 32 * sub, i), k1, s1);
-                s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), k2, s2);
+        for (int i = 0; i < Ge::NK; ++i) {
+            s1 = M::mma(qread.rows(qt, 32 * sub, i), kr[0][i], s1);
+            s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), kr[1][i], s2);
+        }
+        if (!all_on || rs < wfull || d.mask_form == 2) {      // rows that see this lane's key: those from rmin on
+            const int least = rmin - rs - 4 * h;
+            unsigned ok = !on || least > 31 ? 0u : least > 0 ? ~0u << least : ~0u;
+            if (d.mask_form == 2) {
+                const int64_t o = (int64_t)j.b * d.m_sB + (int64_t)min(key, d.Tk - 1) * d.m_sK;
+                unsigned keep = 0;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    keep |= (mask_at(d, o + (int64_t)Ts[buf][32 * sub + acc_off(r) + 4 * h] * d.m_sQ) ? 1u : 0u) << acc_off(r);
+                ok &= keep;
             }
-#pragma unroll
-            for (int i = 0; i < Ge::NV; ++i) {
-                const Frag v = KREG ? vr[KREG ? i : 0] : load_v(i);
-                dp = M::mma(oread.rows(ot, 32 * sub, i), v, dp);
-            }
-            if (!all_on || rs < wfull || d.mask_form == 2) {      // rows that see this lane's key: those from rmin on
-                const int least = rmin - rs - 4 * h;
-                unsigned ok = !on || least > 31 ? 0u : least > 0 ? ~0u << least : ~0u;
-                if (d.mask_form == 2) {
-                    const int64_t o = (int64_t)j.b * d.m_sB + (int64_t)min(key, d.Tk - 1) * d.m_sK;
-                    unsigned keep = 0;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        keep |= (mask_at(d, o + (int64_t)Ts[buf][32 * sub + acc_off(r) + 4 * h] * d.m_sQ) ? 1u : 0u) << acc_off(r);
-                    ok &= keep;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s1[r] = ok >> acc_off(r) & 1 ? s1[r] : -INFINITY;
-                    s2[r] = ok >> acc_off(r) & 1 ? s2[r] : -INFINITY;
-                }
-            }
-            floatx16 p;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int lr = 32 * sub + acc_off(r) + 4 * h;
-                const float x1 = exp2_fast(fmaf(s1[r], c, -Rs[buf][0][lr])), x2 = exp2_fast(fmaf(s2[r], c, -Rs[buf][1][lr]));
-                p[r] = x1 * Rs[buf][2][lr] - x2 * Rs[buf][3][lr];
-                s1[r] = x1 * fmaf(dp[r], Rs[buf][2][lr], -Rs[buf][4][lr]);
-                s2[r] = x2 * fmaf(dp[r], -Rs[buf][3][lr], Rs[buf][5][lr]);
-            }
-#pragma unroll
-            for (int i = 0; i < Ge::NP; ++i) {
-                const Frag fp = acc_frag<M>(p, i), f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
-#pragma unroll
-                for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), fp, av[n]);
-#pragma unroll
-                for (int n = 0; n < DK / 32; ++n) {
-                    ak1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, ak1[n]);
-                    ak2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, ak2[n]);
-                }
+                s1[r] = ok >> acc_off(r) & 1 ? s1[r] : -INFINITY;
+                s2[r] = ok >> acc_off(r) & 1 ? s2[r] : -INFINITY;
             }
         }
-        if (more) put_stats(buf ^ 1);
-    }
-    tile_sync();                             // the tiles are free
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s1[r] = exp2_fast(s1[r] * c);
+            s2[r] = exp2_fast(s2[r] * c);
+        }
+        if (Neg[buf]) {
+            const floatx16 sg = row_values(Xs[buf][X_SIGN] + 32 * sub);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s2[r] *= sg[r];
+        }
+    };
+    auto walk = [&](auto step) {
+        for (int r0 = rbeg, buf = 0; r0 < rend; r0 += RT, buf ^= 1) {
+            tile_sync();
+            const bool more = r0 + RT < rend;
+            if (more) {
+                load_rows(buf ^ 1, r0 + RT);
+                fetch_stats(r0 + RT);
+            }
+#pragma unroll 1
+            for (int sub = 0; sub < RT / 32; ++sub) {
+                const int rs = r0 + 32 * sub;
+                if (wave_on && rs < j.rows && rs + 32 > wstart) step(buf, sub, rs);
+            }
+            if (more) put_stats(buf ^ 1);
+        }
+        tile_sync();                         // the tiles are free
+    };
     // masked keys and keys past the lengths get zeros
     const int64_t first = (int64_t)j.b * d.Tk * d.G + j.g;
     auto key_at = [&](uint64_t p, int r, int64_t width) -> MEP_G T* {
         return key0 + r < d.Tk ? G<T>(p) + (first + (int64_t)(key0 + r) * d.G) * width : nullptr;
     };
-    T* mine = Buf + wave * 32 * ((DK > DV ? DK : DV) + M::E);
-    write_rows<M>(mine, ak1, d.scale, d.d, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
-    write_rows<M>(mine, ak2, d.scale, d.d, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
-    write_rows<M>(mine, av, 1.f, d.dv, [&](int r) { return key_at(bd.dv, r, d.dv); });
+    if (for_v) {
+        floatx16 av[DV / 32];
+#pragma unroll
+        for (int n = 0; n < DV / 32; ++n) av[n] = zero16();
+        walk([&](int buf, int sub, int rs) {
+            floatx16 s1, s2;
+            maps(buf, sub, rs, s1, s2);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s1[r] -= s2[r];
+            const T* ot = Buf + buf * Ge::TSZ + Ge::KSZ;
+#pragma unroll
+            for (int i = 0; i < Ge::NP; ++i) {
+                const Frag p = acc_frag<M>(s1, i);
+#pragma unroll
+                for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), p, av[n]);
+            }
+        });
+        write_rows<M>(Buf + wave * 32 * (DV + M::E), av, 1.f, d.dv, [&](int r) { return key_at(bd.dv, r, d.dv); });
+    } else {
+        Frag vr[Ge::NV];
+#pragma unroll
+        for (int i = 0; i < Ge::NV; ++i) vr[i] = row_frag<M>(vp, M::KS * i + M::E * h, d.dv, on);
+        floatx16 a1[DK / 32], a2[DK / 32];
+#pragma unroll
+        for (int n = 0; n < DK / 32; ++n) a1[n] = a2[n] = zero16();
+        walk([&](int buf, int sub, int rs) {
+            floatx16 s1, s2;
+            maps(buf, sub, rs, s1, s2);
+            const T* qt = Buf + buf * Ge::TSZ;
+            floatx16 dp = row_values(Xs[buf][X_D1] + 32 * sub);
+#pragma unroll
+            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), vr[i], dp);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s1[r] *= dp[r];
+            const floatx16 d12 = row_values(Xs[buf][X_D12] + 32 * sub);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s2[r] *= dp[r] + d12[r];
+#pragma unroll
+            for (int i = 0; i < Ge::NP; ++i) {
+                const Frag f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
+#pragma unroll
+                for (int n = 0; n < DK / 32; ++n) {
+                    a1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, a1[n]);
+                    a2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, a2[n]);
+                }
+            }
+        });
+        T* mine = Buf + KW * 32 * (DV + M::E) + (wave - KW) * 32 * (DK + M::E);
+        write_rows<M>(mine, a1, d.scale, d.d, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
+        write_rows<M>(mine, a2, -d.scale, d.d, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
+    }
 }
 
 // ------------------------------------------------------------------ instances
+// key groups of a k_diff_bwd_kv workgroup: 4 (two waves on a SIMD) where a wave's operands and accumulators fit 256 registers
+constexpr int da_kw(int type, int dk) { return dk >= 128 || (type == MEP_F32 && dk >= 64) ? 2 : 4; }
+
 template <int TYPE, int DK, int DV>
 void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
-    // fp32 keys of 128 + 128 + 256 channels beside their gradients' accumulators would need more than the register file
-    constexpr bool KREG = !(TYPE == MEP_F32 && DK >= 128);
     if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
-    else hipLaunchKernelGGL((k_diff_bwd_kv<TYPE, DK, DV, KREG>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+    else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid), dim3(128 * da_kw(TYPE, DK)), 0, st, *b, blocks);
 }
 
 // the smallest instance that holds the head widths
+inline int da_width(int d, int dv) { return d <= 32 && dv <= 64 ? 32 : d <= 64 && dv <= 128 ? 64 : 128; }
 template <int TYPE>
 void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
     if (d.d <= 32 && d.dv <= 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, st);

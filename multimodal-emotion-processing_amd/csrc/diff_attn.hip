@@ -33,11 +33,11 @@ bool inputs_ok(const mep_diff_attn_desc& d) {
            rows_ok(d, d.v, d.v_sB, d.v_sT, d.v_sH, 0, false);
 }
 
-// the workgroups of a launch over `items` rows or keys per (batch, key head), or -1 (too many)
-int64_t plan(const mep_diff_attn_desc& d, int64_t items, int& blocks) {
-    blocks = (int)((items + DA_ROWS - 1) / DA_ROWS);
+// the workgroups of a launch over `items` rows or keys per (batch, key head), `per` each, or -1 (too many)
+int64_t plan(const mep_diff_attn_desc& d, int64_t items, int per, int& blocks) {
+    blocks = (int)((items + per - 1) / per);
     const int64_t grid = (int64_t)blocks * d.B * d.G;
-    return grid * DA_THREADS < ((int64_t)1 << 32) ? grid : -1;
+    return grid < 1 << 23 ? grid : -1;            // of up to 512 threads: 2^32 threads are a launch's most
 }
 
 void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, hipStream_t st) {
@@ -103,7 +103,7 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     if (d.B == 0 || d.Tq == 0) return 0;
     if (!inputs_ok(d)) { mep_set_error("mep_diff_attn_fwd: rows that cannot be read 16 bytes at a time"); return MEP_EINVAL; }
     int blocks;
-    const int64_t grid = plan(d, (int64_t)d.Tq * (d.H / d.G), blocks);
+    const int64_t grid = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, blocks);
     if (grid < 0) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
     run(DA_FWD, d, nullptr, grid, blocks, (hipStream_t)stream);
     return mep_check_launch("mep_diff_attn_fwd");
@@ -124,7 +124,8 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     }
     hipStream_t st = (hipStream_t)stream;
     int qb, kb;
-    const int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), qb), kg = plan(d, d.Tk, kb);
+    const int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb),
+                  kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
     if (rows) run(DA_BWD_Q, d, &b, qg, qb, st);
     if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, st);
