@@ -128,17 +128,14 @@ struct Stager {
     static_assert(STEP >= 4 && ROWS % STEP == 0, "tile");
     int row;
     unsigned off[NO];                // byte offset of the lane's chunk in row `row`, or DA_NOWHERE
-    static MEP_DEV int chunk(int i) {
-        const int pos = threadIdx.x;
-        return (pos % L::CH) ^ L::sw(pos / L::CH + i * STEP);
-    }
+    static MEP_DEV int chunk(int tid, int i) { return (tid % L::CH) ^ L::sw(tid / L::CH + i * STEP); }
     // where(c): element offset of chunk c within its row, or -1 where there is none
     template <class F>
-    MEP_DEV Stager(unsigned stride, F where) {
-        row = threadIdx.x / L::CH;
+    MEP_DEV Stager(int tid, unsigned stride, F where) {
+        row = tid / L::CH;
 #pragma unroll
         for (int i = 0; i < NO; ++i) {
-            const int o = where(chunk(i));
+            const int o = where(chunk(tid, i));
             off[i] = o < 0 ? DA_NOWHERE : (unsigned)(row * stride + o) * (unsigned)sizeof(T);
         }
     }
@@ -341,6 +338,14 @@ MEP_DEV void mask_keys(const mep_diff_attn_desc& d, const Job& j, int k0, unsign
     }
 }
 
+// threadIdx.x, as a value that the compiler cannot carry from one tile to the next: addresses made of it are made again (a few
+// operations a tile) instead of held in registers, or worse, in scratch memory, whose loads would wait for the DMA in flight
+MEP_DEV int thread_again() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // The keys and values of a (batch, key head), tile by tile
 template <int TYPE, int DK, int DV>
 struct KeyTiles {
@@ -350,20 +355,21 @@ struct KeyTiles {
     const mep_diff_attn_desc& d;
     const MEP_G T* kp;
     const MEP_G T* vp;
-    Stager<M, Ge::KT, 2 * DK> ks;
-    Stager<M, Ge::KT, DV> vs;
-    MEP_DEV KeyTiles(const mep_diff_attn_desc& desc, const Job& j)
-        : d(desc),
-          ks((unsigned)desc.k_sT, [&](int c) {
-              const int m = c >= DK / M::E, col = c * M::E - m * DK;
-              return col < desc.d ? col + (m ? (int)desc.k_sM : 0) : -1;
-          }),
-          vs((unsigned)desc.v_sT, [&](int c) { return c * M::E < desc.dv ? c * M::E : -1; }) {
+    MEP_DEV KeyTiles(const mep_diff_attn_desc& desc, const Job& j) : d(desc) {
         kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
         vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
     }
-    MEP_DEV void load(T* tile, int k0, unsigned long long bits) const {
+    MEP_DEV void load_keys(T* tile, int k0, unsigned long long bits, int tid) const {
+        const Stager<M, Ge::KT, 2 * DK> ks(tid, (unsigned)d.k_sT, [&](int c) {
+            const int m = c >= DK / M::E, col = c * M::E - m * DK;
+            return col < d.d ? col + (m ? (int)d.k_sM : 0) : -1;
+        });
         ks.load(tile, kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
+    }
+    MEP_DEV void load(T* tile, int k0, unsigned long long bits) const {
+        const int tid = thread_again();
+        load_keys(tile, k0, bits, tid);
+        const Stager<M, Ge::KT, DV> vs(tid, (unsigned)d.v_sT, [&](int c) { return c * M::E < d.dv ? c * M::E : -1; });
         vs.load(tile + Ge::KSZ, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
     }
 };
@@ -572,10 +578,11 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
 // ------------------------------------------------------------------ backward: D and dq
 // D_m = dO . (A_m v) is known beforehand only up to the roundings of the forward's out and second = A_2 v.  That error is some
 // 2^-9 of the sum of A_m^2 of the row in dP's units: nothing beside dS's own rounding where many keys carry the row, but all of dS
-// where one does.  So the row sums of A_m dP are formed beside dS without any rounding to 16 bits, and where a row of the
-// workgroup rests on fewer than 16 keys (sum A_m^2 > 1 / 16), a second pass over the keys forms A_m k_m and puts their difference
-// right: dq_m -= (D_m - estimate) A_m k_m.  (In fp32 the estimate is as good as the sum.)  The sums are also lam's gradient and
-// what dk needs.
+// where one does.  So the row sums of A_m dP are formed beside dS without any rounding to 16 bits, and their difference is put right:
+// dq_m -= (D_m - estimate) A_m k_m.  At DK = 32, E_m k_m is summed beside dS (BESIDE).  Wider heads have no registers for that
+// (accumulators that pass through the accumulation registers for every tile cost more than a second pass): there a second pass
+// over the keys forms it where a row of the workgroup rests on fewer than 32 keys (sum A_m^2 > 1 / 32; at that it is a thirtieth of
+// dS's rounding).  (In fp32 the estimate is as good as the sum.)  The sums are also lam's gradient and what dk needs.
 template <int TYPE, int DK, int DV>
 __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
     typedef Geo<TYPE, DK, DV> Ge;
@@ -639,9 +646,10 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
     const int64_t srow = ((int64_t)j.b * d.H + w.head) * d.Tq + w.t;
     const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * srow);      // m1, 1 / l1, m2, 1 / l2
 
-    constexpr bool CORR = TYPE != MEP_F32;
+    constexpr bool BESIDE = TYPE != MEP_F32 && DK == 32, CORR = TYPE != MEP_F32 && DK != 32;
     float sum1 = 0.f, sum2 = 0.f, sq1 = 0.f, sq2 = 0.f;
-    floatx16 a1[DK / 32], a2[DK / 32];
+    floatx16 a1[DK / 32], a2[DK / 32], b1, b2;
+    b1 = b2 = zero16();
 #pragma unroll
     for (int n = 0; n < DK / 32; ++n) a1[n] = a2[n] = zero16();
     for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
@@ -677,16 +685,39 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
                     sq1 = fmaf(e1, e1, sq1);
                     sq2 = fmaf(e2, e2, sq2);
                 }
-                s1[r] = e1 * (dp[r] - d1);
-                s2[r] = e2 * (dp[r] - d2);
+                if constexpr (BESIDE) {
+                    s1[r] = e1;
+                    s2[r] = e2;
+                } else {
+                    s1[r] = e1 * (dp[r] - d1);
+                    s2[r] = e2 * (dp[r] - d2);
+                }
+            }
+            Frag e1[BESIDE ? Ge::NP : 1], e2[BESIDE ? Ge::NP : 1];
+            if constexpr (BESIDE) {
+#pragma unroll
+                for (int i = 0; i < Ge::NP; ++i) {
+                    e1[i] = acc_frag<M>(s1, i);
+                    e2[i] = acc_frag<M>(s2, i);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s1[r] *= dp[r] - d1;
+                    s2[r] *= dp[r] - d2;
+                }
             }
 #pragma unroll
             for (int i = 0; i < Ge::NP; ++i) {
                 const Frag p1 = acc_frag<M>(s1, i), p2 = acc_frag<M>(s2, i);
 #pragma unroll
                 for (int n = 0; n < DK / 32; ++n) {
-                    a1[n] = M::mma(kread.cols(kt, 32 * sub, 32 * n, i), p1, a1[n]);
-                    a2[n] = M::mma(kread.cols(kt, 32 * sub, DK + 32 * n, i), p2, a2[n]);
+                    const Frag k1 = kread.cols(kt, 32 * sub, 32 * n, i), k2 = kread.cols(kt, 32 * sub, DK + 32 * n, i);
+                    a1[n] = M::mma(k1, p1, a1[n]);
+                    a2[n] = M::mma(k2, p2, a2[n]);
+                    if constexpr (BESIDE) {
+                        b1 = M::mma(k1, e1[i], b1);
+                        b2 = M::mma(k2, e2[i], b2);
+                    }
                 }
             }
         }
@@ -699,7 +730,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
     }
     if (!bd.dq) return;
     if constexpr (CORR) {
-        const bool few = w.live && fmaxf(half_sum(sq1) * st[1] * st[1], half_sum(sq2) * st[3] * st[3]) > 0.0625f;
+        const bool few = w.live && fmaxf(half_sum(sq1) * st[1] * st[1], half_sum(sq2) * st[3] * st[3]) > 0.03125f;
         if (__syncthreads_or(few)) {
             floatx16 k1[DK / 32], k2[DK / 32];
 #pragma unroll
@@ -707,7 +738,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
             for (int k0 = 0; k0 < end; k0 += KT) {      // one buffer: this pass is the rare one
                 bits = key_bits(d, j, k0, KT, key_raw(d, j, k0));
                 tile_sync();
-                keys.ks.load(Buf, keys.kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
+                keys.load_keys(Buf, k0, bits, thread_again());
                 tile_sync();
 #pragma unroll 1
                 for (int sub = 0; sub < KT / 32; ++sub) {
@@ -746,6 +777,13 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
                 }
         }
     }
+    if constexpr (BESIDE) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            a1[0][r] = fmaf(b1[r], d1 - sum1, a1[0][r]);
+            a2[0][r] = fmaf(b2[r], d2 - sum2, a2[0][r]);
+        }
+    }
     tile_sync();                             // the tiles are free
     const int64_t first = (int64_t)j.b * d.Tq * d.H * 2 * d.d;
     auto row_at = [&](int m, int r) -> MEP_G T* {
@@ -760,9 +798,10 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
 }
 
 // ------------------------------------------------------------------ backward: dk and dv
-// A workgroup walks the rows of 32 KW keys.  Of its 2 KW waves one half forms dv (an accumulator column per key), the other dk: each
-// needs the scores, but so neither holds more than 256 registers and two waves share a SIMD (in one wave, the accumulators of
-// both pass through the accumulation registers and back for every tile: 335 us against 241 at B 2, T 4096, 8 heads, 64 / 128, causal).
+// A workgroup walks the rows of 32 KW keys, a wave (an accumulator column per key) those of 32.  At DK = 32 a wave forms dv and dk
+// (ROLES = 1).  With wider heads the workgroup has 2 KW waves, one half for dv and the other for dk (ROLES = 2): both form
+// the scores, but so neither holds more than 256 registers and two waves share a SIMD (in one wave, the accumulators of
+// both pass through the accumulation registers and back for every tile: 335 us against 268 at B 2, T 4096, 8 heads, 64 / 128, causal).
 //
 // The scores lie rows x keys here, so a row's statistics are not a lane's.  They come in as a product: the accumulator starts
 // at X 1 with X the row's value in three bf16 parts (24 bits) against a column of ones, one instruction for 16 registers.  With
@@ -772,7 +811,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
 template <int KW, int TYPE, int DK, int DV>
 struct KvShape {
     typedef Geo<TYPE, DK, DV> Ge;
-    static constexpr int THREADS = 128 * KW, KEYS = 32 * KW;
+    static constexpr int ROLES = DK == 32 ? 1 : 2, THREADS = 64 * KW * ROLES, KEYS = 32 * KW;
     static constexpr int OUT = KEYS * (DK + DV + 2 * Ge::M::E), BUF = 2 * Ge::TSZ > OUT ? 2 * Ge::TSZ : OUT;
 };
 
@@ -802,13 +841,13 @@ MEP_DEV floatx16 row_values(const bf16x8_da* x) {
 }
 
 template <int KW, int TYPE, int DK, int DV>
-__global__ __launch_bounds__(128 * KW, KW / 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks) {
+__global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef KvShape<KW, TYPE, DK, DV> Sh;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
     typedef typename Ge::Frag Frag;
-    constexpr int RT = Ge::KT, THREADS = Sh::THREADS;
+    constexpr int RT = Ge::KT, THREADS = Sh::THREADS, ROLES = Sh::ROLES;
     const mep_diff_attn_desc& d = bd.f;
     __shared__ __align__(16) T Buf[Sh::BUF];      // two tiles: their queries, then their upstream gradients
     __shared__ bf16x8_da Xs[2][X_COUNT][RT];      // and their rows' values
@@ -816,7 +855,7 @@ __global__ __launch_bounds__(128 * KW, KW / 2) void k_diff_bwd_kv(mep_diff_attn_
     __shared__ int Neg[2];                        // whether any lam of the tile is negative
     const Job j = make_job(d, blocks, false);
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-    const bool for_v = wave < KW;
+    const bool for_v = ROLES == 1 || wave < KW;
     const int key0 = j.block * Sh::KEYS + wave % KW * 32, key = key0 + (lane & 31);
     const float c = d.scale * DA_LOG2E;
     // rows that see any of the block's / the wave's keys; every one of the wave's keys: from row wfull on; the lane's key: from rmin on
@@ -830,12 +869,13 @@ __global__ __launch_bounds__(128 * KW, KW / 2) void k_diff_bwd_kv(mep_diff_attn_
     const MEP_G T* ob = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
     const Reader<M, 2 * DK> qread;
     const Reader<M, DV> oread;
-    const Stager<M, RT, 2 * DK, THREADS> qs((unsigned)d.q_sT, [&](int ch) {
-        const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
-        return col < d.d ? col + (m ? (int)d.q_sM : 0) : -1;
-    });
-    const Stager<M, RT, DV, THREADS> os((unsigned)bd.o_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
     auto load_rows = [&](int buf, int r0) {
+        const int tid = thread_again();
+        const Stager<M, RT, 2 * DK, THREADS> qs(tid, (unsigned)d.q_sT, [&](int ch) {
+            const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
+            return col < d.d ? col + (m ? (int)d.q_sM : 0) : -1;
+        });
+        const Stager<M, RT, DV, THREADS> os(tid, (unsigned)bd.o_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
         T* tile = Buf + buf * Ge::TSZ;
         if (j.n == 1) {
             const int left = j.rows - r0;
@@ -966,56 +1006,90 @@ __global__ __launch_bounds__(128 * KW, KW / 2) void k_diff_bwd_kv(mep_diff_attn_
     auto key_at = [&](uint64_t p, int r, int64_t width) -> MEP_G T* {
         return key0 + r < d.Tk ? G<T>(p) + (first + (int64_t)(key0 + r) * d.G) * width : nullptr;
     };
-    if (for_v) {
-        floatx16 av[DV / 32];
+    floatx16 av[DV / 32], a1[DK / 32], a2[DK / 32];
+    auto clear_v = [&] {
 #pragma unroll
         for (int n = 0; n < DV / 32; ++n) av[n] = zero16();
+    };
+    auto clear_k = [&] {
+#pragma unroll
+        for (int n = 0; n < DK / 32; ++n) a1[n] = a2[n] = zero16();
+    };
+    // dv += P^T dO
+    auto add_v = [&](const T* ot, int sub, const floatx16& p) {
+#pragma unroll
+        for (int i = 0; i < Ge::NP; ++i) {
+            const Frag f = acc_frag<M>(p, i);
+#pragma unroll
+            for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), f, av[n]);
+        }
+    };
+    // dk_m += dS_m^T q_m; s1, s2: the maps
+    Frag vr[Ge::NV];
+    auto load_v = [&] {
+#pragma unroll
+        for (int i = 0; i < Ge::NV; ++i) vr[i] = row_frag<M>(vp, M::KS * i + M::E * h, d.dv, on);
+    };
+    auto add_k = [&](const T* qt, int buf, int sub, floatx16& s1, floatx16& s2) {
+        floatx16 dp = row_values(Xs[buf][X_D1] + 32 * sub);
+#pragma unroll
+        for (int i = 0; i < Ge::NV; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), vr[i], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s1[r] *= dp[r];
+        const floatx16 d12 = row_values(Xs[buf][X_D12] + 32 * sub);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s2[r] *= dp[r] + d12[r];
+#pragma unroll
+        for (int i = 0; i < Ge::NP; ++i) {
+            const Frag f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
+#pragma unroll
+            for (int n = 0; n < DK / 32; ++n) {
+                a1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, a1[n]);
+                a2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, a2[n]);
+            }
+        }
+    };
+    auto put_v = [&](T* mine) { write_rows<M>(mine, av, 1.f, d.dv, [&](int r) { return key_at(bd.dv, r, d.dv); }); };
+    auto put_k = [&](T* mine) {
+        write_rows<M>(mine, a1, d.scale, d.d, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
+        write_rows<M>(mine, a2, -d.scale, d.d, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
+    };
+    T* vbuf = Buf + wave % KW * 32 * (DV + M::E);
+    T* kbuf = Buf + KW * 32 * (DV + M::E) + wave % KW * 32 * (DK + M::E);
+    if constexpr (ROLES == 1) {
+        clear_v();
+        clear_k();
+        load_v();
+        walk([&](int buf, int sub, int rs) {
+            const T* qt = Buf + buf * Ge::TSZ;
+            floatx16 s1, s2, p;
+            maps(buf, sub, rs, s1, s2);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = s1[r] - s2[r];
+            add_v(qt + Ge::KSZ, sub, p);
+            add_k(qt, buf, sub, s1, s2);
+        });
+        put_v(vbuf);
+        put_k(kbuf);
+    } else if (for_v) {
+        clear_v();
         walk([&](int buf, int sub, int rs) {
             floatx16 s1, s2;
             maps(buf, sub, rs, s1, s2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s1[r] -= s2[r];
-            const T* ot = Buf + buf * Ge::TSZ + Ge::KSZ;
-#pragma unroll
-            for (int i = 0; i < Ge::NP; ++i) {
-                const Frag p = acc_frag<M>(s1, i);
-#pragma unroll
-                for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), p, av[n]);
-            }
+            add_v(Buf + buf * Ge::TSZ + Ge::KSZ, sub, s1);
         });
-        write_rows<M>(Buf + wave * 32 * (DV + M::E), av, 1.f, d.dv, [&](int r) { return key_at(bd.dv, r, d.dv); });
+        put_v(vbuf);
     } else {
-        Frag vr[Ge::NV];
-#pragma unroll
-        for (int i = 0; i < Ge::NV; ++i) vr[i] = row_frag<M>(vp, M::KS * i + M::E * h, d.dv, on);
-        floatx16 a1[DK / 32], a2[DK / 32];
-#pragma unroll
-        for (int n = 0; n < DK / 32; ++n) a1[n] = a2[n] = zero16();
+        clear_k();
+        load_v();
         walk([&](int buf, int sub, int rs) {
             floatx16 s1, s2;
             maps(buf, sub, rs, s1, s2);
-            const T* qt = Buf + buf * Ge::TSZ;
-            floatx16 dp = row_values(Xs[buf][X_D1] + 32 * sub);
-#pragma unroll
-            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), vr[i], dp);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s1[r] *= dp[r];
-            const floatx16 d12 = row_values(Xs[buf][X_D12] + 32 * sub);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s2[r] *= dp[r] + d12[r];
-#pragma unroll
-            for (int i = 0; i < Ge::NP; ++i) {
-                const Frag f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
-#pragma unroll
-                for (int n = 0; n < DK / 32; ++n) {
-                    a1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, a1[n]);
-                    a2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, a2[n]);
-                }
-            }
+            add_k(Buf + buf * Ge::TSZ, buf, sub, s1, s2);
         });
-        T* mine = Buf + KW * 32 * (DV + M::E) + (wave - KW) * 32 * (DK + M::E);
-        write_rows<M>(mine, a1, d.scale, d.d, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
-        write_rows<M>(mine, a2, -d.scale, d.d, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
+        put_k(kbuf);
     }
 }
 
@@ -1027,7 +1101,8 @@ template <int TYPE, int DK, int DV>
 void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
     if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
-    else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid), dim3(128 * da_kw(TYPE, DK)), 0, st, *b, blocks);
+    else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
+                            dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks);
 }
 
 // the smallest instance that holds the head widths
