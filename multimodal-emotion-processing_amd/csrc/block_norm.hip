@@ -8,9 +8,12 @@
 // The stream is formed again from y and x in 32 bits (the stored one is rounded to 16), so parameter gradients kept
 // in 32 bits are sums of exact terms; the four row statistics come from the forward.
 //
-// Bound by memory: every row is read and written once, held in registers in between (E elements in each of L lanes;
-// L = 16 lanes of a wave up to two workgroup halves, by the row's width).  A workgroup walks many rows with the
-// parameters, and in the backward the column sums, in registers; the sums are joined in a fixed order by a second kernel.
+// Bound by memory: every row is read and written once, held in registers in between: 8 elements in each of L lanes, L = 16
+// of a wave to 1024 of a workgroup by the row's width, in 16-byte accesses at any address (TAIL: widths that end inside one).
+// A workgroup walks many rows with the parameters, and in the backward the column sums, in registers; the sums of its row
+// slots are joined in LDS, those of the workgroups by a second kernel, in a fixed order.  8 elements a lane leave the
+// backward's registers (parameters, up to 5 sums and 4 rows) room for 4 waves on a SIMD: at 16384 rows of 4096 in bf16, both
+// norms and a gate, 455 us with 16 elements.
 #include "elem.h"
 
 namespace {
@@ -20,8 +23,10 @@ using namespace mep;
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_SEQUENCE = 2, GATE_FULL = 3 };
 enum { KIND_NONE = 0, KIND_RMS = 1, KIND_LAYER = 2 };
 
+template <int L> constexpr int norm_threads() { return L < 256 ? 256 : L; }
+
 // sums of a and b over the L lanes of a row, in a fixed order, in every lane.  L = 16: a DPP row; 64: a wave;
-// more: the workgroup, through one of red's two halves (`par`, alternated from call to call: a half is written again
+// more: L / 64 waves of the workgroup, through one of red's two halves (`par`, alternated from call to call: a half is written again
 // only behind the barrier of the call between, which every wave reaches after it has read the half)
 template <int L>
 MEP_DEV void row_sum2(float& a, float& b, float* red, int par) {
@@ -34,10 +39,12 @@ MEP_DEV void row_sum2(float& a, float& b, float* red, int par) {
         a = wave_sum(a);
         b = wave_sum(b);
         if constexpr (L > 64) {
-            constexpr int W = L / 64;
-            float* r = red + par * 2 * W;
-            if ((threadIdx.x & 63) == 0) { r[2 * (threadIdx.x >> 6)] = a; r[2 * (threadIdx.x >> 6) + 1] = b; }
+            constexpr int W = L / 64, ALL = norm_threads<L>() / 64;
+            float* r = red + par * 2 * ALL;
+            const int wave = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) { r[2 * wave] = a; r[2 * wave + 1] = b; }
             __syncthreads();
+            r += wave / W * 2 * W;
             a = r[0]; b = r[1];
 #pragma unroll
             for (int i = 1; i < W; ++i) { a += r[2 * i]; b += r[2 * i + 1]; }
@@ -45,8 +52,9 @@ MEP_DEV void row_sum2(float& a, float& b, float* red, int par) {
     }
 }
 
-// lane's elements of a row: chunk c covers columns (c L + lane) V ..
-template <class T, int V, int L, int E>
+constexpr int E = 8;      // elements of a lane: chunk c of V covers columns (c L + lane) V ..; zeros past D
+
+template <class T, int V, int L, bool TAIL>
 MEP_DEV void load_row(const MEP_G T* p, int lane, int D, float (&v)[E]) {
 #pragma unroll
     for (int c = 0; c < E / V; ++c) {
@@ -54,12 +62,17 @@ MEP_DEV void load_row(const MEP_G T* p, int lane, int D, float (&v)[E]) {
         float w[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) w[j] = 0.f;
-        if (col < D) load_f32<T, V>(p + col, w);
+        if (col + V <= D) {
+            load_f32<T, V>(p + col, w);
+        } else if (TAIL) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) if (col + j < D) w[j] = (float)p[col + j];
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) v[c * V + j] = w[j];
     }
 }
-template <class T, int V, int L, int E>
+template <class T, int V, int L, bool TAIL>
 MEP_DEV void store_row(MEP_G T* p, int lane, int D, const float (&v)[E]) {
 #pragma unroll
     for (int c = 0; c < E / V; ++c) {
@@ -67,41 +80,45 @@ MEP_DEV void store_row(MEP_G T* p, int lane, int D, const float (&v)[E]) {
         float w[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) w[j] = v[c * V + j];
-        if (col < D) store_f32<T, V>(p + col, w);
+        if (col + V <= D) {
+            store_f32<T, V>(p + col, w);
+        } else if (TAIL) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) if (col + j < D) p[col + j] = (T)w[j];
+        }
     }
 }
 // a parameter row, fp32 or the activations' type; `miss` where there is none
-template <class T, int V, int L, int E>
+template <class T, int V, int L, bool TAIL>
 MEP_DEV void load_param(uint64_t p, int64_t off, bool wide, float miss, int lane, int D, float (&v)[E]) {
     if (!p) {
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = miss;
     } else if (wide) {
-        load_row<float, V, L, E>(G<const float>(p) + off, lane, D, v);
+        load_row<float, V, L, TAIL>(G<const float>(p) + off, lane, D, v);
     } else {
-        load_row<T, V, L, E>(G<const T>(p) + off, lane, D, v);
+        load_row<T, V, L, TAIL>(G<const T>(p) + off, lane, D, v);
     }
 }
 
-template <int L> constexpr int norm_threads() { return L < 256 ? 256 : L; }
 
 MEP_DEV float residual_scale(const mep_block_norm_desc& d) { return d.scale ? *G<const float>(d.scale) : d.scale_value; }
 
-template <int TYPE, int V, int L, int E>
+template <int TYPE, int V, int L, bool TAIL>
 __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_fwd(mep_block_norm_desc d) {
     typedef typename ElemOf<TYPE>::T T;
     constexpr int RPB = norm_threads<L>() / L;
-    __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
+    __shared__ float red[L > 64 ? norm_threads<L>() / 16 : 1];
     const int lane = threadIdx.x % L, slot = threadIdx.x / L;
     const int D = d.D;
     const bool wide = d.wtype == MEP_F32, gwide = d.gtype == MEP_F32;
     const float inv = 1.0f / (float)D;
     float w[E], bi[E], nw[E], nb[E], gc[E];
-    load_param<T, V, L, E>(d.w, 0, wide, 1.f, lane, D, w);
-    load_param<T, V, L, E>(d.b, 0, wide, 0.f, lane, D, bi);
-    load_param<T, V, L, E>(d.nw, 0, wide, 1.f, lane, D, nw);
-    load_param<T, V, L, E>(d.nb, 0, wide, 0.f, lane, D, nb);
-    if (d.gate_form <= GATE_CHANNEL) load_param<T, V, L, E>(d.gate, 0, gwide, 1.f, lane, D, gc);
+    load_param<T, V, L, TAIL>(d.w, 0, wide, 1.f, lane, D, w);
+    load_param<T, V, L, TAIL>(d.b, 0, wide, 0.f, lane, D, bi);
+    load_param<T, V, L, TAIL>(d.nw, 0, wide, 1.f, lane, D, nw);
+    load_param<T, V, L, TAIL>(d.nb, 0, wide, 0.f, lane, D, nb);
+    if (d.gate_form <= GATE_CHANNEL) load_param<T, V, L, TAIL>(d.gate, 0, gwide, 1.f, lane, D, gc);
     const float sc = residual_scale(d);
     bool in[E];
 #pragma unroll
@@ -112,10 +129,10 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_fwd(mep_block_
         const bool live = row < d.rows;              // a slot past the end reduces zeros and stores nothing
         const int64_t rr = live ? row : d.rows - 1;
         float y[E], x[E];
-        load_row<T, V, L, E>(G<const T>(d.y) + rr * d.y_ld, lane, D, y);
-        if (d.x) load_row<T, V, L, E>(G<const T>(d.x) + rr * d.x_ld, lane, D, x);
-        if (d.gate_form == GATE_SEQUENCE) load_param<T, V, L, E>(d.gate, rr / d.T * D, gwide, 1.f, lane, D, gc);
-        if (d.gate_form == GATE_FULL) load_row<T, V, L, E>(G<const T>(d.gate) + rr * d.g_ld, lane, D, gc);
+        load_row<T, V, L, TAIL>(G<const T>(d.y) + rr * d.y_ld, lane, D, y);
+        if (d.x) load_row<T, V, L, TAIL>(G<const T>(d.x) + rr * d.x_ld, lane, D, x);
+        if (d.gate_form == GATE_SEQUENCE) load_param<T, V, L, TAIL>(d.gate, rr / d.T * D, gwide, 1.f, lane, D, gc);
+        if (d.gate_form == GATE_FULL) load_row<T, V, L, TAIL>(G<const T>(d.gate) + rr * d.g_ld, lane, D, gc);
         float mean = 0.f, r = 1.f, smean = 0.f, sr = 1.f;
         auto stats = [&](const float (&v)[E], int kind, float& mu, float& rs) {
             if (kind == KIND_NONE) return;
@@ -144,37 +161,38 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_fwd(mep_block_
             if (d.x) n = fmaf(sc, x[i], n);
             y[i] = in[i] ? n : 0.f;
         }
-        if (live) store_row<T, V, L, E>(G<T>(d.stream) + row * D, lane, D, y);
+        if (live) store_row<T, V, L, TAIL>(G<T>(d.stream) + row * D, lane, D, y);
         if (d.normed) {
             stats(y, d.next_kind, smean, sr);
 #pragma unroll
             for (int i = 0; i < E; ++i) y[i] = fmaf((y[i] - smean) * sr, nw[i], nb[i]);
-            if (live) store_row<T, V, L, E>(G<T>(d.normed) + row * D, lane, D, y);
+            if (live) store_row<T, V, L, TAIL>(G<T>(d.normed) + row * D, lane, D, y);
         }
         if (d.stats && live && lane == 0)
             *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * row) = f32x4{mean, r, smean, sr};
     }
 }
 
-// Column sums of a workgroup: partial[(seq * gridDim.x + blockIdx.x) * RPB + slot][5][D] = dw, db, dnw, dnb, dgate and
+// Column sums of a workgroup: partial[seq * gridDim.x + blockIdx.x][n_sums][D] = those wanted of dw, db, dnw, dnb, dgate, and
 // the scalar dscale behind all of them.  gridDim.y sequences of d.T rows under a sequence gate, else one of all rows.
-template <int TYPE, int V, int L, int E>
-__global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_bwd(mep_block_norm_bwd_desc bd) {
+template <int TYPE, int V, int L, bool TAIL, bool BIAS>
+__global__ __launch_bounds__(norm_threads<L>(), L >= 512 ? 4 : 2) void k_block_norm_bwd(mep_block_norm_bwd_desc bd) {
     typedef typename ElemOf<TYPE>::T T;
     constexpr int RPB = norm_threads<L>() / L;
     const mep_block_norm_desc& d = bd.f;
-    __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
+    __shared__ float red[L > 64 ? norm_threads<L>() / 16 : 1];
+    __shared__ float slots[RPB > 1 ? RPB * L * E : 1];      // a column sum of each row slot
     const int lane = threadIdx.x % L, slot = threadIdx.x / L;
     const int D = d.D;
     const bool wide = d.wtype == MEP_F32, gwide = d.gtype == MEP_F32, layer = d.kind == KIND_LAYER, nlayer = d.next_kind == KIND_LAYER;
     const float inv = 1.0f / (float)D;
     const bool next = bd.dnormed != 0;
     float w[E], bi[E], nw[E], gc[E];
-    load_param<T, V, L, E>(d.w, 0, wide, 1.f, lane, D, w);
-    load_param<T, V, L, E>(d.b, 0, wide, 0.f, lane, D, bi);
-    load_param<T, V, L, E>(d.nw, 0, wide, 1.f, lane, D, nw);
-    if (d.gate_form <= GATE_CHANNEL) load_param<T, V, L, E>(d.gate, 0, gwide, 1.f, lane, D, gc);
-    else if (d.gate_form == GATE_SEQUENCE) load_param<T, V, L, E>(d.gate, (int64_t)blockIdx.y * D, gwide, 1.f, lane, D, gc);
+    load_param<T, V, L, TAIL>(d.w, 0, wide, 1.f, lane, D, w);
+    load_param<T, V, L, TAIL>(BIAS ? d.b : 0, 0, wide, 0.f, lane, D, bi);
+    load_param<T, V, L, TAIL>(d.nw, 0, wide, 1.f, lane, D, nw);
+    if (d.gate_form <= GATE_CHANNEL) load_param<T, V, L, TAIL>(d.gate, 0, gwide, 1.f, lane, D, gc);
+    else if (d.gate_form == GATE_SEQUENCE) load_param<T, V, L, TAIL>(d.gate, (int64_t)blockIdx.y * D, gwide, 1.f, lane, D, gc);
     const float sc = residual_scale(d);
     float aw[E], ab[E], anw[E], anb[E], ag[E], as = 0.f;
 #pragma unroll
@@ -187,11 +205,11 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_bwd(mep_block_
         const bool live = row < end;                 // a slot past the end works on zeros and stores nothing
         const int64_t rr = live ? row : end - 1;
         float y[E], x[E], g[E], h[E];
-        load_row<T, V, L, E>(G<const T>(d.y) + rr * d.y_ld, lane, D, y);
-        if (d.x) load_row<T, V, L, E>(G<const T>(d.x) + rr * d.x_ld, lane, D, x);
-        if (d.gate_form == GATE_FULL) load_row<T, V, L, E>(G<const T>(d.gate) + rr * d.g_ld, lane, D, gc);
-        if (bd.dstream) load_row<T, V, L, E>(G<const T>(bd.dstream) + rr * bd.ds_ld, lane, D, g);
-        if (next) load_row<T, V, L, E>(G<const T>(bd.dnormed) + rr * bd.dn_ld, lane, D, h);
+        load_row<T, V, L, TAIL>(G<const T>(d.y) + rr * d.y_ld, lane, D, y);
+        if (d.x) load_row<T, V, L, TAIL>(G<const T>(d.x) + rr * d.x_ld, lane, D, x);
+        if (d.gate_form == GATE_FULL) load_row<T, V, L, TAIL>(G<const T>(d.gate) + rr * d.g_ld, lane, D, gc);
+        if (bd.dstream) load_row<T, V, L, TAIL>(G<const T>(bd.dstream) + rr * bd.ds_ld, lane, D, g);
+        if (next) load_row<T, V, L, TAIL>(G<const T>(bd.dnormed) + rr * bd.dn_ld, lane, D, h);
         const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * rr);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -207,7 +225,7 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_bwd(mep_block_
                 const float s = ((d.x ? fmaf(sc, x[i], n) : n) - st[2]) * st[3];   // the normalised stream
                 const float hi = live ? h[i] : 0.f;  // columns past D loaded zeros
                 anw[i] = fmaf(hi, s, anw[i]);
-                anb[i] += hi;
+                if constexpr (BIAS) anb[i] += hi;
                 const float u = hi * nw[i];
                 su += u;
                 sq = fmaf(u, s, sq);
@@ -232,27 +250,42 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_bwd(mep_block_
             ag[i] += dg[i];
             const float dn = g[i] * gc[i];
             aw[i] = fmaf(dn, y[i], aw[i]);
-            ab[i] += dn;
+            if constexpr (BIAS) ab[i] += dn;
             const float u = dn * w[i];
             x[i] = sc * g[i];
             g[i] = u;
             su += u;
             sq = fmaf(u, y[i], sq);
         }
-        if (bd.dx && live) store_row<T, V, L, E>(G<T>(bd.dx) + row * D, lane, D, x);
-        if (bd.dgate_rows && live) store_row<T, V, L, E>(G<T>(bd.dgate_rows) + row * D, lane, D, dg);
+        if (bd.dx && live) store_row<T, V, L, TAIL>(G<T>(bd.dx) + row * D, lane, D, x);
+        if (bd.dgate_rows && live) store_row<T, V, L, TAIL>(G<T>(bd.dgate_rows) + row * D, lane, D, dg);
         if (d.kind != KIND_NONE) { row_sum2<L>(su, sq, red, par); par ^= 1; }
         const float mu = layer ? su * inv : 0.f, mq = d.kind != KIND_NONE ? sq * inv : 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) g[i] = st[1] * (g[i] - mu - y[i] * mq);
-        if (live) store_row<T, V, L, E>(G<T>(bd.dy) + row * D, lane, D, g);
+        if (live) store_row<T, V, L, TAIL>(G<T>(bd.dy) + row * D, lane, D, g);
     }
     if (!bd.partial) return;
-    const int64_t p = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + slot;
+    const int64_t p = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     gfloat* out = G<float>(bd.partial) + p * bd.n_sums * D;
     int k = 0;
     auto put = [&](bool on, const float (&v)[E]) {
-        if (on) store_row<float, V, L, E>(out + (int64_t)k++ * D, lane, D, v);
+        if (!on) return;
+        gfloat* o = out + (int64_t)k++ * D;
+        if constexpr (RPB == 1) {
+            store_row<float, V, L, TAIL>(o, lane, D, v);
+        } else {      // the row slots' sums, in order
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; ++i) slots[slot * L * E + ((i / V) * L + lane) * V + i % V] = v[i];
+            __syncthreads();
+            for (int col = threadIdx.x; col < D; col += norm_threads<L>()) {
+                float s = slots[col];
+#pragma unroll
+                for (int r = 1; r < RPB; ++r) s += slots[r * L * E + col];
+                o[col] = s;
+            }
+        }
     };
     put(bd.dw != 0, aw);
     put(bd.db != 0, ab);
@@ -262,13 +295,21 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_bwd(mep_block_
     if (bd.dscale) {
         float z = 0.f;
         row_sum2<L>(as, z, red, par);
-        if (lane == 0) G<float>(bd.partial)[(int64_t)gridDim.x * gridDim.y * RPB * bd.n_sums * D + p] = as;
+        if constexpr (RPB > 1) {
+            __syncthreads();
+            if (lane == 0) slots[slot] = as;
+            __syncthreads();
+            as = slots[0];
+#pragma unroll
+            for (int r = 1; r < RPB; ++r) as += slots[r];
+        }
+        if (threadIdx.x == 0) G<float>(bd.partial)[(int64_t)gridDim.x * gridDim.y * bd.n_sums * D + p] = as;
     }
 }
 
-// out[k][col] = sum over the partial rows, in order: 4 slices of rows per 64 columns, then the slices.
+// out[k][col] = sum over the partial rows, in order: 16 slices of rows per 16 columns, then the slices.
 // blockIdx.y = sum * nseq + sequence for a sequence gate's sums (each sequence its own rows), else the sum.
-constexpr int NORM_SUM_COLS = 64, NORM_SUM_SLICES = 4;
+constexpr int NORM_SUM_COLS = 16, NORM_SUM_SLICES = 16;
 
 __global__ __launch_bounds__(NORM_SUM_COLS * NORM_SUM_SLICES) void k_block_norm_sums(mep_block_norm_bwd_desc bd, int rows_seq, int nseq) {
     const mep_block_norm_desc& d = bd.f;
@@ -286,7 +327,6 @@ __global__ __launch_bounds__(NORM_SUM_COLS * NORM_SUM_SLICES) void k_block_norm_
     if (scalar) {
         if (blockIdx.x) return;
         src = G<const float>(bd.partial) + (int64_t)all * bd.n_sums * D;
-        // the partial scalars as rows of 64 columns
         float s = 0.f;
         for (int i = threadIdx.x; i < all; i += NORM_SUM_COLS * NORM_SUM_SLICES) s += src[i];
         s = wave_sum(s);
@@ -322,7 +362,9 @@ __global__ __launch_bounds__(NORM_SUM_COLS * NORM_SUM_SLICES) void k_block_norm_
     part[sl][c] = s;
     __syncthreads();
     if (sl == 0 && col < cols) {
-        s = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+        s = part[0][c];
+#pragma unroll
+        for (int i = 1; i < NORM_SUM_SLICES; ++i) s += part[i][c];
         const int64_t o = (int64_t)seq * D + col;
         const int type = kind == 4 ? d.gtype : d.wtype;
         if (type == MEP_F32) G<float>(out)[o] = s;
@@ -331,29 +373,13 @@ __global__ __launch_bounds__(NORM_SUM_COLS * NORM_SUM_SLICES) void k_block_norm_
     }
 }
 
-int lanes_of(int D, int& E) {
-    if (D <= 128) { E = 8; return 16; }
-    if (D <= 512) { E = 8; return 64; }
-    if (D <= 1024) { E = 16; return 64; }
-    if (D <= 2048) { E = 8; return 256; }
-    if (D <= 4096) { E = 16; return 256; }
-    E = 16;
-    return 512;
+int lanes_of(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+int rows_per_block(int D) {
+    const int L = lanes_of(D);
+    return (L < 256 ? 256 : L) / L;
 }
 
-// 16-byte row accesses: the width, every row and every parameter on their boundary
-bool aligned(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b) {
-    const int es = d.type == MEP_F32 ? 4 : 2, V = 16 / es;
-    if (d.D % V) return false;
-    const uint64_t rows[] = {d.y, d.x, d.gate_form == GATE_FULL ? d.gate : 0, d.stream, d.normed, b ? b->dstream : 0,
-                             b ? b->dnormed : 0, b ? b->dy : 0, b ? b->dx : 0, b ? b->dgate_rows : 0};
-    for (uint64_t p : rows) if (p % 16) return false;
-    const uint64_t par[] = {d.w, d.b, d.nw, d.nb, d.gate};
-    for (uint64_t p : par) if (p % 16) return false;
-    return !(d.y_ld % V || d.x_ld % V || d.g_ld % V || (b && (b->ds_ld % V || b->dn_ld % V)));
-}
-
-// workgroups per sequence of the backward: one per two compute units over all sequences, at least 4 rows a slot
+// workgroups per sequence of the backward: two per compute unit over all sequences, at least 4 rows a slot
 // where there are so many (each workgroup's column sums cost 5 D floats), never more than its rows ask for
 int bwd_groups(const mep_block_norm_desc& d, int rpb) {
     const int64_t nseq = d.gate_form == GATE_SEQUENCE ? d.rows / d.T : 1;
@@ -363,40 +389,42 @@ int bwd_groups(const mep_block_norm_desc& d, int rpb) {
     return (int)(n < 1 ? 1 : n);
 }
 
-template <int TYPE, int V, int L, int E>
+template <int TYPE, int V, int L, bool TAIL>
 void run_norm(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hipStream_t st) {
     constexpr int TH = norm_threads<L>(), RPB = TH / L;
     if (!b) {
         const int64_t want = (d.rows + RPB - 1) / RPB, most = 2048;
-        hipLaunchKernelGGL((k_block_norm_fwd<TYPE, V, L, E>), dim3((unsigned)(want < most ? want : most)), dim3(TH), 0, st, d);
+        hipLaunchKernelGGL((k_block_norm_fwd<TYPE, V, L, TAIL>), dim3((unsigned)(want < most ? want : most)), dim3(TH), 0, st, d);
     } else {
-        const int nseq = d.gate_form == GATE_SEQUENCE ? (int)(d.rows / d.T) : 1;
-        hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, E>), dim3(bwd_groups(d, RPB), nseq), dim3(TH), 0, st, *b);
+        const dim3 grid(bwd_groups(d, RPB), d.gate_form == GATE_SEQUENCE ? (int)(d.rows / d.T) : 1);
+        if (d.b || d.nb) hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, TAIL, true>), grid, dim3(TH), 0, st, *b);
+        else hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, TAIL, false>), grid, dim3(TH), 0, st, *b);
     }
 }
 
-template <int TYPE, int V>
+template <int TYPE, bool TAIL>
 void pick_lanes(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hipStream_t st) {
-    int E;
-    const int L = lanes_of(d.D, E);
-    if (L == 16) run_norm<TYPE, V, 16, 8>(d, b, st);
-    else if (L == 64 && E == 8) run_norm<TYPE, V, 64, 8>(d, b, st);
-    else if (L == 64) run_norm<TYPE, V, 64, 16>(d, b, st);
-    else if (L == 256 && E == 8) run_norm<TYPE, V, 256, 8>(d, b, st);
-    else if (L == 256) run_norm<TYPE, V, 256, 16>(d, b, st);
-    else run_norm<TYPE, V, 512, 16>(d, b, st);
+    constexpr int V = TYPE == MEP_F32 ? 4 : 8;
+    switch (lanes_of(d.D)) {
+        case 16: return run_norm<TYPE, V, 16, TAIL>(d, b, st);
+        case 64: return run_norm<TYPE, V, 64, TAIL>(d, b, st);
+        case 128: return run_norm<TYPE, V, 128, TAIL>(d, b, st);
+        case 256: return run_norm<TYPE, V, 256, TAIL>(d, b, st);
+        case 512: return run_norm<TYPE, V, 512, TAIL>(d, b, st);
+        default: return run_norm<TYPE, V, 1024, TAIL>(d, b, st);
+    }
 }
 
 template <int TYPE>
-void pick_width(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hipStream_t st) {
-    if (aligned(d, b)) pick_lanes<TYPE, TYPE == MEP_F32 ? 4 : 8>(d, b, st);
-    else pick_lanes<TYPE, 1>(d, b, st);
+void pick_tail(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hipStream_t st) {
+    if (d.D % (TYPE == MEP_F32 ? 4 : 8)) pick_lanes<TYPE, true>(d, b, st);
+    else pick_lanes<TYPE, false>(d, b, st);
 }
 
 void run_type(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hipStream_t st) {
-    if (d.type == MEP_F32) pick_width<MEP_F32>(d, b, st);
-    else if (d.type == MEP_BF16) pick_width<MEP_BF16>(d, b, st);
-    else pick_width<MEP_F16>(d, b, st);
+    if (d.type == MEP_F32) pick_tail<MEP_F32>(d, b, st);
+    else if (d.type == MEP_BF16) pick_tail<MEP_BF16>(d, b, st);
+    else pick_tail<MEP_F16>(d, b, st);
 }
 
 bool norm_ok(const mep_block_norm_desc& d) {
@@ -408,12 +436,6 @@ bool norm_ok(const mep_block_norm_desc& d) {
     if (d.gate_form < GATE_NONE || d.gate_form > GATE_FULL || (d.gate_form != GATE_NONE) != (d.gate != 0)) return false;
     if (d.gate_form == GATE_SEQUENCE && (d.T < 1 || d.rows % d.T || d.rows / d.T > 65000)) return false;
     return d.eps >= 0.f;
-}
-
-int rows_per_block(int D) {
-    int E;
-    const int L = lanes_of(D, E);
-    return (L < 256 ? 256 : L) / L;
 }
 
 }  // namespace
@@ -429,7 +451,7 @@ extern "C" int mep_block_norm_partial(const mep_block_norm_desc* desc) {
     if (!desc || !norm_ok(*desc)) { mep_set_error("mep_block_norm_partial: invalid descriptor"); return MEP_EINVAL; }
     if (desc->rows == 0) return 0;
     const int nseq = desc->gate_form == GATE_SEQUENCE ? (int)(desc->rows / desc->T) : 1;
-    return bwd_groups(*desc, rows_per_block(desc->D)) * nseq * rows_per_block(desc->D);
+    return bwd_groups(*desc, rows_per_block(desc->D)) * nseq;
 }
 
 extern "C" int mep_block_norm_bwd(const mep_block_norm_bwd_desc* desc, mep_stream_t stream) {
@@ -450,7 +472,7 @@ extern "C" int mep_block_norm_bwd(const mep_block_norm_bwd_desc* desc, mep_strea
     int rc = mep_check_launch("mep_block_norm_bwd");
     if (rc || !b.partial) return rc;
     const int nseq = b.f.gate_form == GATE_SEQUENCE ? (int)(b.f.rows / b.f.T) : 1;
-    const int rpb = rows_per_block(b.f.D), rows_seq = bwd_groups(b.f, rpb) * rpb;
+    const int rows_seq = bwd_groups(b.f, rows_per_block(b.f.D));
     const int ny = sums - !!b.dgate + (b.dgate ? nseq : 0) + !!b.dscale;
     hipLaunchKernelGGL(k_block_norm_sums, dim3((b.f.D + NORM_SUM_COLS - 1) / NORM_SUM_COLS, ny),
                        dim3(NORM_SUM_COLS * NORM_SUM_SLICES), 0, st, b, rows_seq, nseq);

@@ -118,17 +118,8 @@ bool launch_rotary(const mep_rotary_desc& d, hipStream_t st) {
     return true;
 }
 
-// every chunk of V elements of the item layout lies inside the head and on a V-element boundary
-bool fits(const mep_rotary_desc& d, int V) {
-    const int es = d.type == MEP_F32 ? 4 : 2;
-    if ((d.rot / 2) % V || d.D % V || d.rot % V) return false;
-    for (int w = 0; w < 2; ++w) {
-        if (!d.x[w]) continue;
-        if (d.x[w] % (uint64_t)(V * es) || d.y[w] % (uint64_t)(V * es)) return false;
-        if (d.sB[w] % V || d.sT[w] % V || d.sH[w] % V || d.sM[w] % V) return false;
-    }
-    return true;
-}
+// every chunk of V elements of the item layout lies inside its part of the head (its address need not be aligned)
+bool fits(const mep_rotary_desc& d, int V) { return (d.rot / 2) % V == 0 && d.D % V == 0; }
 
 template <int TYPE>
 bool dispatch_rotary(const mep_rotary_desc& d, hipStream_t st) {
