@@ -88,6 +88,28 @@ MEP_DEV void store_row(MEP_G T* p, int lane, int D, const float (&v)[E]) {
         }
     }
 }
+// A row's elements as they lie in memory, on their way to registers a row ahead of their use
+template <class T, int V> struct RawRow { typename VecOf<T, V>::type v[E / V]; };
+template <class T, int V, int L, bool TAIL>
+MEP_DEV void fetch_row(const MEP_G T* p, int lane, int D, RawRow<T, V>& r) {
+#pragma unroll
+    for (int c = 0; c < E / V; ++c) {
+        const int col = (c * L + lane) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) r.v[c][j] = (T)0.f;
+        if (col + V <= D) {
+            r.v[c] = *reinterpret_cast<const MEP_G typename VecOf<T, V>::loose*>(p + col);
+        } else if (TAIL) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) if (col + j < D) r.v[c][j] = p[col + j];
+        }
+    }
+}
+template <class T, int V>
+MEP_DEV void widen(const RawRow<T, V>& r, float (&v)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = (float)r.v[i / V][i % V];
+}
 // a parameter row, fp32 or the activations' type; `miss` where there is none
 template <class T, int V, int L, bool TAIL>
 MEP_DEV void load_param(uint64_t p, int64_t off, bool wide, float miss, int lane, int D, float (&v)[E]) {
@@ -176,7 +198,7 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_fwd(mep_block_
 // Column sums of a workgroup: partial[seq * gridDim.x + blockIdx.x][n_sums][D] = those wanted of dw, db, dnw, dnb, dgate, and
 // the scalar dscale behind all of them.  gridDim.y sequences of d.T rows under a sequence gate, else one of all rows.
 template <int TYPE, int V, int L, bool TAIL, bool BIAS>
-__global__ __launch_bounds__(norm_threads<L>(), L >= 512 ? 4 : 2) void k_block_norm_bwd(mep_block_norm_bwd_desc bd) {
+__global__ __launch_bounds__(norm_threads<L>(), L > 512 ? 4 : 2) void k_block_norm_bwd(mep_block_norm_bwd_desc bd) {
     typedef typename ElemOf<TYPE>::T T;
     constexpr int RPB = norm_threads<L>() / L;
     const mep_block_norm_desc& d = bd.f;
@@ -200,17 +222,33 @@ __global__ __launch_bounds__(norm_threads<L>(), L >= 512 ? 4 : 2) void k_block_n
     const int64_t first = d.gate_form == GATE_SEQUENCE ? (int64_t)blockIdx.y * d.T : 0;
     const int64_t end = d.gate_form == GATE_SEQUENCE ? first + d.T : d.rows;
     int par = 0;
-    for (int64_t r0 = first + (int64_t)blockIdx.x * RPB; r0 < end; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    RawRow<T, V> ry, rx, rg, rs, rn;
+    f32x4 rst;
+    auto fetch = [&](int64_t r0) {
+        const int64_t rr = min(r0 + slot, end - 1);
+        fetch_row<T, V, L, TAIL>(G<const T>(d.y) + rr * d.y_ld, lane, D, ry);
+        if (d.x) fetch_row<T, V, L, TAIL>(G<const T>(d.x) + rr * d.x_ld, lane, D, rx);
+        if (d.gate_form == GATE_FULL) fetch_row<T, V, L, TAIL>(G<const T>(d.gate) + rr * d.g_ld, lane, D, rg);
+        if (bd.dstream) fetch_row<T, V, L, TAIL>(G<const T>(bd.dstream) + rr * bd.ds_ld, lane, D, rs);
+        if (next) fetch_row<T, V, L, TAIL>(G<const T>(bd.dnormed) + rr * bd.dn_ld, lane, D, rn);
+        rst = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * rr);
+    };
+    const int64_t r00 = first + (int64_t)blockIdx.x * RPB;
+    constexpr bool AHEAD = L < 1024;                 // 1024 threads have 128 registers each: no room for a row ahead
+    if (AHEAD && r00 < end) fetch(r00);
+    for (int64_t r0 = r00; r0 < end; r0 += step) {
         const int64_t row = r0 + slot;
         const bool live = row < end;                 // a slot past the end works on zeros and stores nothing
-        const int64_t rr = live ? row : end - 1;
         float y[E], x[E], g[E], h[E];
-        load_row<T, V, L, TAIL>(G<const T>(d.y) + rr * d.y_ld, lane, D, y);
-        if (d.x) load_row<T, V, L, TAIL>(G<const T>(d.x) + rr * d.x_ld, lane, D, x);
-        if (d.gate_form == GATE_FULL) load_row<T, V, L, TAIL>(G<const T>(d.gate) + rr * d.g_ld, lane, D, gc);
-        if (bd.dstream) load_row<T, V, L, TAIL>(G<const T>(bd.dstream) + rr * bd.ds_ld, lane, D, g);
-        if (next) load_row<T, V, L, TAIL>(G<const T>(bd.dnormed) + rr * bd.dn_ld, lane, D, h);
-        const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * rr);
+        if (!AHEAD) fetch(r0);
+        widen(ry, y);
+        if (d.x) widen(rx, x);
+        if (d.gate_form == GATE_FULL) widen(rg, gc);
+        if (bd.dstream) widen(rs, g);
+        if (next) widen(rn, h);
+        const f32x4 st = rst;
+        if (AHEAD && r0 + step < end) fetch(r0 + step);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             y[i] = (y[i] - st[0]) * st[1];           // yh
@@ -223,7 +261,7 @@ __global__ __launch_bounds__(norm_threads<L>(), L >= 512 ? 4 : 2) void k_block_n
             for (int i = 0; i < E; ++i) {
                 const float n = fmaf(y[i], w[i], bi[i]) * gc[i];
                 const float s = ((d.x ? fmaf(sc, x[i], n) : n) - st[2]) * st[3];   // the normalised stream
-                const float hi = live ? h[i] : 0.f;  // columns past D loaded zeros
+                const float hi = live ? h[i] : 0.f;  // columns past D hold zeros
                 anw[i] = fmaf(hi, s, anw[i]);
                 if constexpr (BIAS) anb[i] += hi;
                 const float u = hi * nw[i];
@@ -237,8 +275,8 @@ __global__ __launch_bounds__(norm_threads<L>(), L >= 512 ? 4 : 2) void k_block_n
             for (int i = 0; i < E; ++i) {
                 const float n = fmaf(y[i], w[i], bi[i]) * gc[i];
                 const float s = ((d.x ? fmaf(sc, x[i], n) : n) - st[2]) * st[3];
-                // columns past D hold garbage here; they meet zero gradients only in the sums above, and are
-                // cleared so that they add nothing below
+                // columns past D hold values here, which meet only zeros in the sums above; they are cleared so that
+                // they add nothing below
                 g[i] = ((i / V) * L + lane) * V + i % V < D && live ? g[i] + st[3] * (h[i] - mu - s * mq) : 0.f;
             }
         }
@@ -379,12 +417,13 @@ int rows_per_block(int D) {
     return (L < 256 ? 256 : L) / L;
 }
 
-// workgroups per sequence of the backward: two per compute unit over all sequences, at least 4 rows a slot
+// workgroups per sequence of the backward: as many as the compute units hold over all sequences, at least 4 rows a slot
 // where there are so many (each workgroup's column sums cost 5 D floats), never more than its rows ask for
 int bwd_groups(const mep_block_norm_desc& d, int rpb) {
     const int64_t nseq = d.gate_form == GATE_SEQUENCE ? d.rows / d.T : 1;
     const int64_t rows = d.rows / nseq;
-    int64_t most = (512 + nseq - 1) / nseq, want = (rows + 4 * rpb - 1) / (4 * rpb);
+    const int all = rpb == 1 && d.D > 2048 ? 256 : 512;      // of 512 threads and more, one fits a compute unit
+    int64_t most = (all + nseq - 1) / nseq, want = (rows + 4 * rpb - 1) / (4 * rpb);
     const int64_t n = want < most ? want : most;
     return (int)(n < 1 ? 1 : n);
 }

@@ -5,20 +5,33 @@ namespace {
 
 using namespace mep;
 
-// dlam[h] = -sum of A_2 dP over batch and queries, in a fixed order
-__global__ __launch_bounds__(DA_THREADS) void k_diff_dlam(mep_diff_attn_bwd_desc bd) {
+// dlam[h] = -sum of A_2 dP over batch and queries, in a fixed order: a workgroup per head, threads over the rows, then the waves
+constexpr int DLAM_THREADS = 1024;
+__global__ __launch_bounds__(DLAM_THREADS) void k_diff_dlam(mep_diff_attn_bwd_desc bd) {
     const mep_diff_attn_desc& d = bd.f;
-    __shared__ float part[DA_WAVES];
+    __shared__ float part[DLAM_THREADS / 64];
     const int h = blockIdx.x;
+    const int64_t n = (int64_t)d.B * d.Tq;
     float s = 0.f;
-    for (int b = 0; b < d.B; ++b) {
-        const gfloat* p = G<const float>(bd.delta) + 4 * ((int64_t)b * d.H + h) * d.Tq + 1;
-        for (int t = threadIdx.x; t < d.Tq; t += DA_THREADS) s -= p[4 * (int64_t)t];
+    auto at = [&](int64_t i) {
+        const int64_t b = i / d.Tq;
+        return G<const float>(bd.delta)[4 * ((b * d.H + h) * d.Tq + (i - b * d.Tq)) + 1];
+    };
+    int64_t i = threadIdx.x;
+    for (; i + 3 * DLAM_THREADS < n; i += 4 * DLAM_THREADS) {      // four loads in flight
+        const float a = at(i), b = at(i + DLAM_THREADS), c = at(i + 2 * DLAM_THREADS), e = at(i + 3 * DLAM_THREADS);
+        s -= (a + b) + (c + e);
     }
+    for (; i < n; i += DLAM_THREADS) s -= at(i);
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) G<float>(bd.dlam)[h] = (part[0] + part[1]) + (part[2] + part[3]);
+    if (threadIdx.x == 0) {
+        s = part[0];
+#pragma unroll
+        for (int w = 1; w < DLAM_THREADS / 64; ++w) s += part[w];
+        G<float>(bd.dlam)[h] = s;
+    }
 }
 
 // rows that can be read 16 bytes at a time, a tile of 64 time steps with all its heads and maps within 2^30 elements (the DMA's
@@ -129,6 +142,6 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
     if (rows) run(DA_BWD_Q, d, &b, qg, qb, st);
     if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, st);
-    if (b.dlam) hipLaunchKernelGGL(k_diff_dlam, dim3(d.H), dim3(DA_THREADS), 0, st, b);
+    if (b.dlam) hipLaunchKernelGGL(k_diff_dlam, dim3(d.H), dim3(DLAM_THREADS), 0, st, b);
     return mep_check_launch("mep_diff_attn_bwd");
 }
