@@ -796,6 +796,7 @@ typedef struct {
     int32_t  B, Tq, Tk, H, G, d, dv, type;
     int32_t  causal, mask_form, mask_float;
     float    scale;
+    uint64_t workspace;          /* mep_diff_attn_workspace bytes, 16-byte aligned, or 0: the keys are not split */
 } mep_diff_attn_desc;
 typedef struct {
     mep_diff_attn_desc f;
@@ -815,6 +816,9 @@ typedef struct {
 } mep_pack_rows_desc;
 int mep_pack_rows(const mep_pack_rows_desc* desc, mep_stream_t stream);
 int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_t stream);
+/* bytes that a forward of these sizes (B, Tq, Tk, H, G, d, dv, type) uses to split its keys over workgroups: 0 where it does
+ * not; < 0: MEP_EINVAL */
+int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc);
 
 /* ---------------------------------------------------------------- misc */
 int mep_abi_version(void);

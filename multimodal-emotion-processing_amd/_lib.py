@@ -293,7 +293,7 @@ class DiffAttnDesc(ctypes.Structure):
                 ('k_sM', i64), ('v_sB', i64), ('v_sT', i64), ('v_sH', i64), ('lam_sB', i64), ('lam_sT', i64), ('lam_sH', i64),
                 ('mask', u64), ('m_sB', i64), ('m_sQ', i64), ('m_sK', i64), ('lengths', u64), ('q_start', u64),
                 ('B', i32), ('Tq', i32), ('Tk', i32), ('H', i32), ('G', i32), ('d', i32), ('dv', i32), ('type', i32),
-                ('causal', i32), ('mask_form', i32), ('mask_float', i32), ('scale', f32)]
+                ('causal', i32), ('mask_form', i32), ('mask_float', i32), ('scale', f32), ('workspace', u64)]
 
 
 class DiffAttnBwdDesc(ctypes.Structure):
@@ -351,6 +351,7 @@ SIGNATURES.update({
     'mep_tgemm': [P, i32, i32, i32, i32, P],
     'mep_diff_attn_fwd': [ctypes.POINTER(DiffAttnDesc), P],
     'mep_diff_attn_bwd': [ctypes.POINTER(DiffAttnBwdDesc), P],
+    'mep_diff_attn_workspace': [ctypes.POINTER(DiffAttnDesc)],
     'mep_pack_rows': [ctypes.POINTER(PackRowsDesc), P],
     'mep_rotary': [ctypes.POINTER(RotaryDesc), P],
     'mep_block_norm_fwd': [ctypes.POINTER(BlockNormDesc), P],
@@ -371,6 +372,8 @@ SIGNATURES.update({
     'mep_stamp_khz': [],
 })
 
+RESTYPES = {'mep_diff_attn_workspace': i64}   # the others return int
+
 _LIB = None
 ABI_VERSION = 7   # include/mep.h MEP_ABI_VERSION
 
@@ -386,7 +389,7 @@ def lib():
         for name, args in SIGNATURES.items():
             fn = getattr(L, name)
             fn.argtypes = args
-            fn.restype = ctypes.c_int
+            fn.restype = RESTYPES.get(name, ctypes.c_int)
         if L.mep_abi_version() != ABI_VERSION:   # descriptor layouts would not match: fail loudly
             raise OSError('%s has ABI %d, this host expects %d: rebuild it' % (LIB_PATH, L.mep_abi_version(), ABI_VERSION))
         _LIB = L

@@ -32,7 +32,10 @@ constexpr int DA_THREADS = 256, DA_WAVES = 4, DA_ROWS = 32 * DA_WAVES;
 constexpr float DA_LOG2E = 1.4426950408889634f;
 constexpr float DA_MIN = -1.0e30f;      // the running maximum's start: finite, so that masked scores (-inf) give 2^-inf = 0
 constexpr unsigned DA_NOWHERE = 0x80000000u, DA_SPAN = 0x7fffffffu;   // a DMA offset behind the span reads zeros
-enum { DA_FWD, DA_BWD_Q, DA_BWD_KV };
+enum { DA_FWD, DA_BWD_Q, DA_BWD_KV, DA_SPLIT };
+
+// keys of a tile of k_diff_split: 64 where two tiles fit 160 KB of LDS
+constexpr int da_split_keys(int type, int dk, int dv) { return (type == MEP_F32 ? 4 : 2) * 2 * 64 * (2 * dk + dv) <= 160 * 1024 ? 64 : 32; }
 
 // One 16-byte operand of a lane: E consecutive k of a 2 E step
 template <int TYPE> struct Mat;
@@ -117,15 +120,15 @@ MEP_DEV i32x4 da_buffer(const MEP_G void* p) {
 }
 
 // ROWS x COLS of LDS from rows of global memory, by DMA: an instruction of a wave fills 64 chunks, and instruction i of a
-// lane takes chunk `chunk(i)` of row `row + i STEP`.  The chunk does not depend on i (with 4 rows a step, on its
-// parity alone), so neither does the lane's offset, and a tile costs no address arithmetic: the row steps are the scalar offset.
+// lane takes chunk `chunk(i)` of row `row + i STEP`.  The chunk does not depend on i (with 4 or 2 rows a
+// step, on i modulo 2 or 4 alone), so neither does the lane's offset, and a tile costs no address arithmetic: the row steps are the scalar offset.
 template <class M, int ROWS, int COLS, int THREADS = DA_THREADS>
 struct Stager {
     typedef Lay<M, COLS> L;
     typedef typename M::T T;
-    static constexpr int STEP = THREADS / L::CH < ROWS ? THREADS / L::CH : ROWS, N = ROWS / STEP, NO = STEP % 8 ? 2 : 1;
+    static constexpr int STEP = THREADS / L::CH < ROWS ? THREADS / L::CH : ROWS, N = ROWS / STEP, NO = STEP % 8 ? 8 / STEP : 1;
     static constexpr bool ALL = STEP * L::CH == THREADS;      // else only the first waves load
-    static_assert(STEP >= 4 && ROWS % STEP == 0, "tile");
+    static_assert(STEP >= 2 && ROWS % STEP == 0, "tile");
     int row;
     unsigned off[NO];                // byte offset of the lane's chunk in row `row`, or DA_NOWHERE
     static MEP_DEV int chunk(int tid, int i) { return (tid % L::CH) ^ L::sw(tid / L::CH + i * STEP); }
@@ -374,12 +377,12 @@ struct KeyTiles {
     }
 };
 
-// the rows of a wave: lane's row, its query and head, and what the wave's keys are
+// the rows of a wave from `first` on: lane's row, its query and head, and what the wave's keys are
 struct Rows32 {
     int row0, row, t, head, wend, wfull;
     bool live;
-    MEP_DEV Rows32(const mep_diff_attn_desc& d, const Job& j) {
-        row0 = j.block * DA_ROWS + (threadIdx.x >> 6) * 32;
+    MEP_DEV Rows32(const mep_diff_attn_desc& d, const Job& j, int first) {
+        row0 = first;
         row = row0 + (threadIdx.x & 31);
         live = row < j.rows;
         const int rr = live ? row : j.rows - 1;
@@ -437,43 +440,124 @@ MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, i
 // The maxima m_m are renewed only when a score exceeds one by 8 (e <= 256: the sums are as exact), the lanes of a row agree on them, and
 // the sums l_m stay lane-local to the end.
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks) {
+struct Online {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
     typedef typename Ge::Frag Frag;
+    // The backward's e_m are to be at most 1: it gets maxima 8 up, or in float16, whose subnormals begin at 2^-14, the true ones
+    static constexpr bool TOP = TYPE == MEP_F16;
+    Frag q[2][Ge::NK];
+    float c, lam, m1, m2, l1, l2, f1, f2, top1, top2;
+    floatx16 x[DV / 32], y[DV / 32];
+
+    MEP_DEV Online(const mep_diff_attn_desc& d, const Job& j, const Rows32& w) {
+        const int h = (threadIdx.x & 63) >> 5;
+        const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < Ge::NK; ++i) q[m][i] = row_frag<M>(qp + m * d.q_sM, M::KS * i + M::E * h, d.d, w.live);
+        lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
+        c = d.scale * DA_LOG2E;
+        m1 = m2 = mul_rn(DA_MIN, c);
+        l1 = l2 = f2 = 0.f;
+        f1 = 1.f;
+        top1 = top2 = DA_MIN;
+#pragma unroll
+        for (int n = 0; n < DV / 32; ++n) x[n] = y[n] = zero16();
+    }
+    // the 32 keys from ks on, rows r0 .. of the tile
+    MEP_DEV void step(const mep_diff_attn_desc& d, const Job& j, const Rows32& w, const Reader<M, 2 * DK>& kread, const Reader<M, DV>& vread,
+                      const T* kt, const T* vt, int r0, int ks, unsigned on) {
+        floatx16 s1 = zero16(), s2 = zero16();
+#pragma unroll
+        for (int i = 0; i < Ge::NK; ++i) {
+            s1 = M::mma(kread.rows(kt, r0, i), q[0][i], s1);
+            s2 = M::mma(kread.rows(kt, r0, Ge::NK + i), q[1][i], s2);
+        }
+        if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
+        const float a1 = max16(s1), a2 = max16(s2);
+        if constexpr (TOP) {
+            top1 = fmaxf(top1, a1);
+            top2 = fmaxf(top2, a2);
+        }
+        if (__ballot(a1 * c > m1 + 8.f || a2 * c > m2 + 8.f)) {
+            const float n1 = fmaxf(m1, mul_rn(half_max(a1), c)), n2 = fmaxf(m2, mul_rn(half_max(a2), c));
+            const float g1 = exp2_fast(m1 - n1), g2 = exp2_fast(m2 - n2);
+            l1 *= g1;
+            l2 *= g2;
+            m1 = n1;
+            m2 = n2;
+#pragma unroll
+            for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[n][r] = fmaf(f2, y[n][r], x[n][r]) * g1;      // f1 E_1 alone: g2 may be 0
+                    y[n][r] *= g2;
+                }
+            f2 = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s1[r] = exp2_fast(fmaf(s1[r], c, -m1));
+            s2[r] = exp2_fast(fmaf(s2[r], c, -m2));
+            l1 += s1[r];
+            l2 += s2[r];
+        }
+        const float t1 = lam * half_sum(l1), t2 = half_sum(l2);
+        if (__ballot(fabsf(t1 * f1 - t2 * f2) > 0.25f * fabsf(t1 * f1))) {
+            const float rho = t2 > 0.f ? t1 / t2 : 0.f, h1 = 1.f / fmaxf(1.f, fabsf(rho)), h2 = rho * h1;
+            const float u = h1 / f1, v = u * f2 - h2;
+#pragma unroll
+            for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[n][r] = fmaf(x[n][r], u, y[n][r] * v);
+            f1 = h1;
+            f2 = h2;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s1[r] = fmaf(s1[r], f1, -f2 * s2[r]);
+#pragma unroll
+        for (int i = 0; i < Ge::NP; ++i) {
+            const Frag p = acc_frag<M>(s1, i), e = acc_frag<M>(s2, i);
+#pragma unroll
+            for (int n = 0; n < DV / 32; ++n) {
+                const Frag v = vread.cols(vt, r0, 32 * n, i);
+                x[n] = M::mma(v, p, x[n]);
+                y[n] = M::mma(v, e, y[n]);
+            }
+        }
+    }
+    // the maxima that the backward gets, and 2^(m - those)
+    MEP_DEV void maxima(float& n1, float& n2, float& g1, float& g2) const {      // (one rounding, as m1, m2: without keys g = 1)
+        n1 = TOP ? mul_rn(half_max(top1), c) : m1 + 8.f;
+        n2 = TOP ? mul_rn(half_max(top2), c) : m2 + 8.f;
+        g1 = exp2_fast(m1 - n1);
+        g2 = exp2_fast(m2 - n2);
+    }
+};
+
+template <int TYPE, int DK, int DV>
+__global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks) {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef typename Ge::M M;
+    typedef typename Ge::T T;
     constexpr int KT = Ge::KT;
     __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
     const Job j = make_job(d, blocks, d.causal);
     const int h = (threadIdx.x & 63) >> 5;
-    const Rows32 w(d, j);
+    const Rows32 w(d, j, j.block * DA_ROWS + (threadIdx.x >> 6) * 32);
     const KeyTiles<TYPE, DK, DV> keys(d, j);
     const Reader<M, 2 * DK> kread;
     const Reader<M, DV> vread;
-    const float c = d.scale * DA_LOG2E;
     const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
 
     unsigned raw = key_raw(d, j, 0);
     unsigned long long bits = key_bits(d, j, 0, KT, raw);
     if (end > 0) keys.load(Buf, 0, bits);
     raw = key_raw(d, j, KT);
-    Frag q[2][Ge::NK];
-    {
-        const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < Ge::NK; ++i)
-                q[m][i] = row_frag<M>(qp + m * d.q_sM, M::KS * i + M::E * h, d.d, w.live);
-    }
-    const float lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
-
-    // The backward's e_m are to be at most 1: it gets maxima 8 up, or in float16, whose subnormals begin at 2^-14, the true ones
-    constexpr bool TOP = TYPE == MEP_F16;
-    float m1 = mul_rn(DA_MIN, c), m2 = m1, l1 = 0.f, l2 = 0.f, f1 = 1.f, f2 = 0.f, top1 = DA_MIN, top2 = DA_MIN;
-    floatx16 x[DV / 32], y[DV / 32];
-#pragma unroll
-    for (int n = 0; n < DV / 32; ++n) x[n] = y[n] = zero16();
+    Online<TYPE, DK, DV> o(d, j, w);
     for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
         tile_sync();
         const unsigned long long now = bits;
@@ -483,81 +567,21 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
             raw = key_raw(d, j, k0 + 2 * KT);
         }
         const T* kt = Buf + buf * Ge::TSZ;
-        const T* vt = kt + Ge::KSZ;
 #pragma unroll 1
         for (int sub = 0; sub < KT / 32; ++sub) {
             const int ks = k0 + 32 * sub;
             const unsigned on = (unsigned)(now >> (32 * sub));
-            if (ks >= w.wend || !on) continue;
-            floatx16 s1 = zero16(), s2 = zero16();
-#pragma unroll
-            for (int i = 0; i < Ge::NK; ++i) {
-                s1 = M::mma(kread.rows(kt, 32 * sub, i), q[0][i], s1);
-                s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q[1][i], s2);
-            }
-            if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
-            const float a1 = max16(s1), a2 = max16(s2);
-            if constexpr (TOP) {
-                top1 = fmaxf(top1, a1);
-                top2 = fmaxf(top2, a2);
-            }
-            if (__ballot(a1 * c > m1 + 8.f || a2 * c > m2 + 8.f)) {
-                const float n1 = fmaxf(m1, mul_rn(half_max(a1), c)), n2 = fmaxf(m2, mul_rn(half_max(a2), c));
-                const float g1 = exp2_fast(m1 - n1), g2 = exp2_fast(m2 - n2);
-                l1 *= g1;
-                l2 *= g2;
-                m1 = n1;
-                m2 = n2;
-#pragma unroll
-                for (int n = 0; n < DV / 32; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        x[n][r] = fmaf(f2, y[n][r], x[n][r]) * g1;      // f1 E_1 alone: g2 may be 0
-                        y[n][r] *= g2;
-                    }
-                f2 = 0.f;
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s1[r] = exp2_fast(fmaf(s1[r], c, -m1));
-                s2[r] = exp2_fast(fmaf(s2[r], c, -m2));
-                l1 += s1[r];
-                l2 += s2[r];
-            }
-            const float t1 = lam * half_sum(l1), t2 = half_sum(l2);
-            if (__ballot(fabsf(t1 * f1 - t2 * f2) > 0.25f * fabsf(t1 * f1))) {
-                const float rho = t2 > 0.f ? t1 / t2 : 0.f, h1 = 1.f / fmaxf(1.f, fabsf(rho)), h2 = rho * h1;
-                const float u = h1 / f1, v = u * f2 - h2;
-#pragma unroll
-                for (int n = 0; n < DV / 32; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[n][r] = fmaf(x[n][r], u, y[n][r] * v);
-                f1 = h1;
-                f2 = h2;
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s1[r] = fmaf(s1[r], f1, -f2 * s2[r]);
-#pragma unroll
-            for (int i = 0; i < Ge::NP; ++i) {
-                const Frag p = acc_frag<M>(s1, i), e = acc_frag<M>(s2, i);
-#pragma unroll
-                for (int n = 0; n < DV / 32; ++n) {
-                    const Frag v = vread.cols(vt, 32 * sub, 32 * n, i);
-                    x[n] = M::mma(v, p, x[n]);
-                    y[n] = M::mma(v, e, y[n]);
-                }
-            }
+            if (ks < w.wend && on) o.step(d, j, w, kread, vread, kt, kt + Ge::KSZ, 32 * sub, ks, on);
         }
     }
-    l1 = half_sum(l1);
-    l2 = half_sum(l2);
-    const float i1 = l1 > 0.f ? 1.f / l1 : l1, i2 = l2 > 0.f ? 1.f / l2 : l2;
-    // (one rounding, as m1 and m2 have: without keys the differences are 0)
-    const float n1 = TOP ? mul_rn(half_max(top1), c) : m1 + 8.f, n2 = TOP ? mul_rn(half_max(top2), c) : m2 + 8.f;
+    o.l1 = half_sum(o.l1);
+    o.l2 = half_sum(o.l2);
+    const float i1 = o.l1 > 0.f ? 1.f / o.l1 : o.l1, i2 = o.l2 > 0.f ? 1.f / o.l2 : o.l2;
+    float n1, n2, g1, g2;
+    o.maxima(n1, n2, g1, g2);
     if (d.stats && w.live && h == 0)
-        *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) =
-            f32x4{n1, i1 * exp2_fast(n1 - m1), n2, i2 * exp2_fast(n2 - m2)};
-    const float fx = i1 / f1, fy = fx * f2 - lam * i2;
+        *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) = f32x4{n1, i1 / g1, n2, i2 / g2};
+    const float fx = i1 / o.f1, fy = fx * o.f2 - o.lam * i2;
     tile_sync();                             // the tiles are free
     const int64_t first = (int64_t)j.b * d.Tq * d.H * d.dv;
     auto row_at = [&](uint64_t p, int r) -> MEP_G T* {
@@ -570,9 +594,94 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
 #pragma unroll
     for (int n = 0; n < DV / 32; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[n][r] = fmaf(x[n][r], fx, y[n][r] * fy);
-    write_rows<M>(mine, x, 1.f, d.dv, [&](int r) { return row_at(d.out, r); });
-    if (d.second) write_rows<M>(mine, y, i2, d.dv, [&](int r) { return row_at(d.second, r); });
+        for (int r = 0; r < 16; ++r) o.x[n][r] = fmaf(o.x[n][r], fx, o.y[n][r] * fy);
+    write_rows<M>(mine, o.x, 1.f, d.dv, [&](int r) { return row_at(d.out, r); });
+    if (d.second) write_rows<M>(mine, o.y, i2, d.dv, [&](int r) { return row_at(d.second, r); });
+}
+
+// ------------------------------------------------------------------ forward over split keys
+// Few rows against many keys (single tokens against a cache): a workgroup of two waves takes 32 rows and some tiles of 64
+// keys (32 where two of 64 do not fit LDS), a wave the even or the odd 32 of them, and each wave leaves its row maxima, sums, E_1
+// and E_2 in fp32; k_diff_join joins them.  Bound by reading the keys and values once: two tiles in flight in each of two workgroups
+// on a compute unit.
+// workspace of a wave's 32 rows: (m1, l1, m2, l2)[32], E_1 [32][dv], E_2 [32][dv]
+MEP_DEV int64_t split_floats(int dv) { return 32 * (4 + 2 * (int64_t)dv); }
+
+template <int TYPE, int DK, int DV>
+__global__ __launch_bounds__(128, DV >= 128 || DK >= 128 ? 1 : 2) void k_diff_split(mep_diff_attn_desc d, int blocks, int splits, int tiles) {
+    typedef Geo<TYPE, DK, DV> Ge;
+    typedef typename Ge::M M;
+    typedef typename Ge::T T;
+    constexpr int KT = da_split_keys(TYPE, DK, DV), KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;
+    __shared__ __align__(16) T Buf[2 * TSZ];
+    const Job j = make_job(d, blocks * splits, false);
+    const int wave = threadIdx.x >> 6, h = (threadIdx.x & 63) >> 5;
+    const int rb = j.block / splits, split = j.block - rb * splits;
+    const Rows32 w(d, j, rb * 32);
+    const int end = min(w.wend, (split + 1) * tiles * KT), begin = split * tiles * KT;
+    const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
+    const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
+    const Reader<M, 2 * DK> kread;
+    const Reader<M, DV> vread;
+    auto load = [&](T* tile, int k0, unsigned long long bits) {
+        const int tid = thread_again();
+        const Stager<M, KT, 2 * DK, 128> ks(tid, (unsigned)d.k_sT, [&](int ch) {
+            const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
+            return col < d.d ? col + (m ? (int)d.k_sM : 0) : -1;
+        });
+        ks.load(tile, kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
+        const Stager<M, KT, DV, 128> vs(tid, (unsigned)d.v_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
+        vs.load(tile + KSZ, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
+    };
+    unsigned raw = key_raw(d, j, begin);
+    unsigned long long bits = key_bits(d, j, begin, KT, raw);
+    if (begin < end) load(Buf, begin, bits);
+    raw = key_raw(d, j, begin + KT);
+    Online<TYPE, DK, DV> o(d, j, w);
+    for (int k0 = begin, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+        tile_sync();
+        const unsigned long long now = bits;
+        if (k0 + KT < end) {
+            bits = key_bits(d, j, k0 + KT, KT, raw);
+            load(Buf + (buf ^ 1) * TSZ, k0 + KT, bits);
+            raw = key_raw(d, j, k0 + 2 * KT);
+        }
+        const int sub = KT == 64 ? wave : 0, ks = k0 + 32 * sub;      // one sub-tile a tile: the waves take turns
+        const unsigned on = (unsigned)(now >> (32 * sub));
+        if ((KT == 64 || ((k0 - begin) / KT & 1) == wave) && ks < end && on)
+            o.step(d, j, w, kread, vread, Buf + buf * TSZ, Buf + buf * TSZ + KSZ, 32 * sub, ks, on);
+    }
+    float n1, n2, g1, g2;
+    o.maxima(n1, n2, g1, g2);
+    const float l1 = half_sum(o.l1) * g1, l2 = half_sum(o.l2) * g2;
+    gfloat* part = G<float>(d.workspace) + ((((int64_t)j.b * d.G + j.g) * blocks + rb) * splits * 2 + split * 2 + wave) * split_floats(d.dv);
+    if (!w.live) return;
+    const int row = threadIdx.x & 31;
+    if (h == 0) *reinterpret_cast<MEP_G f32x4*>(part + 4 * row) = f32x4{n1, l1, n2, l2};
+    if (!(l1 != 0.f || l2 != 0.f)) return;      // no key of this row here: the join reads no further
+    const float fx = g1 / o.f1;
+    gfloat* e1 = part + 128 + row * d.dv;
+    gfloat* e2 = e1 + 32 * d.dv;
+#pragma unroll
+    for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int col = 32 * n + acc_off(r) + 4 * h;
+            float a[4], b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = fmaf(o.f2, o.y[n][r + e], o.x[n][r + e]) * fx;
+                b[e] = o.y[n][r + e] * g2;
+            }
+            if (col + 4 <= d.dv) {
+                store_f32<float, 4>(e1 + col, a);
+                store_f32<float, 4>(e2 + col, b);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < d.dv) { e1[col + e] = a[e]; e2[col + e] = b[e]; }
+            }
+        }
 }
 
 // ------------------------------------------------------------------ backward: D and dq
@@ -594,7 +703,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
     __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
     const Job j = make_job(d, blocks, d.causal);
     const int h = (threadIdx.x & 63) >> 5;
-    const Rows32 w(d, j);
+    const Rows32 w(d, j, j.block * DA_ROWS + (threadIdx.x >> 6) * 32);
     const KeyTiles<TYPE, DK, DV> keys(d, j);
     const Reader<M, 2 * DK> kread;
     const Reader<M, DV> vread;
@@ -1098,27 +1207,34 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
 constexpr int da_kw(int type, int dk) { return dk >= 128 || (type == MEP_F32 && dk >= 64) ? 2 : 4; }
 
 template <int TYPE, int DK, int DV>
-void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
+void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {
     if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks);
+    else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, DV>), dim3(grid), dim3(128), 0, st, d, blocks, splits, tiles);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
                             dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks);
 }
 
 // the smallest instance that holds the head widths
+// (its DK; its DV)
 inline int da_width(int d, int dv) { return d <= 32 && dv <= 64 ? 32 : d <= 64 && dv <= 128 ? 64 : 128; }
+inline int da_value_width(int d, int dv) {
+    const int dk = da_width(d, dv);
+    return dk == 32 ? (dv <= 32 ? 32 : 64) : dk == 64 ? (dv <= 64 ? 64 : 128) : (dv <= 128 ? 128 : 256);
+}
 template <int TYPE>
-void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st) {
-    if (d.d <= 32 && d.dv <= 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, st);
-    else if (d.d <= 32 && d.dv <= 64) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, st);
-    else if (d.d <= 64 && d.dv <= 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, st);
-    else if (d.d <= 64 && d.dv <= 128) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, st);
-    else if (d.dv <= 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, st);
-    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, st);
+void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {
+    const int dk = da_width(d.d, d.dv), dv = da_value_width(d.d, d.dv);
+    if (dk == 32 && dv == 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, splits, tiles, st);
+    else if (dk == 32) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, splits, tiles, st);
+    else if (dk == 64 && dv == 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, splits, tiles, st);
+    else if (dk == 64) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, splits, tiles, st);
+    else if (dv == 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, splits, tiles, st);
+    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, splits, tiles, st);
 }
 
-void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st);
-void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st);
-void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, hipStream_t st);
+void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st);
+void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st);
+void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st);
 
 }  // namespace mep

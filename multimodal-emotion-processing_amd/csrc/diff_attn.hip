@@ -34,6 +34,50 @@ __global__ __launch_bounds__(DLAM_THREADS) void k_diff_dlam(mep_diff_attn_bwd_de
     }
 }
 
+// out = E_1 / l_1 - lam E_2 / l_2 of a row from its parts, a thread per value channel; rows side by side in a workgroup
+__global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, int blocks, int parts, int per) {
+    const int ch = threadIdx.x % per;
+    const int64_t r = (int64_t)blockIdx.x * (DA_THREADS / per) + threadIdx.x / per;      // (b, t, head)
+    if (r >= (int64_t)d.B * d.Tq * d.H) return;
+    const int64_t bt = r / d.H;
+    const int head = (int)(r - bt * d.H), b = (int)(bt / d.Tq), t = (int)(bt - (int64_t)b * d.Tq);
+    const int n = d.H / d.G, g = head / n, row = t * n + head - g * n;
+    const int64_t stride = split_floats(d.dv);
+    const gfloat* part = G<const float>(d.workspace) + (((int64_t)b * d.G + g) * blocks + row / 32) * parts * stride;
+    const int lr = row & 31;
+    float m1 = -INFINITY, m2 = -INFINITY;
+    for (int p = 0; p < parts; ++p) {
+        const f32x4 s = *reinterpret_cast<const MEP_G f32x4*>(part + p * stride + 4 * lr);
+        m1 = fmaxf(m1, s[0]);
+        m2 = fmaxf(m2, s[2]);
+    }
+    float l1 = 0.f, l2 = 0.f, e1 = 0.f, e2 = 0.f;
+    for (int p = 0; p < parts; ++p) {
+        const gfloat* q = part + p * stride;
+        const f32x4 s = *reinterpret_cast<const MEP_G f32x4*>(q + 4 * lr);
+        if (!(s[1] != 0.f || s[3] != 0.f)) continue;      // no key of this row there, and nothing written
+        const float w1 = exp2_fast(s[0] - m1), w2 = exp2_fast(s[2] - m2);
+        l1 = fmaf(s[1], w1, l1);
+        l2 = fmaf(s[3], w2, l2);
+        if (ch < d.dv) {
+            e1 = fmaf(q[128 + lr * d.dv + ch], w1, e1);
+            e2 = fmaf(q[128 + (32 + lr) * d.dv + ch], w2, e2);
+        }
+    }
+    const float i1 = l1 > 0.f ? 1.f / l1 : l1, i2 = l2 > 0.f ? 1.f / l2 : l2;
+    const float lam = G<const float>(d.lam)[(int64_t)b * d.lam_sB + (int64_t)t * d.lam_sT + (int64_t)head * d.lam_sH];
+    if (d.stats && ch == 0) *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)b * d.H + head) * d.Tq + t)) = f32x4{m1, i1, m2, i2};
+    if (ch >= d.dv) return;
+    auto put = [&](uint64_t p, float v) {
+        const int64_t o = r * d.dv + ch;
+        if (d.type == MEP_F32) G<float>(p)[o] = v;
+        else if (d.type == MEP_BF16) G<__bf16>(p)[o] = (__bf16)v;
+        else G<_Float16>(p)[o] = (_Float16)v;
+    };
+    put(d.out, fmaf(e1, i1, -lam * (e2 * i2)));
+    if (d.second) put(d.second, e2 * i2);
+}
+
 // rows that can be read 16 bytes at a time, a tile of 64 time steps with all its heads and maps within 2^30 elements (the DMA's
 // 32-bit byte offsets)
 bool rows_ok(const mep_diff_attn_desc& d, uint64_t p, int64_t sB, int64_t sT, int64_t sH, int64_t sM, bool heads) {
@@ -53,16 +97,43 @@ int64_t plan(const mep_diff_attn_desc& d, int64_t items, int per, int& blocks) {
     return grid < 1 << 23 ? grid : -1;            // of up to 512 threads: 2^32 threads are a launch's most
 }
 
-void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, hipStream_t st) {
-    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, st);
-    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, st);
-    else da_run_f16(what, d, b, (unsigned)grid, blocks, st);
+// How the keys of a forward are split, or splits = 0: not at all.  Worth it where the rows are few: up to 32 a (batch, key head) leave
+// three of k_diff_fwd's four waves idle (against a row of 8192 keys, 32 batch rows, 4 key heads: 297 us whole, see k_diff_split),
+// and more rows too when their workgroups are under half the compute units and there are 1024 keys.  Then 8 workgroups
+// a compute unit at most, and 4 tiles each at least.
+struct Split { int blocks, splits, tiles; };
+Split split_of(const mep_diff_attn_desc& d) {
+    Split s = {0, 0, 0};
+    const int64_t rows = (int64_t)d.Tq * (d.H / d.G), pairs = (int64_t)d.B * d.G;
+    const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) < 128;
+    if (pairs == 0 || rows == 0 || !(few || none)) return s;
+    s.blocks = (int)((rows + 31) / 32);
+    const int kt = da_split_keys(d.type, da_width(d.d, d.dv), da_value_width(d.d, d.dv)), all = (d.Tk + kt - 1) / kt;
+    const int64_t want = 2048 / (pairs * s.blocks);
+    s.splits = (int)(want < 1 ? 1 : want > (all + 3) / 4 ? (all + 3) / 4 : want);
+    s.tiles = (all + s.splits - 1) / s.splits;
+    s.splits = (all + s.tiles - 1) / s.tiles;
+    if (pairs * s.blocks * s.splits >= 1 << 23) s.splits = 0;
+    return s;
+}
+int64_t split_bytes(const mep_diff_attn_desc& d, const Split& s) {
+    return (int64_t)d.B * d.G * s.blocks * s.splits * 2 * 32 * (4 + 2 * (int64_t)d.dv) * 4;
 }
 
-bool attn_ok(const mep_diff_attn_desc& d) {
+void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, int tiles, hipStream_t st) {
+    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, tiles, st);
+    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, tiles, st);
+    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, tiles, st);
+}
+
+bool attn_shape_ok(const mep_diff_attn_desc& d) {
     if (d.B < 0 || d.Tq < 0 || d.Tk < 0 || d.H < 1 || d.G < 1 || d.H % d.G || d.type < MEP_F32 || d.type > MEP_F16) return false;
     if (d.d < 1 || d.d > MEP_DIFF_ATTN_MAX_D || d.dv < 1 || d.dv > MEP_DIFF_ATTN_MAX_DV) return false;
     if (d.Tk >= 1 << 30 || (int64_t)d.Tq * (d.H / d.G) >= 1 << 30 || (int64_t)d.B * d.G >= 1 << 30) return false;
+    return true;
+}
+bool attn_ok(const mep_diff_attn_desc& d) {
+    if (!attn_shape_ok(d)) return false;
     if (!(d.scale > 0.f && d.scale <= 1e6f) || d.mask_form < 0 || d.mask_form > 2 || (d.mask_form != 0) != (d.mask != 0)) return false;
     const bool empty = d.B == 0 || d.Tq == 0;
     return empty || (d.q && d.lam && d.out && (d.Tk == 0 || (d.k && d.v)));
@@ -118,8 +189,26 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     int blocks;
     const int64_t grid = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, blocks);
     if (grid < 0) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
-    run(DA_FWD, d, nullptr, grid, blocks, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    const Split s = split_of(d);
+    if (!s.splits || !d.workspace) {
+        run(DA_FWD, d, nullptr, grid, blocks, 1, 0, st);
+        return mep_check_launch("mep_diff_attn_fwd");
+    }
+    run(DA_SPLIT, d, nullptr, (int64_t)s.blocks * s.splits * d.B * d.G, s.blocks, s.splits, s.tiles, st);
+    int rc = mep_check_launch("mep_diff_attn_fwd");
+    if (rc) return rc;
+    int per = 32;
+    while (per < d.dv) per *= 2;
+    const int64_t rows = (int64_t)d.B * d.Tq * d.H, side = DA_THREADS / per;
+    hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, d, s.blocks, 2 * s.splits, per);
     return mep_check_launch("mep_diff_attn_fwd");
+}
+
+extern "C" int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc) {
+    if (!desc || !attn_shape_ok(*desc)) { mep_set_error("mep_diff_attn_workspace: invalid descriptor"); return MEP_EINVAL; }
+    const Split s = split_of(*desc);
+    return s.splits ? split_bytes(*desc, s) : 0;
 }
 
 extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_t stream) {
@@ -140,8 +229,8 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     const int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb),
                   kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
-    if (rows) run(DA_BWD_Q, d, &b, qg, qb, st);
-    if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, st);
+    if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, 0, st);
+    if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, 1, 0, st);
     if (b.dlam) hipLaunchKernelGGL(k_diff_dlam, dim3(d.H), dim3(DLAM_THREADS), 0, st, b);
     return mep_check_launch("mep_diff_attn_bwd");
 }

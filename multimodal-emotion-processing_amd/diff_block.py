@@ -350,6 +350,13 @@ class _DiffAttnFn(torch.autograd.Function):
                               B=B, Tq=Tq, Tk=Tk, H=H, G=G, d=hd, dv=dv, type=TYPES[q.dtype], causal=int(causal),
                               mask_form=0 if mask is None else mask.dim() - 1,
                               mask_float=int(mask is not None and mask.dtype == torch.float32), scale=scale)
+        ws = None
+        n = _lib.lib().mep_diff_attn_workspace(ctypes.byref(d))
+        if n > 0:
+            ws = torch.empty(n // 4, dtype=torch.float32, device=dev)
+            d.workspace = _ptr(ws)
+        elif n < 0:
+            _lib.check(n, 'mep_diff_attn_workspace')
         _launch('mep_diff_attn_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
