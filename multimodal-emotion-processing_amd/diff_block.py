@@ -43,8 +43,14 @@ def _type_of(t, what):
 
 def _launch(name, desc, device):
     """An entry point that takes its descriptor from the host, on the current stream of `device`."""
-    with torch.cuda.device(device):
-        _lib.call(name, ctypes.byref(desc))
+    i = device.index
+    if torch._C._cuda_getDevice() != i or _lib.TIMER is not None:
+        with torch.cuda.device(i):
+            return _lib.call(name, ctypes.byref(desc))
+    # the raw stream: this call is most of a short operator's time, and torch.cuda.current_stream() most of this call
+    rc = getattr(_lib.lib(), name)(ctypes.byref(desc), torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _ptr(t):
@@ -185,7 +191,8 @@ class _NormFn(torch.autograd.Function):
             _launch('mep_block_norm_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
-            ctx.save_for_backward(y2, x2, g2, w, b, scale, nw, nb, stats)
+            ctx.save_for_backward(y2, x2, g2, w, b, scale, nw, nb)
+            ctx.held = stats
             ctx.shapes = (y.shape, None if gate is None else gate.shape, None if scale is None else scale.shape)
             # the backward reads the forward's inputs by address, and asks of its results only which there were
             ctx.desc = d
@@ -194,7 +201,7 @@ class _NormFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dstream, dnormed=None):
-        y2, x2, g2, w, b, scale, nw, nb, stats = ctx.saved_tensors
+        y2, x2, g2, w, b, scale, nw, nb = ctx.saved_tensors
         none = (None,) * 9
         if dstream is None and dnormed is None:
             return none
@@ -360,8 +367,9 @@ class _DiffAttnFn(torch.autograd.Function):
         _launch('mep_diff_attn_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
-            # the packed copies too: the descriptor holds their addresses
-            ctx.save_for_backward(mask, lengths, q_start, q, k, v, lam, stats, second, out, qp, kp, vp)
+            ctx.save_for_backward(mask, lengths, q_start, q, k, v, lam, out)
+            # what the descriptor points to besides: the packed copies where there are any, and the row statistics
+            ctx.held = [t for t, x in ((qp, q), (kp, k), (vp, v)) if t is not x] + [stats, second]
             ctx.desc = d
         return out
 
@@ -370,7 +378,7 @@ class _DiffAttnFn(torch.autograd.Function):
     def backward(ctx, dout):
         if dout is None:
             return (None,) * 8
-        q, k, v, lam = ctx.saved_tensors[3:7]
+        q, k, v, lam = ctx.saved_tensors[3:7]      # (unpacking checks that none was written in between)
         need = ctx.needs_input_grad
         B, Tq, H, _, _ = q.shape
         dev = q.device
