@@ -73,6 +73,8 @@ struct Lay {
     static MEP_DEV int at(int r, int c) { return (r * CH + (c ^ sw(r))) * M::E; }
 };
 
+constexpr int da_piece(int width) { return width < 128 ? width : 128; }      // channels that pass through LDS at a time
+
 // Geometry of an instance: head widths padded to DK (each map) and DV
 template <int TYPE, int DK, int DV>
 struct Geo {
@@ -83,7 +85,7 @@ struct Geo {
     static constexpr int NK = DK / M::KS, NV = DV / M::KS;    // operands along the head widths
     static constexpr int NP = 32 / M::KS;                     // operands of 32 keys
     static constexpr int KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;      // elements of a tile's keys, and of a tile
-    static constexpr int OUT = DA_ROWS * ((DK > DV ? DK : DV) + M::E);  // the results pass through the tiles
+    static constexpr int OUT = DA_ROWS * (da_piece(DK > DV ? DK : DV) + M::E);  // the results pass through the tiles
     static constexpr int BUF = 2 * TSZ > OUT ? 2 * TSZ : OUT;
 };
 
@@ -100,6 +102,36 @@ template <class M>
 MEP_DEV typename M::Frag row_frag(const MEP_G typename M::T* row, int c, int n, bool live) {
     return live && c < n ? *reinterpret_cast<const MEP_G typename M::Frag*>(row + c) : zero_frag<M>();
 }
+
+// The N operands of a lane's row (n elements from p on): held in registers, or (wide fp32 heads, whose products take 16 times as long
+// and whose operands and accumulators would not fit) read again from the cache at each use.  A row that is not there: zeros.
+constexpr bool da_hold(int type, int dk) { return !(type == MEP_F32 && dk >= 64); }
+template <class M, int N, bool HOLD>
+struct Operand {
+    typedef typename M::Frag Frag;
+    Frag f[HOLD ? N : 1];
+    const MEP_G typename M::T* p;
+    int n;
+    bool live;
+    MEP_DEV Operand(const MEP_G typename M::T* row, int width, bool there) : p(row), n(width), live(there) {
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = row_frag<M>(p, M::KS * i + M::E * ((threadIdx.x & 63) >> 5), n, live);
+        }
+    }
+    MEP_DEV Frag at(int i) const {
+        if constexpr (HOLD) {
+            return f[i];
+        } else {      // the load of a valid place without a branch, then the choice
+            const int c = M::KS * i + M::E * ((threadIdx.x & 63) >> 5), last = (n - 1) / M::E * M::E;
+            Frag x = *reinterpret_cast<const MEP_G Frag*>(p + min(c, last));
+            const bool on = live && c < n;
+#pragma unroll
+            for (int e = 0; e < M::E; ++e) x[e] = on ? x[e] : (typename M::T)0.f;
+            return x;
+        }
+    }
+};
 
 typedef __attribute__((address_space(3))) char da_lds_char;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -182,13 +214,13 @@ MEP_DEV void tile_sync() {
 
 // A lane's places in a tile.  a[j]: first-product operand, chunk 2 j + h of row lane & 31 (j = 0 .. 3 of a group of 8 chunks); the
 // other rows and groups are constants away.  t[n]: second-product operand, in the rows of accumulator order and columns
-// 32 n + (lane & 31), n = 0, 1; likewise.
+// 32 n + (lane & 31), n = 0, 1; likewise (fp32: t[j], of row j of 4, any n).
 template <class M, int COLS>
 struct Reader {
     typedef Lay<M, COLS> L;
     typedef typename M::T T;
     typedef typename M::Frag Frag;
-    static constexpr int NA = L::CH >= 8 ? 4 : 2, NT = L::CH >= 8 && M::KS == 16 ? 2 : 1;
+    static constexpr int NA = L::CH >= 8 ? 4 : 2, NT = M::KS == 8 ? 4 : L::CH >= 8 ? 2 : 1;
     int a[NA], t[NT];                // elements
     MEP_DEV Reader() {
         const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -198,8 +230,9 @@ struct Reader {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 t[n] = L::at(4 * h + ((lane & 15) >> 2), (32 * n + (lane & 16)) / M::E + ((lane & 3) >> 1)) + 4 * (lane & 1);
-        } else {
-            t[0] = 0;
+        } else {                         // row j of every 4
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = L::at(4 * h + j, (lane & 31) >> 2) + (lane & 3);
         }
     }
     // operand i (of all COLS) of the rows from r0 on
@@ -210,9 +243,8 @@ struct Reader {
     MEP_DEV Frag cols(const T* tile, int r0, int col0, int i) const {
         if constexpr (M::KS == 8) {
             Frag f;
-            const int lane = threadIdx.x & 63, col = col0 + (lane & 31);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = tile[L::at(r0 + 8 * i + 4 * (lane >> 5) + j, col / M::E) + col % M::E];
+            for (int j = 0; j < 4; ++j) f[j] = tile[t[j] + (r0 + 8 * i) * L::CH * M::E + col0];
             return f;
         } else {
             typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -394,38 +426,40 @@ struct Rows32 {
 };
 
 // A wave's accumulators (32 rows or keys x 32 N channels, transposed) times f, rounded, to rows of global memory: through LDS
-// (a wave's own 32 x (32 N + E) elements), so that a row's channels are written together.  row_at(r): the row's first element, or null.
+// (a wave's own 32 rows of up to 128 channels), so that a row's channels are written together.  row_at(r): the row's first element, or
+// null; whole: rows begin and end on 16 bytes.
 template <class M, int N, class F>
-MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, int n, F row_at) {
+MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, int n, bool whole, F row_at) {
     typedef typename M::T T;
-    constexpr int LD = 32 * N + M::E;
+    constexpr int P = N < 4 ? N : 4, LD = 32 * P + M::E, CH = 32 * P / M::E;
     const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int piece = 0; piece < N; piece += P) {
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            typename VecOf<T, 4>::type v;
+        for (int i = 0; i < P; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][r + e] * f);
-            *reinterpret_cast<typename VecOf<T, 4>::type*>(buf + (lane & 31) * LD + 32 * i + acc_off(r) + 4 * h) = v;
-        }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // this wave's own writes
-    constexpr int CH = 32 * N / M::E;
-    const bool whole = n % M::E == 0;
+            for (int r = 0; r < 16; r += 4) {
+                typename VecOf<T, 4>::type v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[piece + i][r + e] * f);
+                *reinterpret_cast<typename VecOf<T, 4>::type*>(buf + (lane & 31) * LD + 32 * i + acc_off(r) + 4 * h) = v;
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // this wave's own writes
 #pragma unroll 1
-    for (int i = lane; i < 32 * CH; i += 64) {
-        const int r = i / CH, col = i % CH * M::E;
-        MEP_G T* p = row_at(r);
-        if (!p || col >= n) continue;
-        const typename M::Frag v = *reinterpret_cast<const typename M::Frag*>(buf + r * LD + col);
-        if (whole) {
-            *reinterpret_cast<MEP_G typename M::Frag*>(p + col) = v;
-        } else {
+        for (int i = lane; i < 32 * CH; i += 64) {
+            const int r = i / CH, col = i % CH * M::E, to = 32 * piece + col;
+            MEP_G T* p = row_at(r);
+            if (!p || to >= n) continue;
+            const typename M::Frag v = *reinterpret_cast<const typename M::Frag*>(buf + r * LD + col);
+            if (whole) {
+                *reinterpret_cast<MEP_G typename M::Frag*>(p + to) = v;
+            } else {
 #pragma unroll
-            for (int e = 0; e < M::E; ++e) if (col + e < n) p[col + e] = v[e];
+                for (int e = 0; e < M::E; ++e) if (to + e < n) p[to + e] = v[e];
+            }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next one is written
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next one is written
 }
 
 // ------------------------------------------------------------------ forward
@@ -447,17 +481,13 @@ struct Online {
     typedef typename Ge::Frag Frag;
     // The backward's e_m are to be at most 1: it gets maxima 8 up, or in float16, whose subnormals begin at 2^-14, the true ones
     static constexpr bool TOP = TYPE == MEP_F16;
-    Frag q[2][Ge::NK];
+    typedef Operand<M, Ge::NK, da_hold(TYPE, DK)> Q;
+    Q q1, q2;
     float c, lam, m1, m2, l1, l2, f1, f2, top1, top2;
     floatx16 x[DV / 32], y[DV / 32];
 
-    MEP_DEV Online(const mep_diff_attn_desc& d, const Job& j, const Rows32& w) {
-        const int h = (threadIdx.x & 63) >> 5;
-        const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < Ge::NK; ++i) q[m][i] = row_frag<M>(qp + m * d.q_sM, M::KS * i + M::E * h, d.d, w.live);
+    MEP_DEV Online(const mep_diff_attn_desc& d, const Job& j, const Rows32& w)
+        : q1(G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH, d.d, w.live), q2(q1.p + d.q_sM, d.d, w.live) {
         lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
         c = d.scale * DA_LOG2E;
         m1 = m2 = mul_rn(DA_MIN, c);
@@ -473,8 +503,8 @@ struct Online {
         floatx16 s1 = zero16(), s2 = zero16();
 #pragma unroll
         for (int i = 0; i < Ge::NK; ++i) {
-            s1 = M::mma(kread.rows(kt, r0, i), q[0][i], s1);
-            s2 = M::mma(kread.rows(kt, r0, Ge::NK + i), q[1][i], s2);
+            s1 = M::mma(kread.rows(kt, r0, i), q1.at(i), s1);
+            s2 = M::mma(kread.rows(kt, r0, Ge::NK + i), q2.at(i), s2);
         }
         if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
         const float a1 = max16(s1), a2 = max16(s2);
@@ -538,8 +568,9 @@ struct Online {
     }
 };
 
+// ld: channels between out's rows (values wider than 128 channels are taken by two launches)
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks) {
+__global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int ld) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
@@ -583,20 +614,21 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
         *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) = f32x4{n1, i1 / g1, n2, i2 / g2};
     const float fx = i1 / o.f1, fy = fx * o.f2 - o.lam * i2;
     tile_sync();                             // the tiles are free
-    const int64_t first = (int64_t)j.b * d.Tq * d.H * d.dv;
+    const int64_t first = (int64_t)j.b * d.Tq * d.H * ld;
     auto row_at = [&](uint64_t p, int r) -> MEP_G T* {
         const int row = w.row0 + r;
         if (row >= j.rows) return nullptr;
         const int t = row / j.n;
-        return G<T>(p) + first + ((int64_t)t * d.H + j.g * j.n + row - t * j.n) * d.dv;
+        return G<T>(p) + first + ((int64_t)t * d.H + j.g * j.n + row - t * j.n) * ld;
     };
-    T* mine = Buf + (threadIdx.x >> 6) * 32 * (DV + M::E);
+    const bool whole = ld % M::E == 0;
+    T* mine = Buf + (threadIdx.x >> 6) * 32 * (da_piece(DV) + M::E);
 #pragma unroll
     for (int n = 0; n < DV / 32; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o.x[n][r] = fmaf(o.x[n][r], fx, o.y[n][r] * fy);
-    write_rows<M>(mine, o.x, 1.f, d.dv, [&](int r) { return row_at(d.out, r); });
-    if (d.second) write_rows<M>(mine, o.y, i2, d.dv, [&](int r) { return row_at(d.second, r); });
+    write_rows<M>(mine, o.x, 1.f, d.dv, whole, [&](int r) { return row_at(d.out, r); });
+    if (d.second) write_rows<M>(mine, o.y, i2, d.dv, whole, [&](int r) { return row_at(d.second, r); });
 }
 
 // ------------------------------------------------------------------ forward over split keys
@@ -608,7 +640,7 @@ __global__ __launch_bounds__(DA_THREADS, DV >= 256 || DK >= 128 ? 1 : 2) void k_
 MEP_DEV int64_t split_floats(int dv) { return 32 * (4 + 2 * (int64_t)dv); }
 
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(128, DV >= 128 || DK >= 128 ? 1 : 2) void k_diff_split(mep_diff_attn_desc d, int blocks, int splits, int tiles) {
+__global__ __launch_bounds__(128, DV >= 128 || DK >= 128 || TYPE == MEP_F32 ? 1 : 2) void k_diff_split(mep_diff_attn_desc d, int blocks, int splits, int tiles) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
@@ -693,7 +725,7 @@ __global__ __launch_bounds__(128, DV >= 128 || DK >= 128 ? 1 : 2) void k_diff_sp
 // over the keys forms it where a row of the workgroup rests on fewer than 32 keys (sum A_m^2 > 1 / 32; at that it is a thirtieth of
 // dS's rounding).  (In fp32 the estimate is as good as the sum.)  The sums are also lam's gradient and what dk needs.
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
+__global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
@@ -714,36 +746,32 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
     unsigned long long bits = key_bits(d, j, 0, KT, raw);
     if (end > 0) keys.load(Buf, 0, bits);
     raw = key_raw(d, j, KT);
-    Frag q[2][Ge::NK], g[Ge::NV];
+    constexpr bool HOLD = da_hold(TYPE, DK);
+    const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
+    const Operand<M, Ge::NK, HOLD> q1(qp, d.d, w.live), q2(qp + d.q_sM, d.d, w.live);
+    const Operand<M, Ge::NV, HOLD> g(G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)w.t * bd.o_sT + (int64_t)w.head * bd.o_sH, d.dv, w.live);
     float d1 = 0.f, d2 = 0.f;              // the estimates
     {
-        const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
-        const MEP_G T* gp = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)w.t * bd.o_sT + (int64_t)w.head * bd.o_sH;
         const int64_t at = (((int64_t)j.b * d.Tq + w.t) * d.H + w.head) * d.dv;
         const MEP_G T* o = G<const T>(d.out) + at;
         const MEP_G T* o2 = G<const T>(d.second) + at;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < Ge::NK; ++i)
-                q[m][i] = row_frag<M>(qp + m * d.q_sM, M::KS * i + M::E * h, d.d, w.live);
-#pragma unroll
         for (int i = 0; i < Ge::NV; ++i) {
             const int col = M::KS * i + M::E * h;
-            g[i] = row_frag<M>(gp, col, d.dv, w.live);
+            const Frag gi = g.at(i);
             if (d.dv % M::E == 0) {
                 const Frag a = row_frag<M>(o, col, d.dv, true), b = row_frag<M>(o2, col, d.dv, true);
 #pragma unroll
                 for (int e = 0; e < M::E; ++e) {
-                    d1 = fmaf((float)g[i][e], (float)a[e], d1);
-                    d2 = fmaf((float)g[i][e], (float)b[e], d2);
+                    d1 = fmaf((float)gi[e], (float)a[e], d1);
+                    d2 = fmaf((float)gi[e], (float)b[e], d2);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < M::E; ++e)
                     if (col + e < d.dv) {
-                        d1 = fmaf((float)g[i][e], (float)o[col + e], d1);
-                        d2 = fmaf((float)g[i][e], (float)o2[col + e], d2);
+                        d1 = fmaf((float)gi[e], (float)o[col + e], d1);
+                        d2 = fmaf((float)gi[e], (float)o2[col + e], d2);
                     }
             }
         }
@@ -779,11 +807,11 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
             floatx16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
             for (int i = 0; i < Ge::NK; ++i) {
-                s1 = M::mma(kread.rows(kt, 32 * sub, i), q[0][i], s1);
-                s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q[1][i], s2);
+                s1 = M::mma(kread.rows(kt, 32 * sub, i), q1.at(i), s1);
+                s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q2.at(i), s2);
             }
 #pragma unroll
-            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g[i], dp);
+            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g.at(i), dp);
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {      // e_m, the row sums, and dS_m without the row's factors 1 / l1, -lam / l2
@@ -857,8 +885,8 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
                     floatx16 s1 = zero16(), s2 = zero16();
 #pragma unroll
                     for (int i = 0; i < Ge::NK; ++i) {
-                        s1 = M::mma(kread.rows(Buf, 32 * sub, i), q[0][i], s1);
-                        s2 = M::mma(kread.rows(Buf, 32 * sub, Ge::NK + i), q[1][i], s2);
+                        s1 = M::mma(kread.rows(Buf, 32 * sub, i), q1.at(i), s1);
+                        s2 = M::mma(kread.rows(Buf, 32 * sub, Ge::NK + i), q2.at(i), s2);
                     }
                     if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
 #pragma unroll
@@ -901,9 +929,10 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
         const int t = row / j.n;
         return G<T>(bd.dq) + first + (((int64_t)t * d.H + j.g * j.n + row - t * j.n) * 2 + m) * d.d;
     };
-    T* mine = Buf + (threadIdx.x >> 6) * 32 * (DK + M::E);
-    write_rows<M>(mine, a1, st[1] * d.scale, d.d, [&](int r) { return row_at(0, r); });
-    write_rows<M>(mine, a2, -lam * st[3] * d.scale, d.d, [&](int r) { return row_at(1, r); });
+    const bool whole = d.d % M::E == 0;
+    T* mine = Buf + (threadIdx.x >> 6) * 32 * (da_piece(DK) + M::E);
+    write_rows<M>(mine, a1, st[1] * d.scale, d.d, whole, [&](int r) { return row_at(0, r); });
+    write_rows<M>(mine, a2, -lam * st[3] * d.scale, d.d, whole, [&](int r) { return row_at(1, r); });
 }
 
 // ------------------------------------------------------------------ backward: dk and dv
@@ -916,16 +945,18 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (TYPE == MEP_F32 && DK >= 
 // at X 1 with X the row's value in three bf16 parts (24 bits) against a column of ones, one instruction for 16 registers.  With
 //   s' = s - lse_m / c, lse_1 = m_1 + log2 l_1, lse_2 = m_2 + log2 l_2 - log2 |lam|:   2^(c s') = A_1, |lam| A_2
 //   dP' = dP - D_1, and D_1 - D_2 added for the second map
-// the rest is a product and an exponential each.  (lse_m folds a sum into the maximum: its last bits are below those that s has.)
+// the rest is a product and an exponential each.  (lse_m folds a sum into the maximum, which costs last bits where the maximum is
+// large: of no account in 16 bits.  In fp32, whose products take 16 times as long, the row's values are read from LDS.)
 template <int KW, int TYPE, int DK, int DV>
 struct KvShape {
     typedef Geo<TYPE, DK, DV> Ge;
     static constexpr int ROLES = DK == 32 ? 1 : 2, THREADS = 64 * KW * ROLES, KEYS = 32 * KW;
-    static constexpr int OUT = KEYS * (DK + DV + 2 * Ge::M::E), BUF = 2 * Ge::TSZ > OUT ? 2 * Ge::TSZ : OUT;
+    static constexpr int OUT = KEYS * (da_piece(DK) + da_piece(DV) + 2 * Ge::M::E), BUF = 2 * Ge::TSZ > OUT ? 2 * Ge::TSZ : OUT;
 };
 
 typedef __bf16 bf16x8_da __attribute__((ext_vector_type(8)));
 enum { X_LSE1, X_LSE2, X_D1, X_D12, X_SIGN, X_COUNT };
+enum { R_M1, R_I1, R_M2, R_LI2, R_D1, R_D2, R_COUNT };
 
 // -v, in three parts that sum to it to 24 bits, as the k = 0, 1, 2 of an operand
 MEP_DEV bf16x8_da parts3(float v) {
@@ -959,7 +990,9 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
     constexpr int RT = Ge::KT, THREADS = Sh::THREADS, ROLES = Sh::ROLES;
     const mep_diff_attn_desc& d = bd.f;
     __shared__ __align__(16) T Buf[Sh::BUF];      // two tiles: their queries, then their upstream gradients
-    __shared__ bf16x8_da Xs[2][X_COUNT][RT];      // and their rows' values
+    constexpr bool PARTS = TYPE != MEP_F32;       // the rows' values: as products, or in fp32 as they are
+    __shared__ bf16x8_da Xs[2][PARTS ? (int)X_COUNT : 1][PARTS ? RT : 1];
+    __shared__ __align__(16) float Rs[2][PARTS ? 1 : (int)R_COUNT][PARTS ? 1 : RT];
     __shared__ int Ts[2][RT];                     // and queries
     __shared__ int Neg[2];                        // whether any lam of the tile is negative
     const Job j = make_job(d, blocks, false);
@@ -1023,7 +1056,14 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
         if (threadIdx.x < 64) {
             const bool neg = __ballot(threadIdx.x < RT && lv < 0.f) != 0;
             const int i = threadIdx.x;
-            if (i < RT) {
+            if constexpr (!PARTS) {
+                if (i < RT) {
+                    const float v[R_COUNT] = {sv[0], sv[1], sv[2], lv * sv[3], dv4[0], dv4[1]};
+#pragma unroll
+                    for (int x = 0; x < R_COUNT; ++x) Rs[buf][x][i] = v[x];
+                    Ts[buf][i] = tv;
+                }
+            } else if (i < RT) {
                 // without keys, past the end (1 / l = 0) and for lam = 0: A = 0
                 const float al = fabsf(lv) * sv[3];
                 Xs[buf][X_LSE1][i] = parts3(sv[1] > 0.f || sv[1] != sv[1] ? (sv[0] - __log2f(sv[1])) / c : -DA_MIN);
@@ -1046,24 +1086,24 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
     const int64_t krow = on ? key : 0;
     const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH + krow * d.k_sT;
     const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH + krow * d.v_sT;
-    Frag kr[2][Ge::NK];
-#pragma unroll
-    for (int i = 0; i < Ge::NK; ++i) {
-        kr[0][i] = row_frag<M>(kp, M::KS * i + M::E * h, d.d, on);
-        kr[1][i] = row_frag<M>(kp + d.k_sM, M::KS * i + M::E * h, d.d, on);
-    }
+    constexpr bool HOLD = da_hold(TYPE, DK);
+    const Operand<M, Ge::NK, HOLD> k1(kp, d.d, on), k2(kp + d.k_sM, d.d, on);
     const bool wave_on = __ballot(on) != 0, all_on = __ballot(on) == ~0ull;
     if (rbeg < rend) put_stats(0);
 
     // A_1 and lam A_2 of the rows from rs on
     auto maps = [&](int buf, int sub, int rs, floatx16& s1, floatx16& s2) {
         const T* qt = Buf + buf * Ge::TSZ;
-        s1 = row_values(Xs[buf][X_LSE1] + 32 * sub);
-        s2 = row_values(Xs[buf][X_LSE2] + 32 * sub);
+        if constexpr (PARTS) {
+            s1 = row_values(Xs[buf][X_LSE1] + 32 * sub);
+            s2 = row_values(Xs[buf][X_LSE2] + 32 * sub);
+        } else {
+            s1 = s2 = zero16();
+        }
 #pragma unroll
         for (int i = 0; i < Ge::NK; ++i) {
-            s1 = M::mma(qread.rows(qt, 32 * sub, i), kr[0][i], s1);
-            s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), kr[1][i], s2);
+            s1 = M::mma(qread.rows(qt, 32 * sub, i), k1.at(i), s1);
+            s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), k2.at(i), s2);
         }
         if (!all_on || rs < wfull || d.mask_form == 2) {      // rows that see this lane's key: those from rmin on
             const int least = rmin - rs - 4 * h;
@@ -1082,15 +1122,24 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
                 s2[r] = ok >> acc_off(r) & 1 ? s2[r] : -INFINITY;
             }
         }
+        if constexpr (PARTS) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s1[r] = exp2_fast(s1[r] * c);
-            s2[r] = exp2_fast(s2[r] * c);
-        }
-        if (Neg[buf]) {
-            const floatx16 sg = row_values(Xs[buf][X_SIGN] + 32 * sub);
+            for (int r = 0; r < 16; ++r) {
+                s1[r] = exp2_fast(s1[r] * c);
+                s2[r] = exp2_fast(s2[r] * c);
+            }
+            if (Neg[buf]) {
+                const floatx16 sg = row_values(Xs[buf][X_SIGN] + 32 * sub);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s2[r] *= sg[r];
+                for (int r = 0; r < 16; ++r) s2[r] *= sg[r];
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int lr = 32 * sub + acc_off(r) + 4 * h;
+                s1[r] = exp2_fast(fmaf(s1[r], c, -Rs[buf][R_M1][lr])) * Rs[buf][R_I1][lr];
+                s2[r] = exp2_fast(fmaf(s2[r], c, -Rs[buf][R_M2][lr])) * Rs[buf][R_LI2][lr];
+            }
         }
     };
     auto walk = [&](auto step) {
@@ -1134,20 +1183,27 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
         }
     };
     // dk_m += dS_m^T q_m; s1, s2: the maps
-    Frag vr[Ge::NV];
-    auto load_v = [&] {
+    typedef Operand<M, Ge::NV, HOLD> V;
+    auto add_k = [&](const V& v, const T* qt, int buf, int sub, floatx16& s1, floatx16& s2) {
+        floatx16 dp;
+        if constexpr (PARTS) dp = row_values(Xs[buf][X_D1] + 32 * sub);
+        else dp = zero16();
 #pragma unroll
-        for (int i = 0; i < Ge::NV; ++i) vr[i] = row_frag<M>(vp, M::KS * i + M::E * h, d.dv, on);
-    };
-    auto add_k = [&](const T* qt, int buf, int sub, floatx16& s1, floatx16& s2) {
-        floatx16 dp = row_values(Xs[buf][X_D1] + 32 * sub);
+        for (int i = 0; i < Ge::NV; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), v.at(i), dp);
+        if constexpr (PARTS) {
 #pragma unroll
-        for (int i = 0; i < Ge::NV; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), vr[i], dp);
+            for (int r = 0; r < 16; ++r) s1[r] *= dp[r];
+            const floatx16 d12 = row_values(Xs[buf][X_D12] + 32 * sub);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s1[r] *= dp[r];
-        const floatx16 d12 = row_values(Xs[buf][X_D12] + 32 * sub);
+            for (int r = 0; r < 16; ++r) s2[r] *= dp[r] + d12[r];
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s2[r] *= dp[r] + d12[r];
+            for (int r = 0; r < 16; ++r) {
+                const int lr = 32 * sub + acc_off(r) + 4 * h;
+                s1[r] *= dp[r] - Rs[buf][R_D1][lr];
+                s2[r] *= dp[r] - Rs[buf][R_D2][lr];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < Ge::NP; ++i) {
             const Frag f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
@@ -1158,17 +1214,17 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
             }
         }
     };
-    auto put_v = [&](T* mine) { write_rows<M>(mine, av, 1.f, d.dv, [&](int r) { return key_at(bd.dv, r, d.dv); }); };
+    auto put_v = [&](T* mine) { write_rows<M>(mine, av, 1.f, d.dv, d.dv % M::E == 0, [&](int r) { return key_at(bd.dv, r, d.dv); }); };
     auto put_k = [&](T* mine) {
-        write_rows<M>(mine, a1, d.scale, d.d, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
-        write_rows<M>(mine, a2, -d.scale, d.d, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
+        write_rows<M>(mine, a1, d.scale, d.d, d.d % M::E == 0, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
+        write_rows<M>(mine, a2, -d.scale, d.d, d.d % M::E == 0, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
     };
-    T* vbuf = Buf + wave % KW * 32 * (DV + M::E);
-    T* kbuf = Buf + KW * 32 * (DV + M::E) + wave % KW * 32 * (DK + M::E);
+    T* vbuf = Buf + wave % KW * 32 * (da_piece(DV) + M::E);
+    T* kbuf = Buf + KW * 32 * (da_piece(DV) + M::E) + wave % KW * 32 * (da_piece(DK) + M::E);
     if constexpr (ROLES == 1) {
         clear_v();
         clear_k();
-        load_v();
+        const V v(vp, d.dv, on);
         walk([&](int buf, int sub, int rs) {
             const T* qt = Buf + buf * Ge::TSZ;
             floatx16 s1, s2, p;
@@ -1176,7 +1232,7 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] = s1[r] - s2[r];
             add_v(qt + Ge::KSZ, sub, p);
-            add_k(qt, buf, sub, s1, s2);
+            add_k(v, qt, buf, sub, s1, s2);
         });
         put_v(vbuf);
         put_k(kbuf);
@@ -1192,11 +1248,11 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
         put_v(vbuf);
     } else {
         clear_k();
-        load_v();
+        const V v(vp, d.dv, on);
         walk([&](int buf, int sub, int rs) {
             floatx16 s1, s2;
             maps(buf, sub, rs, s1, s2);
-            add_k(Buf + buf * Ge::TSZ, buf, sub, s1, s2);
+            add_k(v, Buf + buf * Ge::TSZ, buf, sub, s1, s2);
         });
         put_k(kbuf);
     }
@@ -1204,12 +1260,12 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
 
 // ------------------------------------------------------------------ instances
 // key groups of a k_diff_bwd_kv workgroup: 4 (two waves on a SIMD) where a wave's operands and accumulators fit 256 registers
-constexpr int da_kw(int type, int dk) { return dk >= 128 || (type == MEP_F32 && dk >= 64) ? 2 : 4; }
+constexpr int da_kw(int type, int dk) { return dk >= 128 && type != MEP_F32 ? 2 : 4; }
 
 template <int TYPE, int DK, int DV>
-void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {
-    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks);
-    else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, DV>), dim3(grid), dim3(128), 0, st, d, blocks, splits, tiles);
+void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {      // (tiles: DA_FWD's ld)
+    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, tiles);
+    else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(128), 0, st, d, blocks, splits, tiles);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
                             dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks);
@@ -1223,8 +1279,8 @@ inline int da_value_width(int d, int dv) {
     return dk == 32 ? (dv <= 32 ? 32 : 64) : dk == 64 ? (dv <= 64 ? 64 : 128) : (dv <= 128 ? 128 : 256);
 }
 template <int TYPE>
-void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {
-    const int dk = da_width(d.d, d.dv), dv = da_value_width(d.d, d.dv);
+void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all) {
+    const int dk = da_width(d.d, all), dv = da_value_width(d.d, all);      // all: the values' whole width
     if (dk == 32 && dv == 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, splits, tiles, st);
     else if (dk == 32) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, splits, tiles, st);
     else if (dk == 64 && dv == 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, splits, tiles, st);
@@ -1233,8 +1289,8 @@ void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc*
     else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, splits, tiles, st);
 }
 
-void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st);
-void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st);
-void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st);
+void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all);
+void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all);
+void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all);
 
 }  // namespace mep

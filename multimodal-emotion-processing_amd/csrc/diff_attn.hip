@@ -35,7 +35,7 @@ __global__ __launch_bounds__(DLAM_THREADS) void k_diff_dlam(mep_diff_attn_bwd_de
 }
 
 // out = E_1 / l_1 - lam E_2 / l_2 of a row from its parts, a thread per value channel; rows side by side in a workgroup
-__global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, int blocks, int parts, int per) {
+__global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, int blocks, int parts, int per, int ld) {
     const int ch = threadIdx.x % per;
     const int64_t r = (int64_t)blockIdx.x * (DA_THREADS / per) + threadIdx.x / per;      // (b, t, head)
     if (r >= (int64_t)d.B * d.Tq * d.H) return;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, 
     if (d.stats && ch == 0) *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)b * d.H + head) * d.Tq + t)) = f32x4{m1, i1, m2, i2};
     if (ch >= d.dv) return;
     auto put = [&](uint64_t p, float v) {
-        const int64_t o = r * d.dv + ch;
+        const int64_t o = r * ld + ch;
         if (d.type == MEP_F32) G<float>(p)[o] = v;
         else if (d.type == MEP_BF16) G<__bf16>(p)[o] = (__bf16)v;
         else G<_Float16>(p)[o] = (_Float16)v;
@@ -108,7 +108,7 @@ Split split_of(const mep_diff_attn_desc& d) {
     const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) < 128;
     if (pairs == 0 || rows == 0 || !(few || none)) return s;
     s.blocks = (int)((rows + 31) / 32);
-    const int kt = da_split_keys(d.type, da_width(d.d, d.dv), da_value_width(d.d, d.dv)), all = (d.Tk + kt - 1) / kt;
+    const int kt = da_split_keys(d.type, da_width(d.d, d.dv), da_piece(da_value_width(d.d, d.dv))), all = (d.Tk + kt - 1) / kt;
     const int64_t want = 2048 / (pairs * s.blocks);
     s.splits = (int)(want < 1 ? 1 : want > (all + 3) / 4 ? (all + 3) / 4 : want);
     s.tiles = (all + s.splits - 1) / s.splits;
@@ -120,10 +120,10 @@ int64_t split_bytes(const mep_diff_attn_desc& d, const Split& s) {
     return (int64_t)d.B * d.G * s.blocks * s.splits * 2 * 32 * (4 + 2 * (int64_t)d.dv) * 4;
 }
 
-void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, int tiles, hipStream_t st) {
-    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, tiles, st);
-    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, tiles, st);
-    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, tiles, st);
+void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, int tiles, hipStream_t st, int dv) {
+    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
+    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
+    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
 }
 
 bool attn_shape_ok(const mep_diff_attn_desc& d) {
@@ -191,18 +191,28 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     if (grid < 0) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
     hipStream_t st = (hipStream_t)stream;
     const Split s = split_of(d);
-    if (!s.splits || !d.workspace) {
-        run(DA_FWD, d, nullptr, grid, blocks, 1, 0, st);
-        return mep_check_launch("mep_diff_attn_fwd");
+    // values of more than 128 channels in two launches: their accumulators would not fit beside each other
+    const int es = d.type == MEP_F32 ? 4 : 2, half = da_piece(d.dv);
+    for (int c = 0; c < d.dv; c += half) {
+        mep_diff_attn_desc p = d;
+        p.dv = d.dv - c < half ? d.dv - c : half;
+        p.v += (uint64_t)c * es;
+        p.out += (uint64_t)c * es;
+        if (p.second) p.second += (uint64_t)c * es;
+        if (c) p.stats = 0;
+        if (!s.splits || !d.workspace) {
+            run(DA_FWD, p, nullptr, grid, blocks, 1, d.dv, st, d.dv);
+        } else {
+            run(DA_SPLIT, p, nullptr, (int64_t)s.blocks * s.splits * d.B * d.G, s.blocks, s.splits, s.tiles, st, d.dv);
+            int per = 32;
+            while (per < p.dv) per *= 2;
+            const int64_t rows = (int64_t)d.B * d.Tq * d.H, side = DA_THREADS / per;
+            hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, p, s.blocks, 2 * s.splits, per, d.dv);
+        }
+        const int rc = mep_check_launch("mep_diff_attn_fwd");
+        if (rc) return rc;
     }
-    run(DA_SPLIT, d, nullptr, (int64_t)s.blocks * s.splits * d.B * d.G, s.blocks, s.splits, s.tiles, st);
-    int rc = mep_check_launch("mep_diff_attn_fwd");
-    if (rc) return rc;
-    int per = 32;
-    while (per < d.dv) per *= 2;
-    const int64_t rows = (int64_t)d.B * d.Tq * d.H, side = DA_THREADS / per;
-    hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, d, s.blocks, 2 * s.splits, per);
-    return mep_check_launch("mep_diff_attn_fwd");
+    return 0;
 }
 
 extern "C" int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc) {
@@ -229,8 +239,8 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     const int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb),
                   kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
-    if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, 0, st);
-    if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, 1, 0, st);
+    if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, 0, st, d.dv);
+    if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, 1, 0, st, d.dv);
     if (b.dlam) hipLaunchKernelGGL(k_diff_dlam, dim3(d.H), dim3(DLAM_THREADS), 0, st, b);
     return mep_check_launch("mep_diff_attn_bwd");
 }
