@@ -298,7 +298,7 @@ class DiffAttnDesc(ctypes.Structure):
 
 class DiffAttnBwdDesc(ctypes.Structure):
     _fields_ = [('f', DiffAttnDesc), ('dout', u64), ('o_sB', i64), ('o_sT', i64), ('o_sH', i64), ('dq', u64), ('dk', u64),
-                ('dv', u64), ('dlam', u64), ('dlam_rows', u64), ('delta', u64)]
+                ('dv', u64), ('dlam', u64), ('dlam_rows', u64), ('delta', u64), ('workspace', u64)]
 
 
 class PackRowsDesc(ctypes.Structure):
@@ -352,6 +352,7 @@ SIGNATURES.update({
     'mep_diff_attn_fwd': [ctypes.POINTER(DiffAttnDesc), P],
     'mep_diff_attn_bwd': [ctypes.POINTER(DiffAttnBwdDesc), P],
     'mep_diff_attn_workspace': [ctypes.POINTER(DiffAttnDesc)],
+    'mep_diff_attn_bwd_workspace': [ctypes.POINTER(DiffAttnDesc)],
     'mep_pack_rows': [ctypes.POINTER(PackRowsDesc), P],
     'mep_rotary': [ctypes.POINTER(RotaryDesc), P],
     'mep_block_norm_fwd': [ctypes.POINTER(BlockNormDesc), P],
@@ -372,7 +373,7 @@ SIGNATURES.update({
     'mep_stamp_khz': [],
 })
 
-RESTYPES = {'mep_diff_attn_workspace': i64}   # the others return int
+RESTYPES = {'mep_diff_attn_workspace': i64, 'mep_diff_attn_bwd_workspace': i64}   # the others return int
 
 _LIB = None
 ABI_VERSION = 7   # include/mep.h MEP_ABI_VERSION

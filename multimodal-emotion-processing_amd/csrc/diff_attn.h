@@ -936,8 +936,8 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
 }
 
 // ------------------------------------------------------------------ backward: dk and dv
-// A workgroup walks the rows of 32 KW keys, a wave (an accumulator column per key) those of 32.  At DK = 32 a wave forms dv and dk
-// (ROLES = 1).  With wider heads the workgroup has 2 KW waves, one half for dv and the other for dk (ROLES = 2): both form
+// A workgroup walks the rows of 32 KW keys, a wave (an accumulator column per key) those of 32.  At DK = 32 (fp32: 64, its
+// operands are not held) a wave forms dv and dk (ROLES = 1).  With wider heads the workgroup has 2 KW waves, one half for dv and the other for dk (ROLES = 2): both form
 // the scores, but so neither holds more than 256 registers and two waves share a SIMD (in one wave, the accumulators of
 // both pass through the accumulation registers and back for every tile: 335 us against 268 at B 2, T 4096, 8 heads, 64 / 128, causal).
 //
@@ -947,10 +947,11 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
 //   dP' = dP - D_1, and D_1 - D_2 added for the second map
 // the rest is a product and an exponential each.  (lse_m folds a sum into the maximum, which costs last bits where the maximum is
 // large: of no account in 16 bits.  In fp32, whose products take 16 times as long, the row's values are read from LDS.)
+constexpr int da_roles(int type, int dk) { return dk == 32 || (type == MEP_F32 && dk == 64) ? 1 : 2; }
 template <int KW, int TYPE, int DK, int DV>
 struct KvShape {
     typedef Geo<TYPE, DK, DV> Ge;
-    static constexpr int ROLES = DK == 32 ? 1 : 2, THREADS = 64 * KW * ROLES, KEYS = 32 * KW;
+    static constexpr int ROLES = da_roles(TYPE, DK), THREADS = 64 * KW * ROLES, KEYS = 32 * KW;
     static constexpr int OUT = KEYS * (da_piece(DK) + da_piece(DV) + 2 * Ge::M::E), BUF = 2 * Ge::TSZ > OUT ? 2 * Ge::TSZ : OUT;
 };
 
@@ -981,7 +982,7 @@ MEP_DEV floatx16 row_values(const bf16x8_da* x) {
 }
 
 template <int KW, int TYPE, int DK, int DV>
-__global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks) {
+__global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks, int splits) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef KvShape<KW, TYPE, DK, DV> Sh;
     typedef typename Ge::M M;
@@ -995,7 +996,9 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
     __shared__ __align__(16) float Rs[2][PARTS ? 1 : (int)R_COUNT][PARTS ? 1 : RT];
     __shared__ int Ts[2][RT];                     // and queries
     __shared__ int Neg[2];                        // whether any lam of the tile is negative
-    const Job j = make_job(d, blocks, false);
+    Job j = make_job(d, blocks * splits, false);
+    const int split = j.block % splits;
+    j.block /= splits;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const bool for_v = ROLES == 1 || wave < KW;
     const int key0 = j.block * Sh::KEYS + wave % KW * 32, key = key0 + (lane & 31);
@@ -1005,7 +1008,9 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
     const int wstart = d.causal ? max(0, min(d.Tq, key0 - j.first)) * j.n : 0;
     const int wfull = d.causal ? max(0, min(d.Tq, key0 + 31 - j.first)) * j.n : 0;
     const int rmin = d.causal ? max(0, min(d.Tq, key - j.first)) * j.n : 0;
-    const int rend = j.block * Sh::KEYS < j.len ? j.rows : 0;
+    // the split's share of the tiles of rows that see a key of the block
+    const int all0 = bstart / RT * RT, all1 = j.block * Sh::KEYS < j.len ? j.rows : 0, share = ((all1 - all0 + RT - 1) / RT + splits - 1) / splits * RT;
+    const int rbeg = all0 + split * share, rend = min(all1, rbeg + share);
 
     const MEP_G T* qb = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)j.g * j.n * d.q_sH;
     const MEP_G T* ob = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
@@ -1076,7 +1081,6 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
             if (i == 0) Neg[buf] = neg;
         }
     };
-    const int rbeg = bstart / RT * RT;
     if (rbeg < rend) {
         load_rows(0, rbeg);
         fetch_stats(rbeg);
@@ -1214,8 +1218,29 @@ __global__ __launch_bounds__(64 * KW * (DK == 32 ? 1 : 2), KW / 2) void k_diff_b
             }
         }
     };
-    auto put_v = [&](T* mine) { write_rows<M>(mine, av, 1.f, d.dv, d.dv % M::E == 0, [&](int r) { return key_at(bd.dv, r, d.dv); }); };
+    // with splits, a split's sums in fp32: [splits][B, Tk, G][2 d + dv]
+    auto put_part = [&](const auto& acc, int at, int n, float f) {
+        if (key >= d.Tk) return;
+        gfloat* p = G<float>(bd.workspace) + (((int64_t)split * d.B * d.Tk * d.G) + first + (int64_t)key * d.G) * (2 * d.d + d.dv) + at;
+        constexpr int N = sizeof(acc) / sizeof(acc[0]);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int col = 32 * i + acc_off(r) + 4 * h;
+                if (col < n) p[col] = acc[i][r] * f;
+            }
+    };
+    auto put_v = [&](T* mine) {
+        if (splits > 1) return put_part(av, 2 * d.d, d.dv, 1.f);
+        write_rows<M>(mine, av, 1.f, d.dv, d.dv % M::E == 0, [&](int r) { return key_at(bd.dv, r, d.dv); });
+    };
     auto put_k = [&](T* mine) {
+        if (splits > 1) {
+            put_part(a1, 0, d.d, d.scale);
+            put_part(a2, d.d, d.d, -d.scale);
+            return;
+        }
         write_rows<M>(mine, a1, d.scale, d.d, d.d % M::E == 0, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
         write_rows<M>(mine, a2, -d.scale, d.d, d.d % M::E == 0, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
     };
@@ -1268,7 +1293,7 @@ void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_
     else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(128), 0, st, d, blocks, splits, tiles);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
-                            dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks);
+                            dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks, splits);
 }
 
 // the smallest instance that holds the head widths

@@ -97,6 +97,23 @@ int64_t plan(const mep_diff_attn_desc& d, int64_t items, int per, int& blocks) {
     return grid < 1 << 23 ? grid : -1;            // of up to 512 threads: 2^32 threads are a launch's most
 }
 
+// dk and dv from the splits' sums, in order
+template <class T>
+__global__ __launch_bounds__(DA_THREADS) void k_diff_kv_join(mep_diff_attn_bwd_desc bd, int splits) {
+    const mep_diff_attn_desc& d = bd.f;
+    const int w = 2 * d.d + d.dv;
+    const int64_t n = (int64_t)d.B * d.Tk * d.G, total = n * w;
+    for (int64_t i = (int64_t)blockIdx.x * DA_THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * DA_THREADS) {
+        const gfloat* p = G<const float>(bd.workspace) + i;
+        float s = p[0];
+        for (int k = 1; k < splits; ++k) s += p[k * total];
+        const int64_t row = i / w;
+        const int c = (int)(i - row * w);
+        if (c < 2 * d.d) G<T>(bd.dk)[row * 2 * d.d + c] = (T)s;
+        else G<T>(bd.dv)[row * d.dv + c - 2 * d.d] = (T)s;
+    }
+}
+
 // How the keys of a forward are split, or splits = 0: not at all.  Worth it where the rows are few: up to 32 a (batch, key head) leave
 // three of k_diff_fwd's four waves idle (against a row of 8192 keys, 32 batch rows, 4 key heads: 297 us whole, see k_diff_split),
 // and more rows too when their workgroups are under half the compute units and there are 1024 keys.  Then 8 workgroups
@@ -124,6 +141,17 @@ void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b,
     if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
     else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
     else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
+}
+
+// Into how many workgroups the rows of a block of keys are split: until there are two for every compute unit, 4 tiles of rows each at
+// least, 8 at most (each leaves its sums in fp32)
+int kv_splits(const mep_diff_attn_desc& d) {
+    const int dk = da_width(d.d, d.dv), per = 32 * da_kw(d.type, dk), tile = d.type == MEP_F32 ? 32 : 64;
+    const int64_t grid = (int64_t)d.B * d.G * ((d.Tk + per - 1) / per), tiles = ((int64_t)d.Tq * (d.H / d.G) + tile - 1) / tile;
+    if (grid == 0) return 1;
+    int64_t n = 512 / grid;
+    n = n > tiles / 4 ? tiles / 4 : n;
+    return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
 }
 
 bool attn_shape_ok(const mep_diff_attn_desc& d) {
@@ -215,6 +243,12 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     return 0;
 }
 
+extern "C" int64_t mep_diff_attn_bwd_workspace(const mep_diff_attn_desc* desc) {
+    if (!desc || !attn_shape_ok(*desc)) { mep_set_error("mep_diff_attn_bwd_workspace: invalid descriptor"); return MEP_EINVAL; }
+    const int n = kv_splits(*desc);
+    return n > 1 ? (int64_t)n * desc->B * desc->Tk * desc->G * (2 * desc->d + desc->dv) * 4 : 0;
+}
+
 extern "C" int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc) {
     if (!desc || !attn_shape_ok(*desc)) { mep_set_error("mep_diff_attn_workspace: invalid descriptor"); return MEP_EINVAL; }
     const Split s = split_of(*desc);
@@ -240,7 +274,17 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
                   kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
     if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, 0, st, d.dv);
-    if (keys && b.dk) run(DA_BWD_KV, d, &b, kg, kb, 1, 0, st, d.dv);
+    if (keys && b.dk) {
+        const int splits = b.workspace ? kv_splits(d) : 1;
+        run(DA_BWD_KV, d, &b, kg * splits, kb, splits, 0, st, d.dv);
+        if (splits > 1) {
+            const int64_t want = ((int64_t)d.B * d.Tk * d.G * (2 * d.d + d.dv) + DA_THREADS - 1) / DA_THREADS;
+            const dim3 grid((unsigned)(want < 4096 ? want : 4096)), block(DA_THREADS);
+            if (d.type == MEP_F32) hipLaunchKernelGGL(k_diff_kv_join<float>, grid, block, 0, st, b, splits);
+            else if (d.type == MEP_BF16) hipLaunchKernelGGL(k_diff_kv_join<__bf16>, grid, block, 0, st, b, splits);
+            else hipLaunchKernelGGL(k_diff_kv_join<_Float16>, grid, block, 0, st, b, splits);
+        }
+    }
     if (b.dlam) hipLaunchKernelGGL(k_diff_dlam, dim3(d.H), dim3(DLAM_THREADS), 0, st, b);
     return mep_check_launch("mep_diff_attn_bwd");
 }

@@ -333,6 +333,13 @@ def _packed(t, heads=1):
     return y
 
 
+def _workspace(name, desc, device):
+    n = getattr(_lib.lib(), name)(ctypes.byref(desc))
+    if n < 0:
+        _lib.check(n, name)
+    return torch.empty(n // 4, dtype=torch.float32, device=device) if n else None
+
+
 class _DiffAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, mask, lengths, q_start, q, k, v, lam):
@@ -357,13 +364,8 @@ class _DiffAttnFn(torch.autograd.Function):
                               B=B, Tq=Tq, Tk=Tk, H=H, G=G, d=hd, dv=dv, type=TYPES[q.dtype], causal=int(causal),
                               mask_form=0 if mask is None else mask.dim() - 1,
                               mask_float=int(mask is not None and mask.dtype == torch.float32), scale=scale)
-        ws = None
-        n = _lib.lib().mep_diff_attn_workspace(ctypes.byref(d))
-        if n > 0:
-            ws = torch.empty(n // 4, dtype=torch.float32, device=dev)
-            d.workspace = _ptr(ws)
-        elif n < 0:
-            _lib.check(n, 'mep_diff_attn_workspace')
+        ws = _workspace('mep_diff_attn_workspace', d, dev)
+        d.workspace = _ptr(ws)
         _launch('mep_diff_attn_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
@@ -389,9 +391,10 @@ class _DiffAttnFn(torch.autograd.Function):
         dlam = like(lam) if need[7] else None
         delta = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev)
         shared = lam.dim() == 1
+        ws = _workspace('mep_diff_attn_bwd_workspace', ctx.desc, dev) if dk is not None else None
         bd = _lib.DiffAttnBwdDesc(f=ctx.desc, dout=_ptr(dout), o_sB=dout.stride(0), o_sT=dout.stride(1), o_sH=dout.stride(2),
                                   dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlam=_ptr(dlam) if shared else 0,
-                                  dlam_rows=0 if shared else _ptr(dlam), delta=_ptr(delta))
+                                  dlam_rows=0 if shared else _ptr(dlam), delta=_ptr(delta), workspace=_ptr(ws))
         _launch('mep_diff_attn_bwd', bd, dev)
         return (None, None, None, None, dq, dk if need[5] else None, dv if need[6] else None, dlam)
 
