@@ -84,10 +84,16 @@ struct Geo {
     static constexpr int KT = TYPE == MEP_F32 ? 32 : 64;      // keys (or rows) of a staged tile
     static constexpr int NK = DK / M::KS, NV = DV / M::KS;    // operands along the head widths
     static constexpr int NP = 32 / M::KS;                     // operands of 32 keys
+    static constexpr int STEP = 16 / M::KS;                   // operands of 16 channels
     static constexpr int KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;      // elements of a tile's keys, and of a tile
     static constexpr int OUT = DA_ROWS * (da_piece(DK > DV ? DK : DV) + M::E);  // the results pass through the tiles
     static constexpr int BUF = 2 * TSZ > OUT ? 2 * TSZ : OUT;
 };
+
+// Narrower heads than the instance: in fp32, whose products take 16 times as long, the products of 16 channels (of results: 32)
+// behind a head's n are left out; in 16 bits the branches would cost more than the products
+template <int TYPE>
+MEP_DEV bool within(int col, int n) { return TYPE != MEP_F32 || col < n; }
 
 template <class M>
 MEP_DEV typename M::Frag zero_frag() {
@@ -105,7 +111,11 @@ MEP_DEV typename M::Frag row_frag(const MEP_G typename M::T* row, int c, int n, 
 
 // The N operands of a lane's row (n elements from p on): held in registers, or (wide fp32 heads, whose products take 16 times as long
 // and whose operands and accumulators would not fit) read again from the cache at each use.  A row that is not there: zeros.
-constexpr bool da_hold(int type, int dk) { return !(type == MEP_F32 && dk >= 64); }
+// One wave a SIMD with all its registers holds 64 channels of fp32, and two waves that read them again are slower (B 4, T 2048, 8
+// heads, 64 / 128: forward 1366 us against 969, dk and dv 1787 against 1365), but for dq (64 / 64: 891 against 1048).
+constexpr bool da_hold(int type, int dk) { return !(type == MEP_F32 && dk >= 128); }
+constexpr bool da_hold_q(int type, int dk) { return !(type == MEP_F32 && dk >= 64); }
+constexpr bool da_wide(int type, int dk) { return dk >= (type == MEP_F32 ? 64 : 128); }
 template <class M, int N, bool HOLD>
 struct Operand {
     typedef typename M::Frag Frag;
@@ -266,6 +276,22 @@ MEP_DEV typename M::Frag acc_frag(const floatx16& p, int i) {
 }
 
 MEP_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 2^(s c - m), c = scale log2 e.  In fp32 the rounding of c is put right (it would shift every exponent the same way, by up to
+// 2^-24 s c: a score's error would not average out); a masked score (-inf) stays one.  In 16 bits the operands' rounding is
+// far above it.
+template <int TYPE>
+struct Exponent {
+    float c, low;
+    MEP_DEV explicit Exponent(float scale) {
+        c = scale * DA_LOG2E;
+        low = fmaf(scale, DA_LOG2E, -c) + scale * 1.9259629911e-8f;      // log2 e - DA_LOG2E
+    }
+    MEP_DEV float at(float s, float m) const {
+        const float t = fmaf(s, c, -m);
+        return exp2_fast(TYPE == MEP_F32 ? fmaf(fmaxf(s, DA_MIN), low, t) : t);
+    }
+};
 // v over both lane halves of a row: lo and hi, each in every lane
 MEP_DEV void both_halves(float v, float& lo, float& hi) {
     const unsigned u = __builtin_bit_cast(unsigned, v);
@@ -482,14 +508,15 @@ struct Online {
     // The backward's e_m are to be at most 1: it gets maxima 8 up, or in float16, whose subnormals begin at 2^-14, the true ones
     static constexpr bool TOP = TYPE == MEP_F16;
     typedef Operand<M, Ge::NK, da_hold(TYPE, DK)> Q;
+    Exponent<TYPE> ex;
     Q q1, q2;
     float c, lam, m1, m2, l1, l2, f1, f2, top1, top2;
     floatx16 x[DV / 32], y[DV / 32];
 
     MEP_DEV Online(const mep_diff_attn_desc& d, const Job& j, const Rows32& w)
-        : q1(G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH, d.d, w.live), q2(q1.p + d.q_sM, d.d, w.live) {
+        : ex(d.scale), q1(G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH, d.d, w.live), q2(q1.p + d.q_sM, d.d, w.live) {
         lam = G<const float>(d.lam)[(int64_t)j.b * d.lam_sB + (int64_t)w.t * d.lam_sT + (int64_t)w.head * d.lam_sH];
-        c = d.scale * DA_LOG2E;
+        c = ex.c;
         m1 = m2 = mul_rn(DA_MIN, c);
         l1 = l2 = f2 = 0.f;
         f1 = 1.f;
@@ -502,10 +529,14 @@ struct Online {
                       const T* kt, const T* vt, int r0, int ks, unsigned on) {
         floatx16 s1 = zero16(), s2 = zero16();
 #pragma unroll
-        for (int i = 0; i < Ge::NK; ++i) {
-            s1 = M::mma(kread.rows(kt, r0, i), q1.at(i), s1);
-            s2 = M::mma(kread.rows(kt, r0, Ge::NK + i), q2.at(i), s2);
-        }
+        for (int g = 0; g < Ge::NK; g += Ge::STEP)
+            if (within<TYPE>(M::KS * g, d.d)) {
+#pragma unroll
+                for (int i = g; i < g + Ge::STEP; ++i) {
+                    s1 = M::mma(kread.rows(kt, r0, i), q1.at(i), s1);
+                    s2 = M::mma(kread.rows(kt, r0, Ge::NK + i), q2.at(i), s2);
+                }
+            }
         if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
         const float a1 = max16(s1), a2 = max16(s2);
         if constexpr (TOP) {
@@ -528,13 +559,16 @@ struct Online {
                 }
             f2 = 0.f;
         }
+        float u1 = 0.f, u2 = 0.f;      // sums of sums: a long row's rounding grows with its tiles
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s1[r] = exp2_fast(fmaf(s1[r], c, -m1));
-            s2[r] = exp2_fast(fmaf(s2[r], c, -m2));
-            l1 += s1[r];
-            l2 += s2[r];
+            s1[r] = ex.at(s1[r], m1);
+            s2[r] = ex.at(s2[r], m2);
+            u1 += s1[r];
+            u2 += s2[r];
         }
+        l1 += u1;
+        l2 += u2;
         const float t1 = lam * half_sum(l1), t2 = half_sum(l2);
         if (__ballot(fabsf(t1 * f1 - t2 * f2) > 0.25f * fabsf(t1 * f1))) {
             const float rho = t2 > 0.f ? t1 / t2 : 0.f, h1 = 1.f / fmaxf(1.f, fabsf(rho)), h2 = rho * h1;
@@ -552,11 +586,12 @@ struct Online {
         for (int i = 0; i < Ge::NP; ++i) {
             const Frag p = acc_frag<M>(s1, i), e = acc_frag<M>(s2, i);
 #pragma unroll
-            for (int n = 0; n < DV / 32; ++n) {
-                const Frag v = vread.cols(vt, r0, 32 * n, i);
-                x[n] = M::mma(v, p, x[n]);
-                y[n] = M::mma(v, e, y[n]);
-            }
+            for (int n = 0; n < DV / 32; ++n)
+                if (within<TYPE>(32 * n, d.dv)) {
+                    const Frag v = vread.cols(vt, r0, 32 * n, i);
+                    x[n] = M::mma(v, p, x[n]);
+                    y[n] = M::mma(v, e, y[n]);
+                }
         }
     }
     // the maxima that the backward gets, and 2^(m - those)
@@ -570,7 +605,7 @@ struct Online {
 
 // ld: channels between out's rows (values wider than 128 channels are taken by two launches)
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int ld) {
+__global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int ld) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
@@ -739,14 +774,14 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
     const KeyTiles<TYPE, DK, DV> keys(d, j);
     const Reader<M, 2 * DK> kread;
     const Reader<M, DV> vread;
-    const float c = d.scale * DA_LOG2E;
+    const Exponent<TYPE> ex(d.scale);
     const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
 
     unsigned raw = key_raw(d, j, 0);
     unsigned long long bits = key_bits(d, j, 0, KT, raw);
     if (end > 0) keys.load(Buf, 0, bits);
     raw = key_raw(d, j, KT);
-    constexpr bool HOLD = da_hold(TYPE, DK);
+    constexpr bool HOLD = da_hold_q(TYPE, DK);
     const MEP_G T* qp = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)w.t * d.q_sT + (int64_t)w.head * d.q_sH;
     const Operand<M, Ge::NK, HOLD> q1(qp, d.d, w.live), q2(qp + d.q_sM, d.d, w.live);
     const Operand<M, Ge::NV, HOLD> g(G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)w.t * bd.o_sT + (int64_t)w.head * bd.o_sH, d.dv, w.live);
@@ -806,18 +841,27 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
             if (ks >= w.wend || !on) continue;
             floatx16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
-            for (int i = 0; i < Ge::NK; ++i) {
-                s1 = M::mma(kread.rows(kt, 32 * sub, i), q1.at(i), s1);
-                s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q2.at(i), s2);
-            }
+            for (int n = 0; n < Ge::NK; n += Ge::STEP)
+                if (within<TYPE>(M::KS * n, d.d)) {
 #pragma unroll
-            for (int i = 0; i < Ge::NV; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g.at(i), dp);
+                    for (int i = n; i < n + Ge::STEP; ++i) {
+                        s1 = M::mma(kread.rows(kt, 32 * sub, i), q1.at(i), s1);
+                        s2 = M::mma(kread.rows(kt, 32 * sub, Ge::NK + i), q2.at(i), s2);
+                    }
+                }
+#pragma unroll
+            for (int n = 0; n < Ge::NV; n += Ge::STEP)
+                if (within<TYPE>(M::KS * n, d.dv)) {
+#pragma unroll
+                    for (int i = n; i < n + Ge::STEP; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g.at(i), dp);
+                }
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
+            float u1 = 0.f, u2 = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {      // e_m, the row sums, and dS_m without the row's factors 1 / l1, -lam / l2
-                const float e1 = exp2_fast(fmaf(s1[r], c, -st[0])), e2 = exp2_fast(fmaf(s2[r], c, -st[2]));
-                sum1 = fmaf(e1, dp[r], sum1);
-                sum2 = fmaf(e2, dp[r], sum2);
+                const float e1 = ex.at(s1[r], st[0]), e2 = ex.at(s2[r], st[2]);
+                u1 = fmaf(e1, dp[r], u1);
+                u2 = fmaf(e2, dp[r], u2);
                 if constexpr (CORR) {
                     sq1 = fmaf(e1, e1, sq1);
                     sq2 = fmaf(e2, e2, sq2);
@@ -830,6 +874,8 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
                     s2[r] = e2 * (dp[r] - d2);
                 }
             }
+            sum1 += u1;
+            sum2 += u2;
             Frag e1[BESIDE ? Ge::NP : 1], e2[BESIDE ? Ge::NP : 1];
             if constexpr (BESIDE) {
 #pragma unroll
@@ -848,6 +894,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
                 const Frag p1 = acc_frag<M>(s1, i), p2 = acc_frag<M>(s2, i);
 #pragma unroll
                 for (int n = 0; n < DK / 32; ++n) {
+                    if (!within<TYPE>(32 * n, d.d)) continue;
                     const Frag k1 = kread.cols(kt, 32 * sub, 32 * n, i), k2 = kread.cols(kt, 32 * sub, DK + 32 * n, i);
                     a1[n] = M::mma(k1, p1, a1[n]);
                     a2[n] = M::mma(k2, p2, a2[n]);
@@ -891,8 +938,8 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
                     if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        s1[r] = exp2_fast(fmaf(s1[r], c, -st[0]));
-                        s2[r] = exp2_fast(fmaf(s2[r], c, -st[2]));
+                        s1[r] = ex.at(s1[r], st[0]);
+                        s2[r] = ex.at(s2[r], st[2]);
                     }
 #pragma unroll
                     for (int i = 0; i < Ge::NP; ++i) {
@@ -947,7 +994,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
 //   dP' = dP - D_1, and D_1 - D_2 added for the second map
 // the rest is a product and an exponential each.  (lse_m folds a sum into the maximum, which costs last bits where the maximum is
 // large: of no account in 16 bits.  In fp32, whose products take 16 times as long, the row's values are read from LDS.)
-constexpr int da_roles(int type, int dk) { return dk == 32 || (type == MEP_F32 && dk == 64) ? 1 : 2; }
+constexpr int da_roles(int type, int dk) { return dk == 32 || type == MEP_F32 ? 1 : 2; }
 template <int KW, int TYPE, int DK, int DV>
 struct KvShape {
     typedef Geo<TYPE, DK, DV> Ge;
@@ -982,7 +1029,7 @@ MEP_DEV floatx16 row_values(const bf16x8_da* x) {
 }
 
 template <int KW, int TYPE, int DK, int DV>
-__global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks, int splits) {
+__global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1 : 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks, int splits) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef KvShape<KW, TYPE, DK, DV> Sh;
     typedef typename Ge::M M;
@@ -1002,7 +1049,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_b
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const bool for_v = ROLES == 1 || wave < KW;
     const int key0 = j.block * Sh::KEYS + wave % KW * 32, key = key0 + (lane & 31);
-    const float c = d.scale * DA_LOG2E;
+    const Exponent<TYPE> ex(d.scale);
+    const float c = ex.c;
     // rows that see any of the block's / the wave's keys; every one of the wave's keys: from row wfull on; the lane's key: from rmin on
     const int bstart = d.causal ? max(0, min(d.Tq, j.block * Sh::KEYS - j.first)) * j.n : 0;
     const int wstart = d.causal ? max(0, min(d.Tq, key0 - j.first)) * j.n : 0;
@@ -1105,10 +1153,14 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_b
             s1 = s2 = zero16();
         }
 #pragma unroll
-        for (int i = 0; i < Ge::NK; ++i) {
-            s1 = M::mma(qread.rows(qt, 32 * sub, i), k1.at(i), s1);
-            s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), k2.at(i), s2);
-        }
+        for (int n = 0; n < Ge::NK; n += Ge::STEP)
+            if (within<TYPE>(M::KS * n, d.d)) {
+#pragma unroll
+                for (int i = n; i < n + Ge::STEP; ++i) {
+                    s1 = M::mma(qread.rows(qt, 32 * sub, i), k1.at(i), s1);
+                    s2 = M::mma(qread.rows(qt, 32 * sub, Ge::NK + i), k2.at(i), s2);
+                }
+            }
         if (!all_on || rs < wfull || d.mask_form == 2) {      // rows that see this lane's key: those from rmin on
             const int least = rmin - rs - 4 * h;
             unsigned ok = !on || least > 31 ? 0u : least > 0 ? ~0u << least : ~0u;
@@ -1141,8 +1193,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_b
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int lr = 32 * sub + acc_off(r) + 4 * h;
-                s1[r] = exp2_fast(fmaf(s1[r], c, -Rs[buf][R_M1][lr])) * Rs[buf][R_I1][lr];
-                s2[r] = exp2_fast(fmaf(s2[r], c, -Rs[buf][R_M2][lr])) * Rs[buf][R_LI2][lr];
+                s1[r] = ex.at(s1[r], Rs[buf][R_M1][lr]) * Rs[buf][R_I1][lr];
+                s2[r] = ex.at(s2[r], Rs[buf][R_M2][lr]) * Rs[buf][R_LI2][lr];
             }
         }
     };
@@ -1183,7 +1235,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_b
         for (int i = 0; i < Ge::NP; ++i) {
             const Frag f = acc_frag<M>(p, i);
 #pragma unroll
-            for (int n = 0; n < DV / 32; ++n) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), f, av[n]);
+            for (int n = 0; n < DV / 32; ++n)
+                if (within<TYPE>(32 * n, d.dv)) av[n] = M::mma(oread.cols(ot, 32 * sub, 32 * n, i), f, av[n]);
         }
     };
     // dk_m += dS_m^T q_m; s1, s2: the maps
@@ -1193,7 +1246,11 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_b
         if constexpr (PARTS) dp = row_values(Xs[buf][X_D1] + 32 * sub);
         else dp = zero16();
 #pragma unroll
-        for (int i = 0; i < Ge::NV; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), v.at(i), dp);
+        for (int n = 0; n < Ge::NV; n += Ge::STEP)
+            if (within<TYPE>(M::KS * n, d.dv)) {
+#pragma unroll
+                for (int i = n; i < n + Ge::STEP; ++i) dp = M::mma(oread.rows(qt + Ge::KSZ, 32 * sub, i), v.at(i), dp);
+            }
         if constexpr (PARTS) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s1[r] *= dp[r];
@@ -1212,10 +1269,11 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), KW / 2) void k_diff_b
         for (int i = 0; i < Ge::NP; ++i) {
             const Frag f1 = acc_frag<M>(s1, i), f2 = acc_frag<M>(s2, i);
 #pragma unroll
-            for (int n = 0; n < DK / 32; ++n) {
-                a1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, a1[n]);
-                a2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, a2[n]);
-            }
+            for (int n = 0; n < DK / 32; ++n)
+                if (within<TYPE>(32 * n, d.d)) {
+                    a1[n] = M::mma(qread.cols(qt, 32 * sub, 32 * n, i), f1, a1[n]);
+                    a2[n] = M::mma(qread.cols(qt, 32 * sub, DK + 32 * n, i), f2, a2[n]);
+                }
         }
     };
     // with splits, a split's sums in fp32: [splits][B, Tk, G][2 d + dv]

@@ -122,7 +122,7 @@ struct Split { int blocks, splits, tiles; };
 Split split_of(const mep_diff_attn_desc& d) {
     Split s = {0, 0, 0};
     const int64_t rows = (int64_t)d.Tq * (d.H / d.G), pairs = (int64_t)d.B * d.G;
-    const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) < 128;
+    const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) < 64;
     if (pairs == 0 || rows == 0 || !(few || none)) return s;
     s.blocks = (int)((rows + 31) / 32);
     const int kt = da_split_keys(d.type, da_width(d.d, d.dv), da_piece(da_value_width(d.d, d.dv))), all = (d.Tk + kt - 1) / kt;
