@@ -559,7 +559,7 @@ struct Online {
                 }
             f2 = 0.f;
         }
-        float u1 = 0.f, u2 = 0.f;      // sums of sums: a long row's rounding grows with its tiles
+        float u1 = 0.f, u2 = 0.f;      // sums by tiles: a long row's rounding grows with their number only
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s1[r] = ex.at(s1[r], m1);
@@ -603,15 +603,26 @@ struct Online {
     }
 };
 
-// ld: channels between out's rows (values wider than 128 channels are taken by two launches)
+// Values wider than 128 channels (parts = 2; their accumulators would not fit beside each other) are taken by two workgroups that both
+// form the scores.
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int ld) {
+__global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int parts) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
     constexpr int KT = Ge::KT;
     __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
-    const Job j = make_job(d, blocks, d.causal);
+    const int ld = d.dv;
+    Job j = make_job(d, blocks * parts, d.causal);
+    if (DV == 128 && parts == 2) {
+        const int c = j.block % 2 * DV;
+        j.block /= 2;
+        d.v += c * sizeof(T);
+        d.out += c * sizeof(T);
+        if (d.second) d.second += c * sizeof(T);
+        if (c) d.stats = 0;
+        d.dv = min(ld - c, DV);
+    }
     const int h = (threadIdx.x & 63) >> 5;
     const Rows32 w(d, j, j.block * DA_ROWS + (threadIdx.x >> 6) * 32);
     const KeyTiles<TYPE, DK, DV> keys(d, j);
@@ -1346,8 +1357,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
 constexpr int da_kw(int type, int dk) { return dk >= 128 && type != MEP_F32 ? 2 : 4; }
 
 template <int TYPE, int DK, int DV>
-void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {      // (tiles: DA_FWD's ld)
-    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, tiles);
+void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {      // (splits: DA_FWD's parts)
+    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
     else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(128), 0, st, d, blocks, splits, tiles);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),

@@ -34,36 +34,66 @@ __global__ __launch_bounds__(DLAM_THREADS) void k_diff_dlam(mep_diff_attn_bwd_de
     }
 }
 
-// out = E_1 / l_1 - lam E_2 / l_2 of a row from its parts, a thread per value channel; rows side by side in a workgroup
+// out = E_1 / l_1 - lam E_2 / l_2 of a row from its parts: a thread per value channel, rows side by side in a workgroup.  Bound by the
+// latency of its loads: the parts' statistics are read a part a lane, and the sums of 8 parts are in flight.
 __global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, int blocks, int parts, int per, int ld) {
-    const int ch = threadIdx.x % per;
-    const int64_t r = (int64_t)blockIdx.x * (DA_THREADS / per) + threadIdx.x / per;      // (b, t, head)
-    if (r >= (int64_t)d.B * d.Tq * d.H) return;
+    const int ch = threadIdx.x % per, lanes = min(per, 64), lane = threadIdx.x % lanes;
+    const int64_t all = (int64_t)d.B * d.Tq * d.H, at = (int64_t)blockIdx.x * (DA_THREADS / per) + threadIdx.x / per;
+    const int64_t r = min(at, all - 1);      // (b, t, head); lanes without a row work on the last one and write nothing
     const int64_t bt = r / d.H;
     const int head = (int)(r - bt * d.H), b = (int)(bt / d.Tq), t = (int)(bt - (int64_t)b * d.Tq);
     const int n = d.H / d.G, g = head / n, row = t * n + head - g * n;
     const int64_t stride = split_floats(d.dv);
     const gfloat* part = G<const float>(d.workspace) + (((int64_t)b * d.G + g) * blocks + row / 32) * parts * stride;
     const int lr = row & 31;
+    auto stats = [&](int p) { return *reinterpret_cast<const MEP_G f32x4*>(part + p * stride + 4 * lr); };
     float m1 = -INFINITY, m2 = -INFINITY;
-    for (int p = 0; p < parts; ++p) {
-        const f32x4 s = *reinterpret_cast<const MEP_G f32x4*>(part + p * stride + 4 * lr);
+    for (int p = lane; p < parts; p += lanes) {
+        const f32x4 s = stats(p);
         m1 = fmaxf(m1, s[0]);
         m2 = fmaxf(m2, s[2]);
     }
+    for (int o = lanes / 2; o; o /= 2) {
+        m1 = fmaxf(m1, __shfl_xor(m1, o));
+        m2 = fmaxf(m2, __shfl_xor(m2, o));
+    }
     float l1 = 0.f, l2 = 0.f, e1 = 0.f, e2 = 0.f;
-    for (int p = 0; p < parts; ++p) {
-        const gfloat* q = part + p * stride;
-        const f32x4 s = *reinterpret_cast<const MEP_G f32x4*>(q + 4 * lr);
-        if (!(s[1] != 0.f || s[3] != 0.f)) continue;      // no key of this row there, and nothing written
-        const float w1 = exp2_fast(s[0] - m1), w2 = exp2_fast(s[2] - m2);
-        l1 = fmaf(s[1], w1, l1);
-        l2 = fmaf(s[3], w2, l2);
-        if (ch < d.dv) {
-            e1 = fmaf(q[128 + lr * d.dv + ch], w1, e1);
-            e2 = fmaf(q[128 + (32 + lr) * d.dv + ch], w2, e2);
+    const gfloat* v1 = part + 128 + lr * d.dv + min(ch, d.dv - 1);
+    const gfloat* v2 = v1 + 32 * d.dv;
+    for (int p0 = 0; p0 < parts; p0 += lanes) {
+        float w1 = 0.f, w2 = 0.f;
+        bool on = false;                          // without a key of this row there, no sums are written
+        if (p0 + lane < parts) {
+            const f32x4 s = stats(p0 + lane);
+            on = s[1] != 0.f || s[3] != 0.f;
+            w1 = on ? exp2_fast(s[0] - m1) : 0.f;
+            w2 = on ? exp2_fast(s[2] - m2) : 0.f;
+            l1 = on ? fmaf(s[1], w1, l1) : l1;
+            l2 = on ? fmaf(s[3], w2, l2) : l2;
+        }
+        const int count = min(lanes, parts - p0);
+        for (int i = 0; i < count; i += 8) {
+            float a[8], c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t o = min(p0 + i + j, parts - 1) * stride;
+                a[j] = v1[o];
+                c[j] = v2[o];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {         // (i + j < lanes, a multiple of 8; weights behind the last part are not on)
+                const float u1 = __shfl(w1, i + j, lanes), u2 = __shfl(w2, i + j, lanes);
+                const bool x = __shfl((int)on, i + j, lanes);
+                e1 = x ? fmaf(a[j], u1, e1) : e1;
+                e2 = x ? fmaf(c[j], u2, e2) : e2;
+            }
         }
     }
+    for (int o = lanes / 2; o; o /= 2) {
+        l1 += __shfl_xor(l1, o);
+        l2 += __shfl_xor(l2, o);
+    }
+    if (at >= all) return;
     const float i1 = l1 > 0.f ? 1.f / l1 : l1, i2 = l2 > 0.f ? 1.f / l2 : l2;
     const float lam = G<const float>(d.lam)[(int64_t)b * d.lam_sB + (int64_t)t * d.lam_sT + (int64_t)head * d.lam_sH];
     if (d.stats && ch == 0) *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)b * d.H + head) * d.Tq + t)) = f32x4{m1, i1, m2, i2};
@@ -219,8 +249,14 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     if (grid < 0) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
     hipStream_t st = (hipStream_t)stream;
     const Split s = split_of(d);
-    // values of more than 128 channels in two launches: their accumulators would not fit beside each other
     const int es = d.type == MEP_F32 ? 4 : 2, half = da_piece(d.dv);
+    if (!s.splits || !d.workspace) {
+        const int parts = d.dv > half ? 2 : 1;
+        if (grid * parts >= 1 << 23) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
+        run(DA_FWD, d, nullptr, grid * parts, blocks, parts, 0, st, d.dv);
+        return mep_check_launch("mep_diff_attn_fwd");
+    }
+    // values of more than 128 channels in two launches: their accumulators would not fit beside each other
     for (int c = 0; c < d.dv; c += half) {
         mep_diff_attn_desc p = d;
         p.dv = d.dv - c < half ? d.dv - c : half;
@@ -228,15 +264,11 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
         p.out += (uint64_t)c * es;
         if (p.second) p.second += (uint64_t)c * es;
         if (c) p.stats = 0;
-        if (!s.splits || !d.workspace) {
-            run(DA_FWD, p, nullptr, grid, blocks, 1, d.dv, st, d.dv);
-        } else {
-            run(DA_SPLIT, p, nullptr, (int64_t)s.blocks * s.splits * d.B * d.G, s.blocks, s.splits, s.tiles, st, d.dv);
-            int per = 32;
-            while (per < p.dv) per *= 2;
-            const int64_t rows = (int64_t)d.B * d.Tq * d.H, side = DA_THREADS / per;
-            hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, p, s.blocks, 2 * s.splits, per, d.dv);
-        }
+        run(DA_SPLIT, p, nullptr, (int64_t)s.blocks * s.splits * d.B * d.G, s.blocks, s.splits, s.tiles, st, d.dv);
+        int per = 32;
+        while (per < p.dv) per *= 2;
+        const int64_t rows = (int64_t)d.B * d.Tq * d.H, side = DA_THREADS / per;
+        hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, p, s.blocks, 2 * s.splits, per, d.dv);
         const int rc = mep_check_launch("mep_diff_attn_fwd");
         if (rc) return rc;
     }
