@@ -108,12 +108,12 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, 
     if (d.second) put(d.second, e2 * i2);
 }
 
-// rows that can be read 16 bytes at a time, a tile of 64 time steps with all its heads and maps within 2^30 elements (the DMA's
-// 32-bit byte offsets)
+// rows that can be read 16 bytes at a time, a tile of 64 time steps with all its heads and maps within 2 GiB (the DMA's 32-bit
+// byte offsets)
 bool rows_ok(const mep_diff_attn_desc& d, uint64_t p, int64_t sB, int64_t sT, int64_t sH, int64_t sM, bool heads) {
-    const int64_t V = d.type == MEP_F32 ? 4 : 8;
+    const int64_t V = d.type == MEP_F32 ? 4 : 8, h = heads ? d.H / d.G : 0;
     return p % 16 == 0 && sB % V == 0 && sT % V == 0 && sH % V == 0 && sM % V == 0 && sT >= 0 && sT < 1 << 23 && sM >= 0 && sM < 1 << 28 &&
-           (!heads || (sH >= 0 && sH * (d.H / d.G) < 1 << 28));
+           (!heads || (sH >= 0 && sH * h < 1 << 28)) && 64 * sT + sM + sH * h < (V << 27) - 512;
 }
 bool inputs_ok(const mep_diff_attn_desc& d) {
     return rows_ok(d, d.q, d.q_sB, d.q_sT, d.q_sH, d.q_sM, true) && rows_ok(d, d.k, d.k_sB, d.k_sT, d.k_sH, d.k_sM, false) &&

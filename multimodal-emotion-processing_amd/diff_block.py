@@ -57,6 +57,19 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _places(saved):
+    """Where saved tensors lie.  Hooks on them (a checkpoint that computes them again, offloading) give the backward others."""
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in saved]
+
+
+def _moved(desc, names, tensors):
+    """A copy of the descriptor with the addresses of `tensors`."""
+    d = type(desc).from_buffer_copy(desc)
+    for n, t in zip(names, tensors):
+        setattr(d, n, _ptr(t))
+    return d
+
+
 # ------------------------------------------------------------------ rotary positions
 def rotary_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, original_len=None, low_turns=1.0,
                        high_turns=32.0, device='cuda'):
@@ -148,6 +161,8 @@ def rotary(q, k=None, *, positions, freqs, layout='half', amplitude=1.0):
     B, T, D = q.shape[0], q.shape[1], q.shape[-1]
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 1 <= freqs.numel() <= D // 2:
         raise ValueError('freqs must be contiguous float64 [r / 2] with 2 <= r <= channels; got %s %s' % (tuple(freqs.shape), freqs.dtype))
+    if freqs.requires_grad:
+        raise ValueError('freqs have no gradient')
     if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((T,), (B, T)):
         raise ValueError('positions must be int32 or int64 [time] or [batch, time]; got %s %s' % (tuple(positions.shape), positions.dtype))
     if layout not in ('half', 'interleaved'):
@@ -169,7 +184,7 @@ def _rows(t, D):
 class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, y, x, w, b, gate, scale, nw, nb):
-        kind, next_kind, gate_form, T, eps, scale_value = cfg
+        kind, next_kind, gate_form, T, eps, scale_value, grad = cfg
         D = y.shape[-1]
         dev = y.device
         y2, y_ld = _rows(y, D)
@@ -179,7 +194,7 @@ class _NormFn(torch.autograd.Function):
         n = y2.shape[0]
         stream = torch.empty(y.shape, dtype=y.dtype, device=dev)
         normed = torch.empty(y.shape, dtype=y.dtype, device=dev) if next_kind else None
-        keep = any(ctx.needs_input_grad)
+        keep = grad and any(ctx.needs_input_grad)
         stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if keep else None
         params = [t for t in (w, b, nw, nb) if t is not None]
         d = _lib.BlockNormDesc(y=_ptr(y2), x=_ptr(x2), gate=_ptr(g2), w=_ptr(w), b=_ptr(b), nw=_ptr(nw), nb=_ptr(nb),
@@ -191,25 +206,34 @@ class _NormFn(torch.autograd.Function):
             _launch('mep_block_norm_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
-            ctx.save_for_backward(y2, x2, g2, w, b, scale, nw, nb)
-            ctx.held = stats
+            saved = (y2, x2, g2, w, b, scale, nw, nb, stats)
+            ctx.save_for_backward(*saved)
             ctx.shapes = (y.shape, None if gate is None else gate.shape, None if scale is None else scale.shape)
             # the backward reads the forward's inputs by address, and asks of its results only which there were
-            ctx.desc = d
+            ctx.desc, ctx.places = d, _places(saved)
         return (stream, normed) if next_kind else stream
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dstream, dnormed=None):
-        y2, x2, g2, w, b, scale, nw, nb = ctx.saved_tensors
+        saved = ctx.saved_tensors
         none = (None,) * 9
         if dstream is None and dnormed is None:
             return none
         need = ctx.needs_input_grad
         shape, gate_shape, scale_shape = ctx.shapes
+        d = ctx.desc
+        if _places(saved) != ctx.places:
+            D = shape[-1]
+            y2, x2, g2 = saved[:3]
+            (y2, y_ld), (x2, x_ld) = _rows(y2, D), _rows(x2, D) if x2 is not None else (None, 0)
+            g2, g_ld = _rows(g2, D) if d.gate_form == 3 else (g2, 0)
+            saved = (y2, x2, g2, *(None if t is None else t.contiguous() for t in saved[3:]))
+            d = _moved(d, ('y', 'x', 'gate', 'w', 'b', 'scale', 'nw', 'nb', 'stats'), saved)
+            d.y_ld, d.x_ld, d.g_ld = y_ld, x_ld, g_ld
+        y2, x2, g2, w, b, scale, nw, nb, _ = saved
         n, D = y2.shape
         dev = y2.device
-        d = ctx.desc
         rows = lambda on: torch.empty(shape, dtype=y2.dtype, device=dev) if on else None  # noqa: E731
         like = lambda t, on: torch.empty_like(t) if t is not None and on else None  # noqa: E731
         dy, dx = rows(True), rows(x2 is not None and need[2])
@@ -304,7 +328,7 @@ def norm_residual(y, residual, weight=None, bias=None, *, kind='rms', gate=None,
     else:
         sv = float(scale)
     _on_device(y, residual, weight, bias, gate, next_weight, next_bias, st)
-    cfg = (KINDS[kind], KINDS[next_kind], form, T, float(eps), sv)
+    cfg = (KINDS[kind], KINDS[next_kind], form, T, float(eps), sv, torch.is_grad_enabled())
     return _NormFn.apply(cfg, y, residual, weight, bias, gate, st, next_weight, next_bias)
 
 
@@ -316,14 +340,14 @@ def norm(x, weight=None, bias=None, *, kind='rms', eps=1e-6):
 
 
 # ------------------------------------------------------------------ differential attention
-def _packed(t, heads=1):
-    """t [B, T, H, (2,) n] as the attention kernels read it: 16 bytes at a time, 64 time steps within 2^30 elements; a copy with
+def _packed(t, heads=0):
+    """t [B, T, H, (2,) n] as the attention kernels read it: 16 bytes at a time, 64 time steps with their heads within 2 GiB; a copy with
     rows padded by zeros (mep_pack_rows) where it does not lie so."""
     V = 16 // t.element_size()
     st = t.stride()
     sM = st[3] if t.dim() == 5 else 0
     if st[-1] == 1 and t.shape[-1] % V == 0 and t.data_ptr() % 16 == 0 and not any(s % V for s in st[:-1]) and \
-            st[1] < 1 << 23 and sM < 1 << 28 and st[2] * heads < 1 << 28:
+            st[1] < 1 << 23 and sM < 1 << 28 and st[2] * heads < 1 << 28 and 64 * st[1] + sM + st[2] * heads < (V << 27) - 512:
         return t
     n = t.shape[-1]
     y = torch.empty(*t.shape[:-1], -(-n // V) * V, dtype=t.dtype, device=t.device)
@@ -340,39 +364,40 @@ def _workspace(name, desc, device):
     return torch.empty(n // 4, dtype=torch.float32, device=device) if n else None
 
 
+def _strides(d, q, k, v, lam, mask):
+    d.q_sB, d.q_sT, d.q_sH, d.q_sM, _ = q.stride()
+    d.k_sB, d.k_sT, d.k_sH, d.k_sM, _ = k.stride()
+    d.v_sB, d.v_sT, d.v_sH, _ = v.stride()
+    d.lam_sB, d.lam_sT, d.lam_sH = (0, 0, lam.stride(0)) if lam.dim() == 1 else lam.stride()
+    if mask is not None:
+        d.m_sB, d.m_sQ, d.m_sK = (mask.stride(0), 0, mask.stride(1)) if mask.dim() == 2 else mask.stride()
+
+
 class _DiffAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, mask, lengths, q_start, q, k, v, lam):
-        causal, scale = cfg
+        causal, scale, grad = cfg
         B, Tq, H, _, hd = q.shape
         Tk, G, dv = k.shape[1], k.shape[2], v.shape[3]
         dev = q.device
         qp, kp, vp = _packed(q, H // G), _packed(k), _packed(v)
         out = torch.empty(B, Tq, H, dv, dtype=q.dtype, device=dev)
-        keep = any(ctx.needs_input_grad)
+        keep = grad and any(ctx.needs_input_grad)
         stats = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev) if keep else None
         second = torch.empty_like(out) if keep else None
-        ls = (0, 0, lam.stride(0)) if lam.dim() == 1 else lam.stride()
-        m = (0, 0, 0)
-        if mask is not None:
-            m = (mask.stride(0), 0, mask.stride(1)) if mask.dim() == 2 else mask.stride()
-        qs, ks, vs = qp.stride(), kp.stride(), vp.stride()
         d = _lib.DiffAttnDesc(q=_ptr(qp), k=_ptr(kp), v=_ptr(vp), lam=_ptr(lam), out=_ptr(out), stats=_ptr(stats), second=_ptr(second),
-                              q_sB=qs[0], q_sT=qs[1], q_sH=qs[2], q_sM=qs[3], k_sB=ks[0], k_sT=ks[1], k_sH=ks[2], k_sM=ks[3],
-                              v_sB=vs[0], v_sT=vs[1], v_sH=vs[2], lam_sB=ls[0], lam_sT=ls[1], lam_sH=ls[2],
-                              mask=_ptr(mask), m_sB=m[0], m_sQ=m[1], m_sK=m[2], lengths=_ptr(lengths), q_start=_ptr(q_start),
-                              B=B, Tq=Tq, Tk=Tk, H=H, G=G, d=hd, dv=dv, type=TYPES[q.dtype], causal=int(causal),
+                              mask=_ptr(mask), lengths=_ptr(lengths), q_start=_ptr(q_start), B=B, Tq=Tq, Tk=Tk, H=H, G=G, d=hd, dv=dv, type=TYPES[q.dtype], causal=int(causal),
                               mask_form=0 if mask is None else mask.dim() - 1,
                               mask_float=int(mask is not None and mask.dtype == torch.float32), scale=scale)
+        _strides(d, qp, kp, vp, lam, mask)
         ws = _workspace('mep_diff_attn_workspace', d, dev)
         d.workspace = _ptr(ws)
         _launch('mep_diff_attn_fwd', d, dev)
         if keep:
             ctx.set_materialize_grads(False)
-            ctx.save_for_backward(mask, lengths, q_start, q, k, v, lam, out)
-            # what the descriptor points to besides: the packed copies where there are any, and the row statistics
-            ctx.held = [t for t, x in ((qp, q), (kp, k), (vp, v)) if t is not x] + [stats, second]
-            ctx.desc = d
+            saved = (mask, lengths, q_start, qp, kp, vp, lam, out, stats, second)
+            ctx.save_for_backward(*saved)
+            ctx.desc, ctx.places = d, _places(saved)
         return out
 
     @staticmethod
@@ -380,19 +405,26 @@ class _DiffAttnFn(torch.autograd.Function):
     def backward(ctx, dout):
         if dout is None:
             return (None,) * 8
-        q, k, v, lam = ctx.saved_tensors[3:7]      # (unpacking checks that none was written in between)
+        saved, d = ctx.saved_tensors, ctx.desc
+        if _places(saved) != ctx.places:
+            mask, lengths, q_start, q, k, v, lam, out, stats, second = saved
+            q, k, v = _packed(q, d.H // d.G), _packed(k), _packed(v)
+            saved = (mask, lengths, q_start, q, k, v, lam, *(t.contiguous() for t in (out, stats, second)))
+            d = _moved(d, ('mask', 'lengths', 'q_start', 'q', 'k', 'v', 'lam', 'out', 'stats', 'second'), saved)
+            _strides(d, q, k, v, lam, mask)
+        lam = saved[6]
         need = ctx.needs_input_grad
-        B, Tq, H, _, _ = q.shape
-        dev = q.device
-        dout = _packed(dout, H // k.shape[2])
-        like = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
-        dq = like(q) if need[4] else None
-        dk, dv = (like(k), like(v)) if need[5] or need[6] else (None, None)
-        dlam = like(lam) if need[7] else None
+        B, Tq, Tk, H, G = d.B, d.Tq, d.Tk, d.H, d.G
+        dev = lam.device
+        dout = _packed(dout, H // G)
+        new = lambda *shape: torch.empty(shape, dtype=dout.dtype, device=dev)  # noqa: E731
+        dq = new(B, Tq, H, 2, d.d) if need[4] else None
+        dk, dv = (new(B, Tk, G, 2, d.d), new(B, Tk, G, d.dv)) if need[5] or need[6] else (None, None)
+        dlam = torch.empty(lam.shape, dtype=torch.float32, device=dev) if need[7] else None
         delta = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev)
         shared = lam.dim() == 1
-        ws = _workspace('mep_diff_attn_bwd_workspace', ctx.desc, dev) if dk is not None else None
-        bd = _lib.DiffAttnBwdDesc(f=ctx.desc, dout=_ptr(dout), o_sB=dout.stride(0), o_sT=dout.stride(1), o_sH=dout.stride(2),
+        ws = _workspace('mep_diff_attn_bwd_workspace', d, dev) if dk is not None else None
+        bd = _lib.DiffAttnBwdDesc(f=d, dout=_ptr(dout), o_sB=dout.stride(0), o_sT=dout.stride(1), o_sH=dout.stride(2),
                                   dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlam=_ptr(dlam) if shared else 0,
                                   dlam_rows=0 if shared else _ptr(dlam), delta=_ptr(delta), workspace=_ptr(ws))
         _launch('mep_diff_attn_bwd', bd, dev)
@@ -434,10 +466,12 @@ def diff_attention(q, k, v, lam, *, mask=None, lengths=None, causal=False, q_sta
     for t, n in ((lengths, 'lengths'), (q_start, 'q_start')):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
             raise ValueError('%s must be contiguous int32 [B]; got %s %s' % (n, tuple(t.shape), t.dtype))
+    if mask is not None and mask.requires_grad:
+        raise ValueError('a mask has no gradient')
     if q_start is not None and not causal:
         raise ValueError('q_start places the queries of a causal call; causal is False')
     scale = hd ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 1e6:
         raise ValueError('scale must be positive and at most 1e6; got %r' % (scale,))
     _on_device(q, k, v, lam, mask, lengths, q_start)
-    return _DiffAttnFn.apply((bool(causal), scale), mask, lengths, q_start, q, k, v, lam)
+    return _DiffAttnFn.apply((bool(causal), scale, torch.is_grad_enabled()), mask, lengths, q_start, q, k, v, lam)

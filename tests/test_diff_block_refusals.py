@@ -141,3 +141,18 @@ def test_descriptors_refused_before_any_launch():
         assert _refused('mep_pack_rows', _lib.PackRowsDesc(**dict(dict(B=1, T=1, H=1, M=1, n=8), **kw))), kw
     for kw in (dict(), dict(dout=16), dict(dout=16, delta=16, dk=16), dict(dout=8, delta=16)):
         assert _refused('mep_diff_attn_bwd', _lib.DiffAttnBwdDesc(f=attn(stats=16, second=16), **kw)), kw
+
+
+def test_what_has_no_gradient_is_refused():
+    with pytest.raises(ValueError, match='freqs'):
+        db.rotary(t(1, 3, 2, 8), positions=POS, freqs=FREQS.clone().requires_grad_())
+    with pytest.raises(ValueError, match='mask'):
+        db.diff_attention(t(1, 3, 2, 2, 8), t(1, 3, 2, 2, 8), t(1, 3, 2, 8), t(2), mask=t(1, 3).requires_grad_())
+
+
+def test_strides_whose_sum_passes_2_gib():
+    """each stride is within its limit, but a tile's farthest element of fp32 is not"""
+    strides = dict(q_sT=64, q_sH=(1 << 28) // 64 - 64, q_sM=(1 << 28) - 64)
+    assert (64 * 64 + 64 * strides['q_sH'] + strides['q_sM']) * 4 >= (1 << 31) - 2048
+    assert _refused('mep_diff_attn_fwd', _lib.DiffAttnDesc(q=16, k=16, v=16, lam=16, out=16, B=1, Tq=1, Tk=1, H=64, G=1, d=8, dv=8,
+                                                           scale=1.0, **strides))
