@@ -324,23 +324,44 @@ struct Job {
 };
 // Workgroups go round the 8 XCDs by their index; where the (batch, key head) pairs divide evenly over them, a pair's blocks
 // stay on one XCD (or on a few, in turn), so that its keys are read into one L2.
-MEP_DEV Job make_job(const mep_diff_attn_desc& d, int blocks, bool reverse) {
+// Causal calls: the blocks differ by up to their number in length, and all pairs' longest come first.  Where two workgroups share a
+// compute unit (`shared`) and both halves of the first 512 are there from the start, the second half goes the other way, so that
+// the longest shares its unit with the shortest (B 2, T 4096, 8 heads, 64 / 128: forward FWD_OLD us pair by pair).
+enum Order { IN_TURN, FIRST_LONGEST, LAST_LONGEST };
+MEP_DEV Job make_job(const mep_diff_attn_desc& d, int blocks, Order order, bool shared) {
     Job j;
     const int x = blockIdx.x, bgs = d.B * d.G;
+    // position s of n on one XCD of 8, or in all; the 32 / 256 units' second ones the other way
+    auto turn = [&](int s, int n, int units) {
+        const int last = min(n, 2 * units) - 1;
+        return shared && s >= units && s <= last ? units + last - s : s;
+    };
     int bg;
     if (bgs % 8 == 0) {
-        const int s = x >> 3, q = s / blocks;
-        bg = q * 8 + (x & 7);
-        j.block = s - q * blocks;
+        const int q = bgs / 8;
+        bg = x & 7;
+        if (order == IN_TURN) {
+            const int s = x >> 3, p = s / blocks;
+            bg += p * 8;
+            j.block = s - p * blocks;
+        } else {
+            const int s = turn(x >> 3, blocks * q, 32);
+            j.block = s / q;
+            bg += (s - j.block * q) * 8;
+        }
     } else if (8 % bgs == 0 && blocks % (8 / bgs) == 0) {
-        const int per = 8 / bgs;
+        const int per = 8 / bgs, s = order == IN_TURN ? x >> 3 : turn(x >> 3, blocks / per, 32);
         bg = (x & 7) / per;
-        j.block = (x >> 3) * per + (x & 7) % per;
-    } else {
+        j.block = s * per + (x & 7) % per;
+    } else if (order == IN_TURN) {
         bg = x / blocks;
         j.block = x - bg * blocks;
+    } else {
+        const int s = turn(x, blocks * bgs, 256);
+        j.block = s / bgs;
+        bg = s - j.block * bgs;
     }
-    if (reverse) j.block = blocks - 1 - j.block;      // causal: the longest blocks start first
+    if (order == LAST_LONGEST) j.block = blocks - 1 - j.block;
     j.b = bg / d.G;
     j.g = bg - j.b * d.G;
     j.n = d.H / d.G;
@@ -582,6 +603,7 @@ struct Online {
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) s1[r] = fmaf(s1[r], f1, -f2 * s2[r]);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < Ge::NP; ++i) {
             const Frag p = acc_frag<M>(s1, i), e = acc_frag<M>(s2, i);
@@ -593,6 +615,7 @@ struct Online {
                     y[n] = M::mma(v, e, y[n]);
                 }
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     // the maxima that the backward gets, and 2^(m - those)
     MEP_DEV void maxima(float& n1, float& n2, float& g1, float& g2) const {      // (one rounding, as m1, m2: without keys g = 1)
@@ -613,7 +636,7 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_
     constexpr int KT = Ge::KT;
     __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
     const int ld = d.dv;
-    Job j = make_job(d, blocks * parts, d.causal);
+    Job j = make_job(d, blocks * parts, d.causal ? LAST_LONGEST : IN_TURN, !da_wide(TYPE, DK));
     if (DV == 128 && parts == 2) {
         const int c = j.block % 2 * DV;
         j.block /= 2;
@@ -692,7 +715,7 @@ __global__ __launch_bounds__(128, DV >= 128 || DK >= 128 || TYPE == MEP_F32 ? 1 
     typedef typename Ge::T T;
     constexpr int KT = da_split_keys(TYPE, DK, DV), KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;
     __shared__ __align__(16) T Buf[2 * TSZ];
-    const Job j = make_job(d, blocks * splits, false);
+    const Job j = make_job(d, blocks * splits, IN_TURN, false);
     const int wave = threadIdx.x >> 6, h = (threadIdx.x & 63) >> 5;
     const int rb = j.block / splits, split = j.block - rb * splits;
     const Rows32 w(d, j, rb * 32);
@@ -779,7 +802,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
     constexpr int KT = Ge::KT;
     const mep_diff_attn_desc& d = bd.f;
     __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
-    const Job j = make_job(d, blocks, d.causal);
+    const Job j = make_job(d, blocks, d.causal ? LAST_LONGEST : IN_TURN, !da_wide(TYPE, DK));
     const int h = (threadIdx.x & 63) >> 5;
     const Rows32 w(d, j, j.block * DA_ROWS + (threadIdx.x >> 6) * 32);
     const KeyTiles<TYPE, DK, DV> keys(d, j);
@@ -866,6 +889,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
 #pragma unroll
                     for (int i = n; i < n + Ge::STEP; ++i) dp = M::mma(vread.rows(vt, 32 * sub, i), g.at(i), dp);
                 }
+            __builtin_amdgcn_s_setprio(1);
             if (on != ~0u || ks + 32 > w.wfull || d.mask_form == 2) mask_keys(d, j, ks, on, w.t, s1, s2);
             float u1 = 0.f, u2 = 0.f;
 #pragma unroll
@@ -915,6 +939,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
                     }
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
         }
     }
     sum1 = half_sum(sum1) * st[1];
@@ -1054,7 +1079,7 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
     __shared__ __align__(16) float Rs[2][PARTS ? 1 : (int)R_COUNT][PARTS ? 1 : RT];
     __shared__ int Ts[2][RT];                     // and queries
     __shared__ int Neg[2];                        // whether any lam of the tile is negative
-    Job j = make_job(d, blocks * splits, false);
+    Job j = make_job(d, blocks * splits, d.causal ? FIRST_LONGEST : IN_TURN, Sh::THREADS <= 256 && !da_wide(TYPE, DK));
     const int split = j.block % splits;
     j.block /= splits;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
