@@ -322,6 +322,15 @@ struct Job {
     int b, g, block, n;          // batch row, key head, block of rows or keys, heads per key head
     int rows, len, first;        // Tq n; allowed keys are below len; causal: key <= first + query
 };
+MEP_DEV void fill_job(const mep_diff_attn_desc& d, Job& j) {
+    j.n = d.H / d.G;
+    j.rows = d.Tq * j.n;
+    j.len = d.Tk;
+    if (d.lengths) j.len = max(0, min(j.len, G<const int>(d.lengths)[j.b]));
+    j.first = d.Tk - d.Tq;
+    if (d.q_start) j.first = max(-(1 << 30), min(1 << 30, G<const int>(d.q_start)[j.b]));
+    if (d.causal) j.len = max(0, min(j.len, j.first + d.Tq));     // what no query sees is never read
+}
 // Workgroups go round the 8 XCDs by their index; where the (batch, key head) pairs divide evenly over them, a pair's blocks
 // stay on one XCD (or on a few, in turn), so that its keys are read into one L2.
 // Causal calls: the blocks differ by up to their number in length, and all pairs' longest come first.  Where two workgroups share a
@@ -364,13 +373,7 @@ MEP_DEV Job make_job(const mep_diff_attn_desc& d, int blocks, Order order, bool 
     if (order == LAST_LONGEST) j.block = blocks - 1 - j.block;
     j.b = bg / d.G;
     j.g = bg - j.b * d.G;
-    j.n = d.H / d.G;
-    j.rows = d.Tq * j.n;
-    j.len = d.Tk;
-    if (d.lengths) j.len = max(0, min(j.len, G<const int>(d.lengths)[j.b]));
-    j.first = d.Tk - d.Tq;
-    if (d.q_start) j.first = max(-(1 << 30), min(1 << 30, G<const int>(d.q_start)[j.b]));
-    if (d.causal) j.len = max(0, min(j.len, j.first + d.Tq));     // what no query sees is never read
+    fill_job(d, j);
     return j;
 }
 // keys that any of the queries up to t may see
@@ -701,88 +704,171 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_
 }
 
 // ------------------------------------------------------------------ forward over split keys
-// Few rows against many keys (single tokens against a cache): a workgroup of two waves takes 32 rows and some tiles of 64
-// keys (32 where two of 64 do not fit LDS), a wave the even or the odd 32 of them, and each wave leaves its row maxima, sums, E_1
-// and E_2 in fp32; k_diff_join joins them.  Bound by reading the keys and values once: two tiles in flight in each of two workgroups
-// on a compute unit.
-// workspace of a wave's 32 rows: (m1, l1, m2, l2)[32], E_1 [32][dv], E_2 [32][dv]
-MEP_DEV int64_t split_floats(int dv) { return 32 * (4 + 2 * (int64_t)dv); }
+// Few rows against many keys (single tokens against a cache).  The tiles of keys of all (batch row, key head, 32 rows) stand in one
+// row, those behind a batch row's length left out, and each of `groups` workgroups takes an equal share of it: equal work whatever
+// the lengths (B 32 of up to 8192 keys, 4 key heads: 81 us, against 105 with as many tiles to a workgroup in each batch row's own
+// splits), neighbouring shares on one XCD; to begin with the next rows counts as DA_SPLIT_START tiles (87 us without).  A workgroup has two waves; of a tile of 64 keys (32 where two of 64 do not fit LDS: of every
+// other tile) a wave takes 32, and for each batch row it comes to it leaves its rows' maxima, sums, E_1 and E_2 in fp32;
+// k_diff_join joins them.  Bound by reading the keys and values once: two tiles in flight in each of two workgroups on a compute unit.
+// workspace: the number of tiles before each batch row, int [B + 1]; then a part for each wave of each (workgroup, (batch row, key head,
+// 32 rows)) that meet, at workgroup + (batch row, key head, 32 rows): (m1, l1, m2, l2) [R], E_1 [R][dv], E_2 [R][dv], R = min(32, rows)
+constexpr int DA_SPLIT_THREADS = 128, DA_SPLIT_START = 3;
+constexpr bool da_split_full(int type, int dk, int dv) { return dv >= 128 || dk >= 128 || type == MEP_F32; }      // all registers of a SIMD
+constexpr int da_split_groups(int type, int dk, int dv) {      // that are on the chip at a time
+    const int lds = (type == MEP_F32 ? 4 : 2) * 2 * da_split_keys(type, dk, dv) * (2 * dk + dv), fit = 160 * 1024 / lds, waves = da_split_full(type, dk, dv) ? 2 : 4;
+    return 256 * (fit < waves ? fit : waves);
+}
+constexpr int64_t split_floats(int rows, int dv) { return (rows * (4 + 2 * (int64_t)dv) + 3) / 4 * 4; }
+struct Parts {
+    int64_t tiles, share, stride;      // in all; a workgroup's; floats of a part
+    int per;                           // (key head, 32 rows) of a batch row
+    gfloat* first;
+};
+MEP_DEV Parts parts_of(const mep_diff_attn_desc& d, int blocks, int groups, int before_end) {
+    Parts p;
+    p.per = d.G * blocks;
+    p.tiles = (int64_t)before_end * p.per;
+    p.share = max((p.tiles + groups - 1) / groups, (int64_t)4);      // 4 tiles at least: a part costs as much as one
+    p.stride = split_floats(min(32, d.Tq * (d.H / d.G)), d.dv);
+    p.first = G<float>(d.workspace) + (d.B + 4) / 4 * 4;
+    return p;
+}
 
 template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(128, DV >= 128 || DK >= 128 || TYPE == MEP_F32 ? 1 : 2) void k_diff_split(mep_diff_attn_desc d, int blocks, int splits, int tiles) {
+__global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 : 2) void k_diff_split(mep_diff_attn_desc d, int blocks, int groups) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
     constexpr int KT = da_split_keys(TYPE, DK, DV), KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;
     __shared__ __align__(16) T Buf[2 * TSZ];
-    const Job j = make_job(d, blocks * splits, IN_TURN, false);
-    const int wave = threadIdx.x >> 6, h = (threadIdx.x & 63) >> 5;
-    const int rb = j.block / splits, split = j.block - rb * splits;
-    const Rows32 w(d, j, rb * 32);
-    const int end = min(w.wend, (split + 1) * tiles * KT), begin = split * tiles * KT;
-    const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
-    const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
+    __shared__ int At[4];                        // the first wave's tiles; all; the first batch row of this share, the tiles before it
+    const int tid = threadIdx.x, wave = tid >> 6, h = (tid & 63) >> 5;
+    // groups is a multiple of 8
+    const int self = (int)(blockIdx.x & 7) * (groups >> 3) + (int)(blockIdx.x >> 3);
+    auto tiles_of = [&](int b) {
+        Job r;
+        r.b = b;
+        fill_job(d, r);
+        return r.len > 0 ? (r.len + KT - 1) / KT + DA_SPLIT_START : 0;
+    };
+    // the tiles before each batch row: a thread sums some rows', the threads' sums are summed up
+    const int rows_each = (d.B + DA_SPLIT_THREADS - 1) / DA_SPLIT_THREADS, b0 = min(d.B, tid * rows_each), b1 = min(d.B, b0 + rows_each);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    int upto = mine;
+    for (int o = 1; o < 64; o *= 2) {
+        const int x = __shfl_up(upto, o);
+        if ((tid & 63) >= o) upto += x;
+    }
+    if (tid == 63) At[0] = upto;
+    __syncthreads();
+    if (wave) upto += At[0];
+    if (tid == DA_SPLIT_THREADS - 1) At[1] = upto;
+    __syncthreads();
+    const Parts parts = parts_of(d, blocks, groups, __builtin_amdgcn_readfirstlane(At[1]));
+    const int64_t start = self * parts.share, stop = min(start + parts.share, parts.tiles);
+    const bool some = start < stop;
+    const int first_tile = some ? (int)(start / parts.per) : 0;      // of the batch rows' tiles
+    int before = upto - mine;
+    for (int b = b0; b < b1; ++b) {
+        const int n = tiles_of(b);
+        if (self == 0) G<int>(d.workspace)[b] = before;
+        if (some && before <= first_tile && first_tile < before + n) {
+            At[2] = b;
+            At[3] = before;
+        }
+        before += n;
+    }
+    if (self == 0 && tid == DA_SPLIT_THREADS - 1) G<int>(d.workspace)[d.B] = upto;
+    if (!some) return;
+    __syncthreads();
+
     const Reader<M, 2 * DK> kread;
     const Reader<M, DV> vread;
-    auto load = [&](T* tile, int k0, unsigned long long bits) {
-        const int tid = thread_again();
-        const Stager<M, KT, 2 * DK, 128> ks(tid, (unsigned)d.k_sT, [&](int ch) {
-            const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
-            return col < d.d ? col + (m ? (int)d.k_sM : 0) : -1;
-        });
-        ks.load(tile, kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
-        const Stager<M, KT, DV, 128> vs(tid, (unsigned)d.v_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
-        vs.load(tile + KSZ, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
-    };
-    unsigned raw = key_raw(d, j, begin);
-    unsigned long long bits = key_bits(d, j, begin, KT, raw);
-    if (begin < end) load(Buf, begin, bits);
-    raw = key_raw(d, j, begin + KT);
-    Online<TYPE, DK, DV> o(d, j, w);
-    for (int k0 = begin, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
-        tile_sync();
-        const unsigned long long now = bits;
-        if (k0 + KT < end) {
-            bits = key_bits(d, j, k0 + KT, KT, raw);
-            load(Buf + (buf ^ 1) * TSZ, k0 + KT, bits);
-            raw = key_raw(d, j, k0 + 2 * KT);
+    int b = __builtin_amdgcn_readfirstlane(At[2]);
+    before = __builtin_amdgcn_readfirstlane(At[3]);
+    for (int64_t at = start; at < stop && b < d.B;) {
+        const int n = __builtin_amdgcn_readfirstlane(tiles_of(b));
+        const int64_t in = at - (int64_t)before * parts.per;
+        if (in >= (int64_t)n * parts.per) {
+            before += n;
+            ++b;
+            continue;
         }
-        const int sub = KT == 64 ? wave : 0, ks = k0 + 32 * sub;      // one sub-tile a tile: the waves take turns
-        const unsigned on = (unsigned)(now >> (32 * sub));
-        if ((KT == 64 || ((k0 - begin) / KT & 1) == wave) && ks < end && on)
-            o.step(d, j, w, kread, vread, Buf + buf * TSZ, Buf + buf * TSZ + KSZ, 32 * sub, ks, on);
+        const int item = (int)(in / n), from = (int)(in - (int64_t)item * n), to = (int)min((int64_t)n, from + (stop - at));
+        const int tile0 = max(0, from - DA_SPLIT_START), tile1 = to - DA_SPLIT_START;
+        at += to - from;
+        if (tile0 >= tile1) continue;
+        Job j;
+        j.b = b;
+        j.g = item / blocks;
+        j.block = item - j.g * blocks;
+        fill_job(d, j);
+        const Rows32 w(d, j, j.block * 32);
+        const int begin = tile0 * KT, end = min(w.wend, tile1 * KT);
+        const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
+        const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
+        auto load = [&](T* tile, int k0, unsigned long long bits) {
+            const int tid = thread_again();
+            const Stager<M, KT, 2 * DK, DA_SPLIT_THREADS> ks(tid, (unsigned)d.k_sT, [&](int ch) {
+                const int m = ch >= DK / M::E, col = ch * M::E - m * DK;
+                return col < d.d ? col + (m ? (int)d.k_sM : 0) : -1;
+            });
+            ks.load(tile, kp + k0 * d.k_sT, (unsigned)d.k_sT, bits);
+            const Stager<M, KT, DV, DA_SPLIT_THREADS> vs(tid, (unsigned)d.v_sT, [&](int ch) { return ch * M::E < d.dv ? ch * M::E : -1; });
+            vs.load(tile + KSZ, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
+        };
+        unsigned raw = key_raw(d, j, begin);
+        unsigned long long bits = key_bits(d, j, begin, KT, raw);
+        if (begin < end) load(Buf, begin, bits);
+        raw = key_raw(d, j, begin + KT);
+        Online<TYPE, DK, DV> o(d, j, w);
+        for (int k0 = begin, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
+            tile_sync();
+            const unsigned long long now = bits;
+            if (k0 + KT < end) {
+                bits = key_bits(d, j, k0 + KT, KT, raw);
+                load(Buf + (buf ^ 1) * TSZ, k0 + KT, bits);
+                raw = key_raw(d, j, k0 + 2 * KT);
+            }
+            const int sub = KT == 64 ? wave : 0, ks = k0 + 32 * sub;      // one sub-tile a tile: the waves take turns
+            const unsigned on = (unsigned)(now >> (32 * sub));
+            if ((KT == 64 || ((k0 - begin) / KT & 1) == wave) && ks < end && on)
+                o.step(d, j, w, kread, vread, Buf + buf * TSZ, Buf + buf * TSZ + KSZ, 32 * sub, ks, on);
+        }
+        tile_sync();                             // the tiles are free for the next batch row's
+        float n1, n2, g1, g2;
+        o.maxima(n1, n2, g1, g2);
+        const float l1 = half_sum(o.l1) * g1, l2 = half_sum(o.l2) * g2;
+        gfloat* part = parts.first + ((self + (int64_t)b * parts.per + item) * 2 + wave) * parts.stride;
+        const int row = tid & 31, rows = min(32, j.rows);
+        if (w.live && h == 0) *reinterpret_cast<MEP_G f32x4*>(part + 4 * row) = f32x4{n1, l1, n2, l2};
+        if (w.live && (l1 != 0.f || l2 != 0.f)) {      // without a key of this row here the join reads no further
+            const float fx = g1 / o.f1;
+            gfloat* e1 = part + 4 * rows + row * d.dv;
+            gfloat* e2 = e1 + rows * d.dv;
+#pragma unroll
+            for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int col = 32 * n + acc_off(r) + 4 * h;
+                    float a[4], b[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        a[e] = fmaf(o.f2, o.y[n][r + e], o.x[n][r + e]) * fx;
+                        b[e] = o.y[n][r + e] * g2;
+                    }
+                    if (col + 4 <= d.dv) {
+                        store_f32<float, 4>(e1 + col, a);
+                        store_f32<float, 4>(e2 + col, b);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (col + e < d.dv) { e1[col + e] = a[e]; e2[col + e] = b[e]; }
+                    }
+                }
+        }
     }
-    float n1, n2, g1, g2;
-    o.maxima(n1, n2, g1, g2);
-    const float l1 = half_sum(o.l1) * g1, l2 = half_sum(o.l2) * g2;
-    gfloat* part = G<float>(d.workspace) + ((((int64_t)j.b * d.G + j.g) * blocks + rb) * splits * 2 + split * 2 + wave) * split_floats(d.dv);
-    if (!w.live) return;
-    const int row = threadIdx.x & 31;
-    if (h == 0) *reinterpret_cast<MEP_G f32x4*>(part + 4 * row) = f32x4{n1, l1, n2, l2};
-    if (!(l1 != 0.f || l2 != 0.f)) return;      // no key of this row here: the join reads no further
-    const float fx = g1 / o.f1;
-    gfloat* e1 = part + 128 + row * d.dv;
-    gfloat* e2 = e1 + 32 * d.dv;
-#pragma unroll
-    for (int n = 0; n < DV / 32; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int col = 32 * n + acc_off(r) + 4 * h;
-            float a[4], b[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[e] = fmaf(o.f2, o.y[n][r + e], o.x[n][r + e]) * fx;
-                b[e] = o.y[n][r + e] * g2;
-            }
-            if (col + 4 <= d.dv) {
-                store_f32<float, 4>(e1 + col, a);
-                store_f32<float, 4>(e2 + col, b);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < d.dv) { e1[col + e] = a[e]; e2[col + e] = b[e]; }
-            }
-        }
 }
 
 // ------------------------------------------------------------------ backward: D and dq
@@ -1382,9 +1468,9 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
 constexpr int da_kw(int type, int dk) { return dk >= 128 && type != MEP_F32 ? 2 : 4; }
 
 template <int TYPE, int DK, int DV>
-void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st) {      // (splits: DA_FWD's parts)
+void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st) {      // splits: DA_FWD's parts, DA_SPLIT's groups
     if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
-    else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(128), 0, st, d, blocks, splits, tiles);
+    else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_SPLIT_THREADS), 0, st, d, blocks, splits);
     else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
                             dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks, splits);
@@ -1398,18 +1484,18 @@ inline int da_value_width(int d, int dv) {
     return dk == 32 ? (dv <= 32 ? 32 : 64) : dk == 64 ? (dv <= 64 ? 64 : 128) : (dv <= 128 ? 128 : 256);
 }
 template <int TYPE>
-void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all) {
+void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all) {
     const int dk = da_width(d.d, all), dv = da_value_width(d.d, all);      // all: the values' whole width
-    if (dk == 32 && dv == 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, splits, tiles, st);
-    else if (dk == 32) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, splits, tiles, st);
-    else if (dk == 64 && dv == 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, splits, tiles, st);
-    else if (dk == 64) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, splits, tiles, st);
-    else if (dv == 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, splits, tiles, st);
-    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, splits, tiles, st);
+    if (dk == 32 && dv == 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, splits, st);
+    else if (dk == 32) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, splits, st);
+    else if (dk == 64 && dv == 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, splits, st);
+    else if (dk == 64) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, splits, st);
+    else if (dv == 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, splits, st);
+    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, splits, st);
 }
 
-void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all);
-void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all);
-void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all);
+void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all);
+void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all);
+void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all);
 
 }  // namespace mep

@@ -1,4 +1,6 @@
 // mep_diff_attn_fwd / _bwd: checks, launch geometry and the join of lam's gradient (kernels: diff_attn.h).
+#include <cfloat>
+
 #include "diff_attn.h"
 
 namespace {
@@ -36,18 +38,24 @@ __global__ __launch_bounds__(DLAM_THREADS) void k_diff_dlam(mep_diff_attn_bwd_de
 
 // out = E_1 / l_1 - lam E_2 / l_2 of a row from its parts: a thread per value channel, rows side by side in a workgroup.  Bound by the
 // latency of its loads: the parts' statistics are read a part a lane, and the sums of 8 parts are in flight.
-__global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, int blocks, int parts, int per, int ld) {
+__global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, int blocks, int groups, int per, int ld) {
     const int ch = threadIdx.x % per, lanes = min(per, 64), lane = threadIdx.x % lanes;
     const int64_t all = (int64_t)d.B * d.Tq * d.H, at = (int64_t)blockIdx.x * (DA_THREADS / per) + threadIdx.x / per;
     const int64_t r = min(at, all - 1);      // (b, t, head); lanes without a row work on the last one and write nothing
     const int64_t bt = r / d.H;
     const int head = (int)(r - bt * d.H), b = (int)(bt / d.Tq), t = (int)(bt - (int64_t)b * d.Tq);
-    const int n = d.H / d.G, g = head / n, row = t * n + head - g * n;
-    const int64_t stride = split_floats(d.dv);
-    const gfloat* part = G<const float>(d.workspace) + (((int64_t)b * d.G + g) * blocks + row / 32) * parts * stride;
+    const int n = d.H / d.G, g = head / n, row = t * n + head - g * n, rows = min(32, d.Tq * n);
+    const int* before = reinterpret_cast<const int*>(d.workspace);
+    const Parts ps = parts_of(d, blocks, groups, before[d.B]);
+    // the row's tiles are tile .. tile + tiles - 1 of all
+    const int item = g * blocks + row / 32, tiles = before[b + 1] - before[b];
+    const int64_t tile = (int64_t)before[b] * ps.per + (int64_t)item * tiles, w0 = (tile + DA_SPLIT_START) / ps.share;
+    const int parts = tiles ? 2 * (int)((tile + tiles - 1) / ps.share - w0 + 1) : 0;
+    const int64_t stride = ps.stride;
+    const gfloat* part = ps.first + (w0 + (int64_t)b * ps.per + item) * 2 * stride;
     const int lr = row & 31;
     auto stats = [&](int p) { return *reinterpret_cast<const MEP_G f32x4*>(part + p * stride + 4 * lr); };
-    float m1 = -INFINITY, m2 = -INFINITY;
+    float m1 = -FLT_MAX, m2 = -FLT_MAX;      // (without keys the backward gets finite ones)
     for (int p = lane; p < parts; p += lanes) {
         const f32x4 s = stats(p);
         m1 = fmaxf(m1, s[0]);
@@ -58,8 +66,8 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, 
         m2 = fmaxf(m2, __shfl_xor(m2, o));
     }
     float l1 = 0.f, l2 = 0.f, e1 = 0.f, e2 = 0.f;
-    const gfloat* v1 = part + 128 + lr * d.dv + min(ch, d.dv - 1);
-    const gfloat* v2 = v1 + 32 * d.dv;
+    const gfloat* v1 = part + 4 * rows + lr * d.dv + min(ch, d.dv - 1);
+    const gfloat* v2 = v1 + rows * d.dv;
     for (int p0 = 0; p0 < parts; p0 += lanes) {
         float w1 = 0.f, w2 = 0.f;
         bool on = false;                          // without a key of this row there, no sums are written
@@ -144,33 +152,32 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_kv_join(mep_diff_attn_bwd_d
     }
 }
 
-// How the keys of a forward are split, or splits = 0: not at all.  Worth it where the rows are few: up to 32 a (batch, key head) leave
-// three of k_diff_fwd's four waves idle (against a row of 8192 keys, 32 batch rows, 4 key heads: 297 us whole, see k_diff_split),
-// and more rows too when their workgroups are under half the compute units and there are 1024 keys.  Then 8 workgroups
-// a compute unit at most, and 4 tiles each at least.
-struct Split { int blocks, splits, tiles; };
+// Whether the keys of a forward are split (groups > 0), and over how many workgroups.  Worth it where the rows are few: up to 32 a
+// (batch row, key head) leave three of k_diff_fwd's four waves idle (against a row of 8192 keys, 32 batch rows, 4 key heads: 297 us
+// whole, 84 split and joined), and more rows too when their workgroups are under a quarter of the compute units and there are 1024 keys
+// (16 / 32 bf16, 64 workgroups: 36 us whole, 38 split).  As many workgroups as are on the chip at a time, and 4 tiles for each.
+struct Split { int blocks, groups; };
 Split split_of(const mep_diff_attn_desc& d) {
-    Split s = {0, 0, 0};
+    Split s = {0, 0};
     const int64_t rows = (int64_t)d.Tq * (d.H / d.G), pairs = (int64_t)d.B * d.G;
     const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) < 64;
     if (pairs == 0 || rows == 0 || !(few || none)) return s;
     s.blocks = (int)((rows + 31) / 32);
-    const int kt = da_split_keys(d.type, da_width(d.d, d.dv), da_piece(da_value_width(d.d, d.dv))), all = (d.Tk + kt - 1) / kt;
-    const int64_t want = 2048 / (pairs * s.blocks);
-    s.splits = (int)(want < 1 ? 1 : want > (all + 3) / 4 ? (all + 3) / 4 : want);
-    s.tiles = (all + s.splits - 1) / s.splits;
-    s.splits = (all + s.tiles - 1) / s.tiles;
-    if (pairs * s.blocks * s.splits >= 1 << 23) s.splits = 0;
+    const int dk = da_width(d.d, d.dv), dv = da_piece(da_value_width(d.d, d.dv)), kt = da_split_keys(d.type, dk, dv);
+    const int64_t items = pairs * s.blocks, all = (d.Tk + kt - 1) / kt, want = (items * all + 3) / 4, most = da_split_groups(d.type, dk, dv);
+    if (items >= 1 << 20 || d.B * (all + DA_SPLIT_START) >= INT_MAX) return s;      // there are enough rows, or too many tiles to count in 32 bits
+    s.groups = (int)((want < most ? want : most) + 7) / 8 * 8;
     return s;
 }
 int64_t split_bytes(const mep_diff_attn_desc& d, const Split& s) {
-    return (int64_t)d.B * d.G * s.blocks * s.splits * 2 * 32 * (4 + 2 * (int64_t)d.dv) * 4;
+    const int64_t rows = (int64_t)d.Tq * (d.H / d.G), parts = s.groups + (int64_t)d.B * d.G * s.blocks;
+    return ((d.B + 4) / 4 * 4 + parts * 2 * split_floats((int)(rows < 32 ? rows : 32), da_piece(d.dv))) * 4;
 }
 
-void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, int tiles, hipStream_t st, int dv) {
-    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
-    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
-    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, tiles, st, dv);
+void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, hipStream_t st, int dv) {
+    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, st, dv);
+    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, st, dv);
+    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, st, dv);
 }
 
 // Into how many workgroups the rows of a block of keys are split: until there are two for every compute unit, 4 tiles of rows each at
@@ -250,10 +257,10 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     hipStream_t st = (hipStream_t)stream;
     const Split s = split_of(d);
     const int es = d.type == MEP_F32 ? 4 : 2, half = da_piece(d.dv);
-    if (!s.splits || !d.workspace) {
+    if (!s.groups || !d.workspace) {
         const int parts = d.dv > half ? 2 : 1;
         if (grid * parts >= 1 << 23) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
-        run(DA_FWD, d, nullptr, grid * parts, blocks, parts, 0, st, d.dv);
+        run(DA_FWD, d, nullptr, grid * parts, blocks, parts, st, d.dv);
         return mep_check_launch("mep_diff_attn_fwd");
     }
     // values of more than 128 channels in two launches: their accumulators would not fit beside each other
@@ -264,11 +271,11 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
         p.out += (uint64_t)c * es;
         if (p.second) p.second += (uint64_t)c * es;
         if (c) p.stats = 0;
-        run(DA_SPLIT, p, nullptr, (int64_t)s.blocks * s.splits * d.B * d.G, s.blocks, s.splits, s.tiles, st, d.dv);
+        run(DA_SPLIT, p, nullptr, s.groups, s.blocks, s.groups, st, d.dv);
         int per = 32;
         while (per < p.dv) per *= 2;
         const int64_t rows = (int64_t)d.B * d.Tq * d.H, side = DA_THREADS / per;
-        hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, p, s.blocks, 2 * s.splits, per, d.dv);
+        hipLaunchKernelGGL(k_diff_join, dim3((unsigned)((rows + side - 1) / side)), dim3(DA_THREADS), 0, st, p, s.blocks, s.groups, per, d.dv);
         const int rc = mep_check_launch("mep_diff_attn_fwd");
         if (rc) return rc;
     }
@@ -284,7 +291,7 @@ extern "C" int64_t mep_diff_attn_bwd_workspace(const mep_diff_attn_desc* desc) {
 extern "C" int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc) {
     if (!desc || !attn_shape_ok(*desc)) { mep_set_error("mep_diff_attn_workspace: invalid descriptor"); return MEP_EINVAL; }
     const Split s = split_of(*desc);
-    return s.splits ? split_bytes(*desc, s) : 0;
+    return s.groups ? split_bytes(*desc, s) : 0;
 }
 
 extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_t stream) {
@@ -305,10 +312,10 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     const int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb),
                   kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
-    if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, 0, st, d.dv);
+    if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, st, d.dv);
     if (keys && b.dk) {
         const int splits = b.workspace ? kv_splits(d) : 1;
-        run(DA_BWD_KV, d, &b, kg * splits, kb, splits, 0, st, d.dv);
+        run(DA_BWD_KV, d, &b, kg * splits, kb, splits, st, d.dv);
         if (splits > 1) {
             const int64_t want = ((int64_t)d.B * d.Tk * d.G * (2 * d.d + d.dv) + DA_THREADS - 1) / DA_THREADS;
             const dim3 grid((unsigned)(want < 4096 ? want : 4096)), block(DA_THREADS);

@@ -1,6 +1,6 @@
 // The differential-attention kernels in MEP_F16.
 #include "diff_attn.h"
 
-void mep::da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, int tiles, hipStream_t st, int all) {
-    da_run<MEP_F16>(what, d, b, grid, blocks, splits, tiles, st, all);
+void mep::da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all) {
+    da_run<MEP_F16>(what, d, b, grid, blocks, splits, st, all);
 }

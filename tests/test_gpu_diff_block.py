@@ -177,6 +177,15 @@ def test_keys_split(cuda, size, dtype):
     check(*case(*size, dtype, lam='row'), lengths=lengths)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('B,G', [(7, 2), (300, 1)])
+def test_ragged_cache(cuda, B, G, dtype):
+    """single tokens against caches of very different lengths, empty ones among them: workgroups share out the tiles of all"""
+    H, Tk = 2 * G, 1500 if B < 10 else 200
+    lengths = torch.tensor([(0, Tk, 1, 64, 65, Tk - 1, 700, 129)[i % 8] % (Tk + 1) for i in range(B)], dtype=torch.int32, device='cuda')
+    check(*case(B, 1, Tk, H, G, 32, 64, dtype), grads=B < 10, lengths=lengths)
+
+
 @pytest.mark.parametrize('size', [(2, 140, 70, 4, 4, 40, 160), (1, 140, 70, 8, 4, 40, 160), (1, 300, 70, 1, 1, 40, 160)])
 @pytest.mark.parametrize('causal', [False, True])
 def test_values_in_two_halves(cuda, size, causal):
