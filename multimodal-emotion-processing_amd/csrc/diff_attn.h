@@ -32,7 +32,7 @@ constexpr int DA_THREADS = 256, DA_WAVES = 4, DA_ROWS = 32 * DA_WAVES;
 constexpr float DA_LOG2E = 1.4426950408889634f;
 constexpr float DA_MIN = -1.0e30f;      // the running maximum's start: finite, so that masked scores (-inf) give 2^-inf = 0
 constexpr unsigned DA_NOWHERE = 0x80000000u, DA_SPAN = 0x7fffffffu;   // a DMA offset behind the span reads zeros
-enum { DA_FWD, DA_BWD_Q, DA_BWD_KV, DA_SPLIT };
+enum { DA_FWD, DA_FWD_TWO, DA_BWD_Q, DA_BWD_Q_TWO, DA_BWD_KV, DA_SPLIT };
 
 // keys of a tile of k_diff_split: 64 where two tiles fit 160 KB of LDS
 constexpr int da_split_keys(int type, int dk, int dv) { return (type == MEP_F32 ? 4 : 2) * 2 * 64 * (2 * dk + dv) <= 160 * 1024 ? 64 : 32; }
@@ -432,7 +432,7 @@ MEP_DEV int thread_again() {
 }
 
 // The keys and values of a (batch, key head), tile by tile
-template <int TYPE, int DK, int DV>
+template <int TYPE, int DK, int DV, int KT>
 struct KeyTiles {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
@@ -445,7 +445,7 @@ struct KeyTiles {
         vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
     }
     MEP_DEV void load_keys(T* tile, int k0, unsigned long long bits, int tid) const {
-        const Stager<M, Ge::KT, 2 * DK> ks(tid, (unsigned)d.k_sT, [&](int c) {
+        const Stager<M, KT, 2 * DK> ks(tid, (unsigned)d.k_sT, [&](int c) {
             const int m = c >= DK / M::E, col = c * M::E - m * DK;
             return col < d.d ? col + (m ? (int)d.k_sM : 0) : -1;
         });
@@ -454,8 +454,8 @@ struct KeyTiles {
     MEP_DEV void load(T* tile, int k0, unsigned long long bits) const {
         const int tid = thread_again();
         load_keys(tile, k0, bits, tid);
-        const Stager<M, Ge::KT, DV> vs(tid, (unsigned)d.v_sT, [&](int c) { return c * M::E < d.dv ? c * M::E : -1; });
-        vs.load(tile + Ge::KSZ, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
+        const Stager<M, KT, DV> vs(tid, (unsigned)d.v_sT, [&](int c) { return c * M::E < d.dv ? c * M::E : -1; });
+        vs.load(tile + KT * 2 * DK, vp + k0 * d.v_sT, (unsigned)d.v_sT, bits);
     }
 };
 
@@ -631,15 +631,61 @@ struct Online {
 
 // Values wider than 128 channels (parts = 2; their accumulators would not fit beside each other) are taken by two workgroups that both
 // form the scores.
-template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int parts) {
+// KS = 2: a workgroup takes 64 rows instead of 128, and two waves share each 32 of them, one for either half of a tile of keys; they are
+// joined in LDS.  For launches of few workgroups, whose time is the chain of a row's keys while compute units stand idle (forward and dq
+// at B 2, T 1024, 8 heads, 128 workgroups of 128 rows: bf16 16 / 32 35 us and 26, 39 and 32; 128 / 128 84 and 63, 77 and 59; fp32
+// 64 / 128 256 and 159, 345 and 232; of 256 workgroups bf16 64 / 128 67 us and 103, but causal ones 113 and 107, 108 and 98).
+template <int TYPE, int DK, int DV, int KS>
+struct RowShape {
+    typedef Geo<TYPE, DK, DV> Ge;
+    static constexpr int RG = 4 / KS, ROWS = 32 * RG;
+    static constexpr int KT = KS == 2 ? 64 : Ge::KT, KSZ = KT * 2 * DK, TSZ = KSZ + KT * DV;
+    static constexpr int OUT = ROWS * (da_piece(DK > DV ? DK : DV) + Ge::M::E);      // the results pass through the tiles
+    static constexpr int BUF = 2 * TSZ > OUT ? 2 * TSZ : OUT;
+};
+// there is a KS = 2: its tiles of 64 keys fit
+constexpr bool da_two(int type, int dk, int dv) { return (type == MEP_F32 ? 4 : 2) * 2 * 64 * (2 * dk + dv) <= 160 * 1024; }
+
+// The second waves' accumulators added to the first's: as many at a time as fit BYTES of LDS, 16 bytes of every lane side by side
+template <int RG, int BYTES, int N>
+MEP_DEV void join_waves(void* lds, floatx16 (&x)[N], int wave, int half) {
+    constexpr int FIT = BYTES / (RG * 4096), PER = FIT < N ? FIT : N;
+    static_assert(PER > 0, "LDS");
+    f32x4* at = reinterpret_cast<f32x4*>(lds) + wave * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int n0 = 0; n0 < N; n0 += PER) {
+        if (half) {
+#pragma unroll
+            for (int n = n0; n < n0 + PER && n < N; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) at[((n - n0) * 4 + q) * RG * 64] = f32x4{x[n][4 * q], x[n][4 * q + 1], x[n][4 * q + 2], x[n][4 * q + 3]};
+        }
+        tile_sync();
+        if (!half) {
+#pragma unroll
+            for (int n = n0; n < n0 + PER && n < N; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = at[((n - n0) * 4 + q) * RG * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][4 * q + e] += v[e];
+                }
+        }
+        tile_sync();
+    }
+}
+
+template <int TYPE, int DK, int DV, int KS>
+__global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) || (KS == 2 && DV >= 128) ? 1 : 2) void k_diff_fwd(mep_diff_attn_desc d, int blocks, int parts) {
+    typedef RowShape<TYPE, DK, DV, KS> Sh;
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
-    constexpr int KT = Ge::KT;
-    __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
+    constexpr int KT = Sh::KT, RG = Sh::RG;
+    __shared__ __align__(16) T Buf[Sh::BUF];      // two tiles: their keys, then their values
+    __shared__ __align__(16) f32x4 Meet[KS == 2 ? 2 : 1][KS == 2 ? Sh::ROWS : 1];
     const int ld = d.dv;
-    Job j = make_job(d, blocks * parts, d.causal ? LAST_LONGEST : IN_TURN, !da_wide(TYPE, DK));
+    Job j = make_job(d, blocks * parts, d.causal ? LAST_LONGEST : IN_TURN, !da_wide(TYPE, DK) && KS == 1);
     if (DV == 128 && parts == 2) {
         const int c = j.block % 2 * DV;
         j.block /= 2;
@@ -649,12 +695,12 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_
         if (c) d.stats = 0;
         d.dv = min(ld - c, DV);
     }
-    const int h = (threadIdx.x & 63) >> 5;
-    const Rows32 w(d, j, j.block * DA_ROWS + (threadIdx.x >> 6) * 32);
-    const KeyTiles<TYPE, DK, DV> keys(d, j);
+    const int h = (threadIdx.x & 63) >> 5, wave = KS == 2 ? (threadIdx.x >> 6) % RG : threadIdx.x >> 6, half = KS == 2 ? (threadIdx.x >> 6) / RG : 0;
+    const Rows32 w(d, j, j.block * Sh::ROWS + wave * 32);
+    const KeyTiles<TYPE, DK, DV, KT> keys(d, j);
     const Reader<M, 2 * DK> kread;
     const Reader<M, DV> vread;
-    const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
+    const int end = key_end(d, j, (min(j.rows, (j.block + 1) * Sh::ROWS) - 1) / j.n);
 
     unsigned raw = key_raw(d, j, 0);
     unsigned long long bits = key_bits(d, j, 0, KT, raw);
@@ -666,26 +712,62 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_
         const unsigned long long now = bits;
         if (k0 + KT < end) {
             bits = key_bits(d, j, k0 + KT, KT, raw);
-            keys.load(Buf + (buf ^ 1) * Ge::TSZ, k0 + KT, bits);
+            keys.load(Buf + (buf ^ 1) * Sh::TSZ, k0 + KT, bits);
             raw = key_raw(d, j, k0 + 2 * KT);
         }
-        const T* kt = Buf + buf * Ge::TSZ;
+        const T* kt = Buf + buf * Sh::TSZ;
+        int subs = KT / 32;
+        if constexpr (KS == 2) asm("" : "+s"(subs));      // or the loop of one pass is folded into the outer one, whose accumulators are then copied
 #pragma unroll 1
-        for (int sub = 0; sub < KT / 32; ++sub) {
+        for (int sub = half; sub < subs; sub += KS) {
             const int ks = k0 + 32 * sub;
             const unsigned on = (unsigned)(now >> (32 * sub));
-            if (ks < w.wend && on) o.step(d, j, w, kread, vread, kt, kt + Ge::KSZ, 32 * sub, ks, on);
+            if (ks < w.wend && on) o.step(d, j, w, kread, vread, kt, kt + Sh::KSZ, 32 * sub, ks, on);
         }
     }
     o.l1 = half_sum(o.l1);
     o.l2 = half_sum(o.l2);
-    const float i1 = o.l1 > 0.f ? 1.f / o.l1 : o.l1, i2 = o.l2 > 0.f ? 1.f / o.l2 : o.l2;
     float n1, n2, g1, g2;
     o.maxima(n1, n2, g1, g2);
-    if (d.stats && w.live && h == 0)
-        *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) = f32x4{n1, i1 / g1, n2, i2 / g2};
-    const float fx = i1 / o.f1, fy = fx * o.f2 - o.lam * i2;
+    float l1 = o.l1 * g1, l2 = o.l2 * g2, xx, xy, yy;      // of 2^n; E_1 = xx X + xy Y, E_2 = yy Y of 2^n
     tile_sync();                             // the tiles are free
+    if constexpr (KS == 2) {
+        const int r = wave * 32 + (threadIdx.x & 31);
+        if (h == 0) Meet[half][r] = f32x4{n1, l1, n2, l2};
+        tile_sync();
+        const f32x4 m = Meet[half ^ 1][r];
+        const float t1 = fmaxf(n1, m[0]), t2 = fmaxf(n2, m[2]);
+        const float a1 = l1 * exp2_fast(n1 - t1), b1 = m[1] * exp2_fast(m[0] - t1), a2 = l2 * exp2_fast(n2 - t2), b2 = m[3] * exp2_fast(m[2] - t2);
+        l1 = a1 + b1;
+        l2 = a2 + b2;
+        g1 = exp2_fast(o.m1 - t1);
+        g2 = exp2_fast(o.m2 - t2);
+        n1 = t1;
+        n2 = t2;
+        xx = g1 / o.f1;
+        xy = xx * o.f2;
+        yy = g2;
+#pragma unroll
+        for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                o.x[n][i] = fmaf(o.x[n][i], xx, o.y[n][i] * xy);
+                o.y[n][i] *= yy;
+            }
+        join_waves<RG, Sh::BUF * (int)sizeof(T)>(Buf, o.x, wave, half);
+        join_waves<RG, Sh::BUF * (int)sizeof(T)>(Buf, o.y, wave, half);
+        if (half) return;
+        xx = yy = 1.f;
+        xy = 0.f;
+    } else {
+        xx = g1 / o.f1;
+        xy = xx * o.f2;
+        yy = g2;
+    }
+    const float i1 = l1 > 0.f ? 1.f / l1 : l1, i2 = l2 > 0.f ? 1.f / l2 : l2;
+    if (d.stats && w.live && h == 0)
+        *reinterpret_cast<MEP_G f32x4*>(G<float>(d.stats) + 4 * (((int64_t)j.b * d.H + w.head) * d.Tq + w.t)) = f32x4{n1, i1, n2, i2};
+    const float fx = i1 * xx, fy = i1 * xy - o.lam * i2 * yy;
     const int64_t first = (int64_t)j.b * d.Tq * d.H * ld;
     auto row_at = [&](uint64_t p, int r) -> MEP_G T* {
         const int row = w.row0 + r;
@@ -694,13 +776,13 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) ? 1 : 2) void k_diff_
         return G<T>(p) + first + ((int64_t)t * d.H + j.g * j.n + row - t * j.n) * ld;
     };
     const bool whole = ld % M::E == 0;
-    T* mine = Buf + (threadIdx.x >> 6) * 32 * (da_piece(DV) + M::E);
+    T* mine = Buf + wave * 32 * (da_piece(DV) + M::E);
 #pragma unroll
     for (int n = 0; n < DV / 32; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o.x[n][r] = fmaf(o.x[n][r], fx, o.y[n][r] * fy);
     write_rows<M>(mine, o.x, 1.f, d.dv, whole, [&](int r) { return row_at(d.out, r); });
-    if (d.second) write_rows<M>(mine, o.y, i2, d.dv, whole, [&](int r) { return row_at(d.second, r); });
+    if (d.second) write_rows<M>(mine, o.y, i2 * yy, d.dv, whole, [&](int r) { return row_at(d.second, r); });
 }
 
 // ------------------------------------------------------------------ forward over split keys
@@ -879,23 +961,25 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
 // (accumulators that pass through the accumulation registers for every tile cost more than a second pass): there a second pass
 // over the keys forms it where a row of the workgroup rests on fewer than 32 keys (sum A_m^2 > 1 / 32; at that it is a thirtieth of
 // dS's rounding).  (In fp32 the estimate is as good as the sum.)  The sums are also lam's gradient and what dk needs.
-template <int TYPE, int DK, int DV>
-__global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
+template <int TYPE, int DK, int DV, int KS>
+__global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
+    typedef RowShape<TYPE, DK, DV, KS> Sh;
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
     typedef typename Ge::T T;
     typedef typename Ge::Frag Frag;
-    constexpr int KT = Ge::KT;
+    constexpr int KT = Sh::KT, RG = Sh::RG;
     const mep_diff_attn_desc& d = bd.f;
-    __shared__ __align__(16) T Buf[Ge::BUF];      // two tiles: their keys, then their values
-    const Job j = make_job(d, blocks, d.causal ? LAST_LONGEST : IN_TURN, !da_wide(TYPE, DK));
-    const int h = (threadIdx.x & 63) >> 5;
-    const Rows32 w(d, j, j.block * DA_ROWS + (threadIdx.x >> 6) * 32);
-    const KeyTiles<TYPE, DK, DV> keys(d, j);
+    __shared__ __align__(16) T Buf[Sh::BUF];      // two tiles: their keys, then their values
+    __shared__ __align__(16) f32x4 Meet[KS == 2 ? 2 : 1][KS == 2 ? Sh::ROWS : 1];
+    const Job j = make_job(d, blocks, d.causal ? LAST_LONGEST : IN_TURN, !da_wide(TYPE, DK) && KS == 1);
+    const int h = (threadIdx.x & 63) >> 5, wave = KS == 2 ? (threadIdx.x >> 6) % RG : threadIdx.x >> 6, half = KS == 2 ? (threadIdx.x >> 6) / RG : 0;
+    const Rows32 w(d, j, j.block * Sh::ROWS + wave * 32);
+    const KeyTiles<TYPE, DK, DV, KT> keys(d, j);
     const Reader<M, 2 * DK> kread;
     const Reader<M, DV> vread;
     const Exponent<TYPE> ex(d.scale);
-    const int end = key_end(d, j, (min(j.rows, (j.block + 1) * DA_ROWS) - 1) / j.n);
+    const int end = key_end(d, j, (min(j.rows, (j.block + 1) * Sh::ROWS) - 1) / j.n);
 
     unsigned raw = key_raw(d, j, 0);
     unsigned long long bits = key_bits(d, j, 0, KT, raw);
@@ -944,18 +1028,20 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
     b1 = b2 = zero16();
 #pragma unroll
     for (int n = 0; n < DK / 32; ++n) a1[n] = a2[n] = zero16();
+    int subs = KT / 32;
+    if constexpr (KS == 2) asm("" : "+s"(subs));      // or the loop of one pass is folded into the outer one, whose accumulators are then copied
     for (int k0 = 0, buf = 0; k0 < end; k0 += KT, buf ^= 1) {
         tile_sync();
         const unsigned long long now = bits;
         if (k0 + KT < end) {
             bits = key_bits(d, j, k0 + KT, KT, raw);
-            keys.load(Buf + (buf ^ 1) * Ge::TSZ, k0 + KT, bits);
+            keys.load(Buf + (buf ^ 1) * Sh::TSZ, k0 + KT, bits);
             raw = key_raw(d, j, k0 + 2 * KT);
         }
-        const T* kt = Buf + buf * Ge::TSZ;
-        const T* vt = kt + Ge::KSZ;
+        const T* kt = Buf + buf * Sh::TSZ;
+        const T* vt = kt + Sh::KSZ;
 #pragma unroll 1
-        for (int sub = 0; sub < KT / 32; ++sub) {
+        for (int sub = half; sub < subs; sub += KS) {
             const int ks = k0 + 32 * sub;
             const unsigned on = (unsigned)(now >> (32 * sub));
             if (ks >= w.wend || !on) continue;
@@ -1028,15 +1114,31 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
             __builtin_amdgcn_s_setprio(0);
         }
     }
-    sum1 = half_sum(sum1) * st[1];
-    sum2 = half_sum(sum2) * st[3];
-    if (w.live && h == 0) {
+    sum1 = half_sum(sum1);
+    sum2 = half_sum(sum2);
+    if constexpr (CORR) {
+        sq1 = half_sum(sq1);
+        sq2 = half_sum(sq2);
+    }
+    if constexpr (KS == 2) {
+        const int r = wave * 32 + (threadIdx.x & 31);
+        if (h == 0) Meet[half][r] = f32x4{sum1, sum2, sq1, sq2};
+        __syncthreads();
+        const f32x4 m = Meet[half ^ 1][r];
+        sum1 += m[0];
+        sum2 += m[1];
+        sq1 += m[2];
+        sq2 += m[3];
+    }
+    sum1 *= st[1];
+    sum2 *= st[3];
+    if (w.live && h == 0 && half == 0) {
         *reinterpret_cast<MEP_G f32x4*>(G<float>(bd.delta) + 4 * srow) = f32x4{sum1, sum2, 0.f, 0.f};
         if (bd.dlam_rows) G<float>(bd.dlam_rows)[((int64_t)j.b * d.Tq + w.t) * d.H + w.head] = -sum2;
     }
     if (!bd.dq) return;
     if constexpr (CORR) {
-        const bool few = w.live && fmaxf(half_sum(sq1) * st[1] * st[1], half_sum(sq2) * st[3] * st[3]) > 0.03125f;
+        const bool few = w.live && fmaxf(sq1 * st[1] * st[1], sq2 * st[3] * st[3]) > 0.03125f;
         if (__syncthreads_or(few)) {
             floatx16 k1[DK / 32], k2[DK / 32];
 #pragma unroll
@@ -1047,7 +1149,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
                 keys.load_keys(Buf, k0, bits, thread_again());
                 tile_sync();
 #pragma unroll 1
-                for (int sub = 0; sub < KT / 32; ++sub) {
+                for (int sub = half; sub < subs; sub += KS) {
                     const int ks = k0 + 32 * sub;
                     const unsigned on = (unsigned)(bits >> (32 * sub));
                     if (ks >= w.wend || !on) continue;
@@ -1091,6 +1193,11 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
         }
     }
     tile_sync();                             // the tiles are free
+    if constexpr (KS == 2) {
+        join_waves<RG, Sh::BUF * (int)sizeof(T)>(Buf, a1, wave, half);
+        join_waves<RG, Sh::BUF * (int)sizeof(T)>(Buf, a2, wave, half);
+        if (half) return;
+    }
     const int64_t first = (int64_t)j.b * d.Tq * d.H * 2 * d.d;
     auto row_at = [&](int m, int r) -> MEP_G T* {
         const int row = w.row0 + r;
@@ -1099,7 +1206,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 ? 1 : 2) void k_diff_bwd_q(me
         return G<T>(bd.dq) + first + (((int64_t)t * d.H + j.g * j.n + row - t * j.n) * 2 + m) * d.d;
     };
     const bool whole = d.d % M::E == 0;
-    T* mine = Buf + (threadIdx.x >> 6) * 32 * (da_piece(DK) + M::E);
+    T* mine = Buf + wave * 32 * (da_piece(DK) + M::E);
     write_rows<M>(mine, a1, st[1] * d.scale, d.d, whole, [&](int r) { return row_at(0, r); });
     write_rows<M>(mine, a2, -lam * st[3] * d.scale, d.d, whole, [&](int r) { return row_at(1, r); });
 }
@@ -1469,9 +1576,15 @@ constexpr int da_kw(int type, int dk) { return dk >= 128 && type != MEP_F32 ? 2 
 
 template <int TYPE, int DK, int DV>
 void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st) {      // splits: DA_FWD's parts, DA_SPLIT's groups
-    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
+    constexpr int PV = da_piece(DV);
+    if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, PV, 1>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
+    else if (what == DA_FWD_TWO) {
+        if constexpr (da_two(TYPE, DK, PV)) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, PV, 2>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
+    } else if (what == DA_BWD_Q_TWO) {
+        if constexpr (da_two(TYPE, DK, DV)) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV, 2>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+    }
     else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_SPLIT_THREADS), 0, st, d, blocks, splits);
-    else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+    else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV, 1>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
                             dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks, splits);
 }

@@ -191,6 +191,13 @@ int kv_splits(const mep_diff_attn_desc& d) {
     return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
 }
 
+// Whether two waves share a row's keys (KS = 2) in a launch of `grid` workgroups of 128 rows, over dv channels of the values at a time:
+// while that leaves half of the compute units idle; causal ones, of which the longest are left at the end, while there is one for each
+bool two_waves(const mep_diff_attn_desc& d, int64_t grid, int dv) {
+    const int dk = da_width(d.d, d.dv), width = da_value_width(d.d, d.dv);
+    return grid <= (d.causal ? 256 : 128) && d.Tk > 64 && da_two(d.type, dk, width < dv ? width : dv);
+}
+
 bool attn_shape_ok(const mep_diff_attn_desc& d) {
     if (d.B < 0 || d.Tq < 0 || d.Tk < 0 || d.H < 1 || d.G < 1 || d.H % d.G || d.type < MEP_F32 || d.type > MEP_F16) return false;
     if (d.d < 1 || d.d > MEP_DIFF_ATTN_MAX_D || d.dv < 1 || d.dv > MEP_DIFF_ATTN_MAX_DV) return false;
@@ -252,15 +259,17 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
     if (d.B == 0 || d.Tq == 0) return 0;
     if (!inputs_ok(d)) { mep_set_error("mep_diff_attn_fwd: rows that cannot be read 16 bytes at a time"); return MEP_EINVAL; }
     int blocks;
-    const int64_t grid = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, blocks);
+    int64_t grid = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, blocks);
     if (grid < 0) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
     hipStream_t st = (hipStream_t)stream;
     const Split s = split_of(d);
     const int es = d.type == MEP_F32 ? 4 : 2, half = da_piece(d.dv);
     if (!s.groups || !d.workspace) {
         const int parts = d.dv > half ? 2 : 1;
+        const bool two = two_waves(d, grid * parts, 128);
+        if (two) grid = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS / 2, blocks);
         if (grid * parts >= 1 << 23) { mep_set_error("mep_diff_attn_fwd: too many rows for one launch"); return MEP_EINVAL; }
-        run(DA_FWD, d, nullptr, grid * parts, blocks, parts, st, d.dv);
+        run(two ? DA_FWD_TWO : DA_FWD, d, nullptr, grid * parts, blocks, parts, st, d.dv);
         return mep_check_launch("mep_diff_attn_fwd");
     }
     // values of more than 128 channels in two launches: their accumulators would not fit beside each other
@@ -309,10 +318,14 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     }
     hipStream_t st = (hipStream_t)stream;
     int qb, kb;
-    const int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb),
-                  kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
+    const int64_t kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
+    int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
-    if (rows) run(DA_BWD_Q, d, &b, qg, qb, 1, st, d.dv);
+    if (rows) {
+        const bool two = two_waves(d, qg, 256);
+        if (two) qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS / 2, qb);
+        run(two ? DA_BWD_Q_TWO : DA_BWD_Q, d, &b, qg, qb, 1, st, d.dv);
+    }
     if (keys && b.dk) {
         const int splits = b.workspace ? kv_splits(d) : 1;
         run(DA_BWD_KV, d, &b, kg * splits, kb, splits, st, d.dv);

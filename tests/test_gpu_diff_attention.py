@@ -51,7 +51,13 @@ def check(q, k, v, lam, grads=True, dout=None, scale=None, same_maps=False, **ma
         both = a[:, :, 0] + lamb * a[:, :, 1]
         diff = (a[:, :, 0] - lamb * a[:, :, 1]).abs()
         upto = lambda x: x.cumsum(-1)[..., [min(32 * (i // 32) + 31, Tk - 1) for i in range(Tk)]] if Tk else x  # noqa: E731
+        # rho comes from the keys that the wave has seen.  Where two waves share a row, one sees the even 32 of the keys and the other the odd,
+        # and its own sums up to there stand in the same bound
         late = upto(a[:, :, 0]) / upto(a[:, :, 1]).clamp_min(1e-300)
+        odd = (torch.arange(Tk) // 32 % 2).bool()
+        for side in (odd, ~odd):
+            own = upto(a[:, :, 0] * side) / upto(a[:, :, 1] * side).clamp_min(1e-300)
+            late = torch.where(side, torch.maximum(late, own), late)
         fwd = diff if same_maps else a[:, :, 0] + lamb * a[:, :, 1] * (1.25 * late + 0.25)
     half = ref.half_step(q.dtype) if q.dtype != torch.float32 else 0.0
     terms = 64 + 16 * big + Tk / 8      # the exponents, and the sums over keys
