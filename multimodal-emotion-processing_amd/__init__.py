@@ -7,6 +7,7 @@ Public surface (mirrors the reference scripts):
   mep_amd.ren_mme     Base_model (+ Ren-MME variants of the same classes), multi_loss, train, valid
   mep_amd.optim       FusedAdamW / FusedAdam (clip + update over the flat parameter buffer)
   mep_amd.engine      TrainEngine (graph-captured fused step, RCCL data parallel)
+  mep_amd.diff_block  operators of a differential-attention block: rotary, norm, norm_residual, diff_attention
 Kernels: libmep_hip.so (csrc/, C ABI in include/mep.h).  No CPU fallback.
 """
 import os

@@ -13,7 +13,7 @@
 // A workgroup walks many rows with the parameters, and in the backward the column sums, in registers; the sums of its row
 // slots are joined in LDS, those of the workgroups by a second kernel, in a fixed order.  8 elements a lane leave the
 // backward's registers (parameters, up to 5 sums and 4 rows) room for 4 waves on a SIMD: at 16384 rows of 4096 in bf16, both
-// norms and a gate, 455 us with 16 elements.
+// norms and a gate, 211 us (4.1 TB/s), 455 with 16 elements; the forward 131 us.
 #include "elem.h"
 
 namespace {

@@ -335,7 +335,8 @@ MEP_DEV void fill_job(const mep_diff_attn_desc& d, Job& j) {
 // stay on one XCD (or on a few, in turn), so that its keys are read into one L2.
 // Causal calls: the blocks differ by up to their number in length, and all pairs' longest come first.  Where two workgroups share a
 // compute unit (`shared`) and both halves of the first 512 are there from the start, the second half goes the other way, so that
-// the longest shares its unit with the shortest (B 2, T 4096, 8 heads, 64 / 128: forward FWD_OLD us pair by pair).
+// the longest shares its unit with the shortest (B 2, T 4096, 8 heads, 64 / 128, bf16: forward 199 us, 207 without that turn, 230 pair by
+// pair).
 enum Order { IN_TURN, FIRST_LONGEST, LAST_LONGEST };
 MEP_DEV Job make_job(const mep_diff_attn_desc& d, int blocks, Order order, bool shared) {
     Job j;
@@ -523,6 +524,10 @@ MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, i
 // that the row's weights do not have.
 // The maxima m_m are renewed only when a score exceeds one by 8 (e <= 256: the sums are as exact), the lanes of a row agree on them, and
 // the sums l_m stay lane-local to the end.
+// Bound by vector operations beside the products: a step of 32 keys x 32 rows has 24 matrix instructions (64 / 128; 768 cycles) and about
+// 240 others, 32 of them exponentials (1350 cycles), and two waves on a SIMD overlap them in part; s_setprio lets the wave whose products
+// are ready go first (254 us -> 230).  B 2, T 4096, 8 heads, causal: 199 us; B 1, T 8192, 16 heads on 4 key heads: 490 us, 560 TFLOP/s
+// of the 512 operations that a pair takes by the formula.
 template <int TYPE, int DK, int DV>
 struct Online {
     typedef Geo<TYPE, DK, DV> Ge;
@@ -789,9 +794,10 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) || (KS == 2 && DV >= 
 // Few rows against many keys (single tokens against a cache).  The tiles of keys of all (batch row, key head, 32 rows) stand in one
 // row, those behind a batch row's length left out, and each of `groups` workgroups takes an equal share of it: equal work whatever
 // the lengths (B 32 of up to 8192 keys, 4 key heads: 81 us, against 105 with as many tiles to a workgroup in each batch row's own
-// splits), neighbouring shares on one XCD; to begin with the next rows counts as DA_SPLIT_START tiles (87 us without).  A workgroup has two waves; of a tile of 64 keys (32 where two of 64 do not fit LDS: of every
-// other tile) a wave takes 32, and for each batch row it comes to it leaves its rows' maxima, sums, E_1 and E_2 in fp32;
-// k_diff_join joins them.  Bound by reading the keys and values once: two tiles in flight in each of two workgroups on a compute unit.
+// splits), neighbouring shares on one XCD; to begin with the next rows counts as DA_SPLIT_START tiles (87 us without).  A workgroup has
+// two waves; of a tile of 64 keys (32 where two of 64 do not fit LDS: of every other tile) a wave takes 32, and for each batch row it
+// comes to it leaves its rows' maxima, sums, E_1 and E_2 in fp32; k_diff_join joins them.  Bound by reading the keys and values once,
+// at 4.3 TB/s: two tiles in flight in each of two workgroups on a compute unit.
 // workspace: the number of tiles before each batch row, int [B + 1]; then a part for each wave of each (workgroup, (batch row, key head,
 // 32 rows)) that meet, at workgroup + (batch row, key head, 32 rows): (m1, l1, m2, l2) [R], E_1 [R][dv], E_2 [R][dv], R = min(32, rows)
 constexpr int DA_SPLIT_THREADS = 128, DA_SPLIT_START = 3;
@@ -1212,10 +1218,11 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
 }
 
 // ------------------------------------------------------------------ backward: dk and dv
-// A workgroup walks the rows of 32 KW keys, a wave (an accumulator column per key) those of 32.  At DK = 32 (fp32: 64, its
-// operands are not held) a wave forms dv and dk (ROLES = 1).  With wider heads the workgroup has 2 KW waves, one half for dv and the other for dk (ROLES = 2): both form
-// the scores, but so neither holds more than 256 registers and two waves share a SIMD (in one wave, the accumulators of
-// both pass through the accumulation registers and back for every tile: 335 us against 268 at B 2, T 4096, 8 heads, 64 / 128, causal).
+// A workgroup walks the rows of 32 KW keys, a wave (an accumulator column per key) those of 32.  At DK = 32 and in fp32 (one wave a
+// SIMD, with all its registers) a wave forms dv and dk (ROLES = 1).  In 16 bits with wider heads the workgroup has 2 KW waves, one half
+// for dv and the other for dk (ROLES = 2): both form the scores, but so neither holds more than 256 registers and two waves share a
+// SIMD (in one wave, the accumulators of both pass through the accumulation registers and back for every tile: 335 us against 264
+// at B 2, T 4096, 8 heads, 64 / 128, causal).  Where the blocks of keys are few, splits of the rows are summed by k_diff_kv_join.
 //
 // The scores lie rows x keys here, so a row's statistics are not a lane's.  They come in as a product: the accumulator starts
 // at X 1 with X the row's value in three bf16 parts (24 bits) against a column of ones, one instruction for 16 registers.  With

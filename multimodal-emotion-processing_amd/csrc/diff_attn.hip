@@ -154,13 +154,14 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_kv_join(mep_diff_attn_bwd_d
 
 // Whether the keys of a forward are split (groups > 0), and over how many workgroups.  Worth it where the rows are few: up to 32 a
 // (batch row, key head) leave three of k_diff_fwd's four waves idle (against a row of 8192 keys, 32 batch rows, 4 key heads: 297 us
-// whole, 84 split and joined), and more rows too when their workgroups are under a quarter of the compute units and there are 1024 keys
-// (16 / 32 bf16, 64 workgroups: 36 us whole, 38 split).  As many workgroups as are on the chip at a time, and 4 tiles for each.
+// whole, 84 split and joined), and more rows too when they make up to 32 workgroups and there are 1024 keys (32 workgroups against
+// 4096 keys: bf16 16 / 32 79 us whole, 37 split, 64 / 128 141 and 82; 56 against 2048: 128 / 128 98 and 145).  As many workgroups
+// as are on the chip at a time, and 4 tiles for each.
 struct Split { int blocks, groups; };
 Split split_of(const mep_diff_attn_desc& d) {
     Split s = {0, 0};
     const int64_t rows = (int64_t)d.Tq * (d.H / d.G), pairs = (int64_t)d.B * d.G;
-    const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) < 64;
+    const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) <= 32;
     if (pairs == 0 || rows == 0 || !(few || none)) return s;
     s.blocks = (int)((rows + 31) / 32);
     const int dk = da_width(d.d, d.dv), dv = da_piece(da_value_width(d.d, d.dv)), kt = da_split_keys(d.type, dk, dv);
@@ -181,7 +182,8 @@ void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b,
 }
 
 // Into how many workgroups the rows of a block of keys are split: until there are two for every compute unit, 4 tiles of rows each at
-// least, 8 at most (each leaves its sums in fp32)
+// least, 8 at most (each leaves its sums in fp32, which k_diff_kv_join adds: 10 us at B 2, T 1024, 4 key heads, 64 / 64, where dk and dv
+// take 187 us in fp32 split and 480 whole)
 int kv_splits(const mep_diff_attn_desc& d) {
     const int dk = da_width(d.d, d.dv), per = 32 * da_kw(d.type, dk), tile = d.type == MEP_F32 ? 32 : 64;
     const int64_t grid = (int64_t)d.B * d.G * ((d.Tk + per - 1) / per), tiles = ((int64_t)d.Tq * (d.H / d.G) + tile - 1) / tile;

@@ -6,9 +6,10 @@
     x, h = norm_residual(y, x, ...)                       norm behind the block, gate, residual scale, next norm
 
 They stand beside the residual-attention blocks of the reference (its Attention_Block takes position tables, one
-softmax map and a LayerNorm behind the block, cmu-mosei/run.py:206-262) and have no counterpart there.  Each call is
-one launch (two where column sums or key splits are joined) on the current stream of its tensors' device, allocates
-nothing but its results and workspace, never synchronises, and may be captured into a graph.  float32, bfloat16 and float16
+softmax map and a LayerNorm behind the block, cmu-mosei/run.py:206-262) and have no counterpart there.  Each call launches
+its kernels (one; more where column sums or splits are joined, an unaligned input is copied, or dq, dk and lam's gradient
+follow each other) on the current stream of its tensors' device, allocates nothing but its results and workspace, never
+synchronises, and may be captured into a graph.  float32, bfloat16 and float16
 activations; sums, statistics and angles in 32 bits or more; results do not depend on the order of atomics.
 
 Gradients come through torch.autograd.  To capture a backward pass into a graph, make the leaves it differentiates inside
