@@ -848,7 +848,10 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
         const int x = __shfl_up(upto, o);
         if ((tid & 63) >= o) upto += x;
     }
-    if (tid == 63) At[0] = upto;
+    if (tid == 63) {
+        At[0] = upto;
+        At[2] = d.B;      // (no row is looked for past the last)
+    }
     __syncthreads();
     if (wave) upto += At[0];
     if (tid == DA_SPLIT_THREADS - 1) At[1] = upto;

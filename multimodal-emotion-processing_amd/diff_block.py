@@ -175,7 +175,9 @@ def rotary(q, k=None, *, positions, freqs, layout='half', amplitude=1.0):
 
 # ------------------------------------------------------------------ the norms around a block
 def _rows(t, D):
-    """(2-D row view, row stride) of [..., D]; a copy only where the rows have no common stride"""
+    """(rows, row stride) of [..., D]: as it is, or a 2-D view; a copy only where the rows have no common stride"""
+    if t.is_contiguous():
+        return t, D
     t = t.reshape(-1, D)
     if D > 1 and t.stride(1) != 1:
         t = t.contiguous()
@@ -192,9 +194,9 @@ class _NormFn(torch.autograd.Function):
         x2, x_ld = _rows(x, D) if x is not None else (None, 0)
         g2, g_ld = _rows(gate, D) if gate_form == 3 else (gate.contiguous() if gate is not None else None, 0)
         w, b, nw, nb = (None if t is None else t.contiguous() for t in (w, b, nw, nb))
-        n = y2.shape[0]
+        n = y.numel() // D
         stream = torch.empty(y.shape, dtype=y.dtype, device=dev)
-        normed = torch.empty(y.shape, dtype=y.dtype, device=dev) if next_kind else None
+        normed = torch.empty_like(stream) if next_kind else None
         keep = grad and any(ctx.needs_input_grad)
         stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if keep else None
         params = [t for t in (w, b, nw, nb) if t is not None]
@@ -225,7 +227,7 @@ class _NormFn(torch.autograd.Function):
         shape, gate_shape, scale_shape = ctx.shapes
         d = ctx.desc
         if _places(saved) != ctx.places:
-            D = shape[-1]
+            D = d.D
             y2, x2, g2 = saved[:3]
             (y2, y_ld), (x2, x_ld) = _rows(y2, D), _rows(x2, D) if x2 is not None else (None, 0)
             g2, g_ld = _rows(g2, D) if d.gate_form == 3 else (g2, 0)
@@ -233,14 +235,14 @@ class _NormFn(torch.autograd.Function):
             d = _moved(d, ('y', 'x', 'gate', 'w', 'b', 'scale', 'nw', 'nb', 'stats'), saved)
             d.y_ld, d.x_ld, d.g_ld = y_ld, x_ld, g_ld
         y2, x2, g2, w, b, scale, nw, nb, _ = saved
-        n, D = y2.shape
-        dev = y2.device
+        n, D, dev = d.rows, d.D, y2.device
         rows = lambda on: torch.empty(shape, dtype=y2.dtype, device=dev) if on else None  # noqa: E731
         like = lambda t, on: torch.empty_like(t) if t is not None and on else None  # noqa: E731
         dy, dx = rows(True), rows(x2 is not None and need[2])
-        dw, db, dgate, dscale, dnw, dnb = (like(t, need[i]) for t, i in ((w, 3), (b, 4), (g2, 5), (scale, 6), (nw, 7), (nb, 8)))
-        if d.gate_form == 3 and dgate is not None:
-            dgate = rows(True)
+        dw, db, dgate, dscale, dnw, dnb = (like(t, need[i]) for t, i in ((w, 3), (b, 4), (None if d.gate_form == 3 else g2, 5),
+                                                                         (scale, 6), (nw, 7), (nb, 8)))
+        if d.gate_form == 3:
+            dgate = rows(need[5])
         if dnormed is None:    # the second norm took no part
             for t in (dnw, dnb):
                 if t is not None:
@@ -266,9 +268,9 @@ class _NormFn(torch.autograd.Function):
                                        dgate=_ptr(dgate) if d.gate_form != 3 else 0, dscale=_ptr(dscale),
                                        partial=_ptr(partial), ds_ld=ds_ld, dn_ld=dn_ld, n_sums=len(sums))
             _launch('mep_block_norm_bwd', bd, dev)
-        if dgate is not None:
+        if dgate is not None and dgate.shape != gate_shape:
             dgate = dgate.reshape(gate_shape)
-        if dscale is not None:
+        if dscale is not None and dscale.shape != scale_shape:
             dscale = dscale.reshape(scale_shape)
         return (None, dy if need[1] else None, dx, dw, db, dgate, dscale, dnw, dnb)
 
