@@ -842,6 +842,7 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
     // the tiles before each batch row: a thread sums some rows', the threads' sums are summed up
     const int rows_each = (d.B + DA_SPLIT_THREADS - 1) / DA_SPLIT_THREADS, b0 = min(d.B, tid * rows_each), b1 = min(d.B, b0 + rows_each);
     int mine = 0;
+#pragma unroll 8
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
     int upto = mine;
     for (int o = 1; o < 64; o *= 2) {
@@ -861,14 +862,16 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
     const bool some = start < stop;
     const int first_tile = some ? (int)(start / parts.per) : 0;      // of the batch rows' tiles
     int before = upto - mine;
-    for (int b = b0; b < b1; ++b) {
-        const int n = tiles_of(b);
-        if (self == 0) G<int>(d.workspace)[b] = before;
-        if (some && before <= first_tile && first_tile < before + n) {
-            At[2] = b;
-            At[3] = before;
+    if (self == 0 || (some && before <= first_tile && first_tile < upto)) {      // (only the thread that has it looks)
+        for (int b = b0; b < b1; ++b) {
+            const int n = tiles_of(b);
+            if (self == 0) G<int>(d.workspace)[b] = before;
+            if (some && before <= first_tile && first_tile < before + n) {
+                At[2] = b;
+                At[3] = before;
+            }
+            before += n;
         }
-        before += n;
     }
     if (self == 0 && tid == DA_SPLIT_THREADS - 1) G<int>(d.workspace)[d.B] = upto;
     if (!some) return;
