@@ -153,15 +153,16 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_kv_join(mep_diff_attn_bwd_d
 }
 
 // Whether the keys of a forward are split (groups > 0), and over how many workgroups.  Worth it where the rows are few: up to 32 a
-// (batch row, key head) leave three of k_diff_fwd's four waves idle (against a row of 8192 keys, 32 batch rows, 4 key heads: 297 us
-// whole, 84 split and joined), and more rows too when they make up to 32 workgroups and there are 1024 keys (32 workgroups against
+// (batch row, key head) leave three of k_diff_fwd's four waves idle (with 4 key heads, 64 / 128, full and ragged caches: 64 batch rows of
+// 8192 keys 336 and 330 us whole, 213 and 120 split; 64 of 1024 49 and 48, 48 and 39; 128 of 1024 55 and 52, 66 and 54; 64 of 512
+// 30 and 28, 37 and 30), and more rows too when they make up to 32 workgroups and there are 1024 keys (32 workgroups against
 // 4096 keys: bf16 16 / 32 79 us whole, 37 split, 64 / 128 141 and 82; 56 against 2048: 128 / 128 98 and 145).  As many workgroups
 // as are on the chip at a time, and 4 tiles for each.
 struct Split { int blocks, groups; };
 Split split_of(const mep_diff_attn_desc& d) {
     Split s = {0, 0};
     const int64_t rows = (int64_t)d.Tq * (d.H / d.G), pairs = (int64_t)d.B * d.G;
-    const bool few = rows <= 32 && d.Tk > 128, none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) <= 32;
+    const bool few = rows <= 32 && d.Tk >= (pairs < 512 ? 1024 : 2048), none = rows > 32 && d.Tk >= 1024 && pairs * ((rows + DA_ROWS - 1) / DA_ROWS) <= 32;
     if (pairs == 0 || rows == 0 || !(few || none)) return s;
     s.blocks = (int)((rows + 31) / 32);
     const int dk = da_width(d.d, d.dv), dv = da_piece(da_value_width(d.d, d.dv)), kt = da_split_keys(d.type, dk, dv);

@@ -170,7 +170,7 @@ def test_rows_split(cuda, size, masks, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('size', [(1, 40, 1100, 2, 1, 16, 32), (1, 100, 1030, 1, 1, 40, 200), (2, 3, 300, 4, 1, 72, 256)])
+@pytest.mark.parametrize('size', [(1, 40, 1100, 2, 1, 16, 32), (1, 100, 1030, 1, 1, 40, 200), (2, 3, 300, 4, 1, 72, 256), (2, 3, 1100, 4, 1, 72, 256)])
 def test_keys_split(cuda, size, dtype):
     """few rows and many keys, with gradients"""
     lengths = torch.full((size[0],), size[2] - 90, dtype=torch.int32, device='cuda')
@@ -178,10 +178,10 @@ def test_keys_split(cuda, size, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('B,G', [(7, 2), (300, 1)])
-def test_ragged_cache(cuda, B, G, dtype):
+@pytest.mark.parametrize('B,G,Tk', [(7, 2, 1500), (300, 1, 200), (300, 1, 1024)])
+def test_ragged_cache(cuda, B, G, Tk, dtype):
     """single tokens against caches of very different lengths, empty ones among them: workgroups share out the tiles of all"""
-    H, Tk = 2 * G, 1500 if B < 10 else 200
+    H = 2 * G
     lengths = torch.tensor([(0, Tk, 1, 64, 65, Tk - 1, 700, 129)[i % 8] % (Tk + 1) for i in range(B)], dtype=torch.int32, device='cuda')
     check(*case(B, 1, Tk, H, G, 32, 64, dtype), grads=B < 10, lengths=lengths)
 
