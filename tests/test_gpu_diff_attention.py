@@ -52,7 +52,8 @@ def check(q, k, v, lam, grads=True, dout=None, scale=None, same_maps=False, **ma
         diff = (a[:, :, 0] - lamb * a[:, :, 1]).abs()
         upto = lambda x: x.cumsum(-1)[..., [min(32 * (i // 32) + 31, Tk - 1) for i in range(Tk)]] if Tk else x  # noqa: E731
         # rho, the estimate that f1 e_1 - f2 e_2 is formed with, comes from the keys that the wave has seen: the rounded operand is at most
-        # A_1 + rho A_2 with rho <= lam (1.25 late + 0.25), late the ratio of the maps' sums over those keys.  Where two waves share a row, one sees the even 32 of the keys and the other the odd,
+        # A_1 + rho A_2 with rho <= lam (1.25 late + 0.25), late the ratio of the maps' sums over those keys.  Where two waves share a row,
+        # one sees the even 32 of the keys and the other the odd,
         # and its own sums up to there stand in the same bound
         late = upto(a[:, :, 0]) / upto(a[:, :, 1]).clamp_min(1e-300)
         odd = (torch.arange(Tk) // 32 % 2).bool()

@@ -186,6 +186,35 @@ def test_ragged_cache(cuda, B, G, Tk, dtype):
     check(*case(B, 1, Tk, H, G, 32, 64, dtype), grads=B < 10, lengths=lengths)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_new_tokens_of_long_caches(cuda, dtype):
+    """three new tokens a row at places of their own (one row's first sees nothing), masked keys, and the same call in a graph whose
+    lengths, places and masks change between the replays"""
+    from mep_amd import diff_block as db
+    q, k, v, lam = case(4, 3, 1300, 4, 2, 20, 40, dtype)
+    start = torch.tensor([1297, 5, -1, 700], dtype=torch.int32, device='cuda')
+    lengths = torch.tensor([1300, 8, 3, 650], dtype=torch.int32, device='cuda')
+    mask = (torch.arange(4 * 1300, device='cuda').reshape(4, 1300) % 11 != 4).to(torch.uint8)
+    kw = dict(mask=mask, lengths=lengths, causal=True, q_start=start)
+    check(q, k, v, lam, **kw)
+    a = [t.detach() for t in (q, k, v, lam)]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        db.diff_attention(*a, **kw)
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = db.diff_attention(*a, **kw)
+    for step in range(4):
+        lengths.copy_(torch.tensor([1300 - 400 * step, 0 if step == 2 else 900, 1300, 64 * step], dtype=torch.int32))
+        start.copy_(torch.tensor([1000, 400 * step, 1297, -2], dtype=torch.int32))
+        mask[1].fill_(step % 2)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, db.diff_attention(*a, **kw))
+
+
 @pytest.mark.parametrize('size', [(2, 140, 70, 4, 4, 40, 160), (1, 140, 70, 8, 4, 40, 160), (1, 300, 70, 1, 1, 40, 160)])
 @pytest.mark.parametrize('causal', [False, True])
 def test_values_in_two_halves(cuda, size, causal):
