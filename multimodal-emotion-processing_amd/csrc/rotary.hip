@@ -10,7 +10,7 @@
 // Bound by memory: 2 D elements per head and token against ~20 operations per pair and token.  A thread
 // owns one 2V-channel item of one token (V pairs, or 2V copied channels), forms its V sines once and walks
 // the heads with them; the heads are split over threads only where tokens alone do not fill the chip.
-// 4 x 8192 tokens of 16 + 4 heads of 128 in bf16: 88 us, 3.8 TB/s.
+// 4 x 8192 tokens of 16 + 4 heads of 128 in bf16: 73 us, 4.6 TB/s.
 #include "elem.h"
 
 namespace {
@@ -109,8 +109,10 @@ bool launch_rotary(const mep_rotary_desc& d, hipStream_t st) {
     const int ni = np + (d.D - d.rot + 2 * V - 1) / (2 * V);
     const int64_t tok = (int64_t)d.B * d.T;
     const int heads = d.H[0] * d.M[0] > d.H[1] * d.M[1] || !d.x[1] ? d.H[0] * d.M[0] : d.H[1] * d.M[1];
-    // split the heads until 8 waves per compute unit are there (131,072 threads), at most one head each
-    int64_t hsplit = 131072 / (tok * ni);
+    // split the heads until two rounds of 32 waves per compute unit are there (1,048,576 threads), at most one head each: with more
+    // the sines are formed too often, with less the loads of a walk are too few in flight (32768 tokens of 20 heads: 88 us with 262,144
+    // or 524,288 threads, 73, 81 with 2,621,440)
+    int64_t hsplit = 1048576 / (tok * ni);
     hsplit = hsplit < 1 ? 1 : hsplit > heads ? heads : hsplit;
     if (tok * ni * hsplit >= (int64_t)1 << 32) return false;
     const int64_t blocks = (tok * ni * hsplit + ROT_THREADS - 1) / ROT_THREADS;
