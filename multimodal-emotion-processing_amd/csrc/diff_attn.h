@@ -966,13 +966,19 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
 }
 
 // ------------------------------------------------------------------ backward: D and dq
-// D_m = dO . (A_m v) is known beforehand only up to the roundings of the forward's out and second = A_2 v.  That error is some
-// 2^-9 of the sum of A_m^2 of the row in dP's units: nothing beside dS's own rounding where many keys carry the row, but all of dS
-// where one does.  So the row sums of A_m dP are formed beside dS without any rounding to 16 bits, and their difference is put right:
-// dq_m -= (D_m - estimate) A_m k_m.  At DK = 32, E_m k_m is summed beside dS (BESIDE).  Wider heads have no registers for that
-// (accumulators that pass through the accumulation registers for every tile cost more than a second pass): there a second pass
-// over the keys forms it where a row of the workgroup rests on fewer than 32 keys (sum A_m^2 > 1 / 32; at that it is a thirtieth of
-// dS's rounding).  (In fp32 the estimate is as good as the sum.)  The sums are also lam's gradient and what dk needs.
+// D_m = dO . (A_m v) is known beforehand only up to the roundings of the forward's out and second = A_2 v.  The error's effect on dq
+// is error * sum A_m k_m, beside dS's own rounding, which comes to about r = u sqrt(sum (A_m (dP - D_m))^2) in the same units (u = 2^-9,
+// in float16 2^-12).  Where the values have no mean, the error is about r (out shrinks with the keys as r does); where they have one, out
+// keeps its size and the error is many times r (4096 keys, means as large as the deviations: 100 r, and dq 5 % off); and where one
+// key carries the row, r itself is that error.  So the row sums of A_m dP are formed beside dS without any rounding to 16 bits, and the
+// difference is put right: dq_m -= (D_m - estimate) sum A_m k_m.  At DK = 32, E_m k_m is summed beside dS (BESIDE).  Wider heads have no
+// registers for that (accumulators that pass through the accumulation registers for every tile cost more than a second pass): there
+// a second pass over the keys forms it where the error of a wave's 32 rows has a root mean square over 3 r, or a row rests on few
+// keys (a weight over 1 / 4).  (Without a mean that is 1.3 r, 2.5 r at most in 4096 waves.  Single rows reach 8 r, and one pass
+// taken twice keeps its whole launch waiting: asked of each row, B 4, T 2048, 8 heads, 64 / 128 took 185 us instead of 143.)  What the
+// second pass costs where keys and values have a mean (as large as the deviation, bf16): 64 / 128 at B 2, T 4096, causal 208 -> 313 us,
+// at B 4, T 2048 152 -> 229, 128 / 128 there 282 -> 474.  (In fp32 the estimate is as good as the sum.)  The sums are also lam's
+// gradient and what dk needs.
 template <int TYPE, int DK, int DV, int KS>
 __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
     typedef RowShape<TYPE, DK, DV, KS> Sh;
@@ -1035,7 +1041,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
     const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * srow);      // m1, 1 / l1, m2, 1 / l2
 
     constexpr bool BESIDE = TYPE != MEP_F32 && DK == 32, CORR = TYPE != MEP_F32 && DK != 32;
-    float sum1 = 0.f, sum2 = 0.f, sq1 = 0.f, sq2 = 0.f;
+    float sum1 = 0.f, sum2 = 0.f, sq1 = 0.f, sq2 = 0.f, top1 = 0.f, top2 = 0.f;
     floatx16 a1[DK / 32], a2[DK / 32], b1, b2;
     b1 = b2 = zero16();
 #pragma unroll
@@ -1081,16 +1087,18 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
                 const float e1 = ex.at(s1[r], st[0]), e2 = ex.at(s2[r], st[2]);
                 u1 = fmaf(e1, dp[r], u1);
                 u2 = fmaf(e2, dp[r], u2);
-                if constexpr (CORR) {
-                    sq1 = fmaf(e1, e1, sq1);
-                    sq2 = fmaf(e2, e2, sq2);
-                }
                 if constexpr (BESIDE) {
                     s1[r] = e1;
                     s2[r] = e2;
                 } else {
                     s1[r] = e1 * (dp[r] - d1);
                     s2[r] = e2 * (dp[r] - d2);
+                }
+                if constexpr (CORR) {
+                    sq1 = fmaf(s1[r], s1[r], sq1);
+                    sq2 = fmaf(s2[r], s2[r], sq2);
+                    top1 = fmaxf(top1, e1);
+                    top2 = fmaxf(top2, e2);
                 }
             }
             sum1 += u1;
@@ -1132,6 +1140,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
         sq1 = half_sum(sq1);
         sq2 = half_sum(sq2);
     }
+    const bool few = CORR && w.live && fmaxf(top1 * st[1], top2 * st[3]) > 0.25f;      // (some lane has the row's largest)
     if constexpr (KS == 2) {
         const int r = wave * 32 + (threadIdx.x & 31);
         if (h == 0) Meet[half][r] = f32x4{sum1, sum2, sq1, sq2};
@@ -1150,8 +1159,13 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
     }
     if (!bd.dq) return;
     if constexpr (CORR) {
-        const bool few = w.live && fmaxf(sq1 * st[1] * st[1], sq2 * st[3] * st[3]) > 0.03125f;
-        if (__syncthreads_or(few)) {
+        constexpr float u = TYPE == MEP_F16 ? 0x1p-12f : 0x1p-9f;
+        auto off = [](float error, float r) {      // (error / r)^2, finite
+            const float x = error == 0.f ? 0.f : fminf(fabsf(error) / r, 1e3f);
+            return x * x;
+        };
+        const float x = w.live ? fmaxf(off(d1 - sum1, u * st[1] * sqrtf(sq1)), off(d2 - sum2, u * st[3] * sqrtf(sq2))) : 0.f;
+        if (__syncthreads_or(few || wave_sum(x) > 2 * 32 * 9.f)) {      // (a row is in two lanes)
             floatx16 k1[DK / 32], k2[DK / 32];
 #pragma unroll
             for (int n = 0; n < DK / 32; ++n) k1[n] = k2[n] = zero16();

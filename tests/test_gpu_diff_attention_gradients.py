@@ -1,0 +1,90 @@
+"""Gradients of mep_amd.diff_block.diff_attention by their whole error (the Frobenius norm), against the 64-bit form: keys and values
+that have a mean."""
+import math
+
+import pytest
+import torch
+
+from tests import diff_block_ref as ref
+from tests.test_gpu_diff_attention import rand
+
+pytestmark = pytest.mark.gpu
+HALVES = [torch.bfloat16, torch.float16]
+
+
+def case(B, Tq, Tk, H, G, d, dv, dtype, k_mean, v_mean, v_std=1.0, seed=1):
+    """keys and values with a mean of either sign in each channel"""
+    g = torch.Generator().manual_seed(seed + 7)
+    sign = lambda *s: (torch.randint(0, 2, s, generator=g) * 2 - 1).float()  # noqa: E731
+    make = lambda shape, mean, std, at, tail: (  # noqa: E731
+        (torch.randn(shape, generator=torch.Generator().manual_seed(at)) + mean * sign(*tail)) * std).to(dtype).cuda().requires_grad_()
+    q = rand((B, Tq, H, 2, d), dtype, seed)
+    k = make((B, Tk, G, 2, d), k_mean, 1.0, seed + 1, (2, d))
+    v = make((B, Tk, G, dv), v_mean, v_std, seed + 2, (dv,))
+    lam = (torch.rand(H, generator=g) * 0.6 + 0.2).cuda().requires_grad_()
+    return q, k, v, lam
+
+
+def check(q, k, v, lam, dout, causal=False):
+    """The error of a whole gradient.  With half = half a step of the type, dS = A (dP - D):
+
+    dq   rounding dS adds at most half sqrt(sum dS^2 |k|^2) / sqrt(3) on average, independent from key to key.  A row's D may be off
+         from what the row's sums say, by up to 3 times half / 2 sqrt(sum dS^2) in the root mean square over 32 rows before that is
+         put right: 1.5 half sqrt(sum dS^2), which meets |sum A k| <= sqrt(sum A |k|^2).  Both together are under 2 half of
+         S = sqrt(sum over rows of (sum dS^2) (sum A |k|^2)) plus sqrt(sum dS^2 |k|^2).
+    dk   sums dS^T q of rows with their D as summed: 2 half sqrt(sum dS^2 |q|^2) for its 0.6.
+    dv   sums P^T dO: likewise.
+    Each is rounded once more (half, and half a subnormal step of every element).  float32's own sums are far below."""
+    from mep_amd import diff_block as db
+    B, Tq, H, _, d = q.shape
+    Tk, G = k.shape[1], k.shape[2]
+    n, sc = H // G, d ** -0.5
+    half = ref.half_step(q.dtype)
+    tiny = torch.finfo(q.dtype).smallest_normal * half
+    got = torch.autograd.grad(db.diff_attention(q, k, v, lam, causal=causal), (q, k, v, lam), dout)
+    w = [ref.wide(t) for t in (q, k, v, lam)]
+    ok = ref.allowed(B, Tq, Tk, None, None, causal, None)
+    exact = torch.autograd.grad(ref.diff_attention(*w, ok), w, dout.cpu().double())
+    with torch.no_grad():
+        kk, vv, do = w[1].repeat_interleave(n, 2), w[2].repeat_interleave(n, 2), dout.cpu().double()
+        s = torch.einsum('bthmd,bshmd->bhmts', w[0], kk) * sc
+        a = torch.softmax(s.masked_fill(~ok[:, None, None], -1e300), -1)
+        l = w[3].reshape(1, H, 1, 1)
+        dp = torch.einsum('bthe,bshe->bhts', do, vv)
+        ds = a * (dp[:, :, None] - (a * dp[:, :, None]).sum(-1, keepdim=True)) * torch.stack([torch.ones_like(l), l], 2) * sc
+        k2 = (kk * kk).sum(-1).permute(0, 2, 3, 1)[:, :, :, None]          # [B, H, 2, 1, Tk]
+        q2 = (w[0] * w[0]).sum(-1).permute(0, 2, 3, 1)[..., None]
+        ds2 = ds * ds
+        tq = math.sqrt(float((ds2 * k2).sum())) + math.sqrt(float((ds2.sum(-1) * (a * k2).sum(-1)).sum()))
+        tk = math.sqrt(float((ds2 * q2).sum()))
+        p = a[:, :, 0] - l * a[:, :, 1]
+        tv = math.sqrt(float((p * p * (do * do).sum(-1).permute(0, 2, 1)[..., None]).sum()))
+    report = []
+    for name, x, e, t in zip(('dq', 'dk', 'dv'), got, exact, (tq, tk, tv)):
+        x = x.cpu().double()
+        norm = float(e.norm())
+        tol = half * (norm + 2 * t) + tiny * math.sqrt(e.numel())
+        err = float((x - e).norm())
+        report.append('%s %.2e of %.2e' % (name, err / norm, tol / norm))
+        if not err <= tol:
+            report[-1] += ' OFF'
+    report = '; '.join(report)
+    print(report, flush=True)
+    assert 'OFF' not in report, report
+
+
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('k_mean,v_mean', [(0.0, 0.0), (1.0, 1.0), (1.0, 3.0), (3.0, 3.0), (0.0, 3.0)])
+@pytest.mark.parametrize('size', [(1, 128, 4096, 1, 1, 64, 128), (1, 1024, 1024, 2, 1, 64, 64), (1, 200, 1500, 2, 1, 128, 128),
+                                  (1, 130, 1000, 1, 1, 128, 256), (1, 200, 1500, 2, 1, 32, 64), (16, 160, 1024, 8, 8, 64, 128)])
+def test_means(cuda, size, k_mean, v_mean, dtype):
+    """whole rows, shared heads, a row's keys shared by two waves (few workgroups) and not (the last: 256)"""
+    if size[0] > 1 and (k_mean, v_mean) not in ((1.0, 1.0), (3.0, 3.0)):
+        pytest.skip('the large case, at two means')
+    a = case(*size, dtype, k_mean, v_mean)
+    check(*a, rand((*size[:2], size[3], size[6]), dtype, 77, grad=False))
+
+
+@pytest.mark.parametrize('dtype', HALVES)
+def test_means_causal(cuda, dtype):
+    check(*case(2, 700, 700, 4, 2, 64, 128, dtype, 2.0, 2.0), rand((2, 700, 4, 128), dtype, 77, grad=False), causal=True)
