@@ -806,7 +806,7 @@ typedef struct {
     uint64_t dlam;               /* fp32 [H] for a lam shared by batch and queries, or 0          */
     uint64_t dlam_rows;          /* fp32 [B, Tq, H], or 0                                         */
     uint64_t delta;              /* workspace, fp32 [B, H, Tq, 4]                                 */
-    uint64_t workspace;          /* mep_diff_attn_bwd_workspace bytes, or 0: the rows are not split */
+    uint64_t workspace;          /* mep_diff_attn_bwd_workspace bytes, 16-byte aligned, or (not in float16) 0: the rows are not split */
 } mep_diff_attn_bwd_desc;
 int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t stream);
 /* y [B, T, H, M, n rounded up to 16 bytes] = x [B, T, H, M, n] of any strides (sN: of the channels), zeros behind n */
@@ -820,7 +820,8 @@ int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_t stream);
 /* bytes that a forward of these sizes (B, Tq, Tk, H, G, d, dv, type) uses to split its keys over workgroups: 0 where it does
  * not; < 0: MEP_EINVAL */
 int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc);
-int64_t mep_diff_attn_bwd_workspace(const mep_diff_attn_desc* desc);      /* of a backward that splits the rows */
+/* of a backward that splits the rows; in float16 of any: the sizes of the values and the upstream gradient, which its operands are scaled by */
+int64_t mep_diff_attn_bwd_workspace(const mep_diff_attn_desc* desc);
 
 /* ---------------------------------------------------------------- misc */
 int mep_abi_version(void);

@@ -32,7 +32,7 @@ constexpr int DA_THREADS = 256, DA_WAVES = 4, DA_ROWS = 32 * DA_WAVES;
 constexpr float DA_LOG2E = 1.4426950408889634f;
 constexpr float DA_MIN = -1.0e30f;      // the running maximum's start: finite, so that masked scores (-inf) give 2^-inf = 0
 constexpr unsigned DA_NOWHERE = 0x80000000u, DA_SPAN = 0x7fffffffu;   // a DMA offset behind the span reads zeros
-enum { DA_FWD, DA_FWD_TWO, DA_BWD_Q, DA_BWD_Q_TWO, DA_BWD_KV, DA_SPLIT };
+enum { DA_FWD, DA_FWD_TWO, DA_SIZES, DA_BWD_Q, DA_BWD_Q_TWO, DA_BWD_KV, DA_SPLIT };
 
 // keys of a tile of k_diff_split: 64 where two tiles fit 160 KB of LDS
 constexpr int da_split_keys(int type, int dk, int dv) { return (type == MEP_F32 ? 4 : 2) * 2 * 64 * (2 * dk + dv) <= 160 * 1024 ? 64 : 32; }
@@ -430,6 +430,103 @@ MEP_DEV int thread_again() {
     int t = threadIdx.x;
     asm volatile("" : "+v"(t));
     return t;
+}
+
+// ------------------------------------------------------------------ float16: the range of the backward's operands
+// float16 is exact to 2^-11 between 2^-14 and 2^16 only, and dS and P are of any size (a loss scale; the weights of many keys).  So their
+// columns are multiplied by powers of two before they are rounded, and the accumulators divided by them: with
+//   |dP - D| <= 2 sum|dO_t| max|v| (dq, by row),  2 max|dO_t| sum|v_k| (dk, by key),  A_1, |lam| A_2 <= w = max(1, |lam|),  |P| <= 2 w
+// no value passes 2^15, and where bound and typical value are 2^6 apart (128 channels of either sign), what is 2^-19 of the
+// typical value is still above 2^-24.  The maxima over a (batch row, key head) come from this kernel, a pass over the values and the
+// upstream gradient: B 4, T 2048, 8 heads, 64 / 128 11 us (B 2, T 1024 7), dq 155 us and dk and dv 277, unscaled 155 and 260.  (Found
+// beside the products instead, with the accumulators scaled down whenever a value passes the range: 172 and 298; at 128 / 128 437 and
+// 715, with this kernel 287 and 610.)
+// part p of a (batch row, key head): max |v|, max |dO| w, max w
+constexpr int DA_SIZE_PARTS = 64;
+struct Sizes { float v, o, w; };
+template <int TYPE>
+struct Fit {
+    static constexpr bool ON = TYPE == MEP_F16;
+    const MEP_G f32x4* parts;
+    int n;
+    MEP_DEV Fit(uint64_t sizes, int count, const mep_diff_attn_desc& d, const Job& j) : parts(G<const f32x4>(sizes) + ((int64_t)j.b * d.G + j.g) * count), n(count) {}
+    MEP_DEV Sizes all() const {
+        Sizes z = {0.f, 0.f, 1.f};
+        if ((int)(threadIdx.x & 63) < n) {
+            const f32x4 x = parts[threadIdx.x & 63];
+            z = {x[0], x[1], x[2]};
+        }
+        for (int o = 32; o; o /= 2) {
+            z.v = fmaxf(z.v, __shfl_xor(z.v, o));
+            z.o = fmaxf(z.o, __shfl_xor(z.o, o));
+            z.w = fmaxf(z.w, __shfl_xor(z.w, o));
+        }
+        return z;
+    }
+    // the n of the power of two that takes values up to `most` to under 2^15
+    static MEP_DEV int lift(float most) { return max(-120, min(60, 15 - __builtin_amdgcn_frexp_expf(most))); }
+};
+// sum |x| over a lane's operands and its other half's
+template <class M, class Op, int N>
+MEP_DEV float size_sum(const Op& x) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const typename M::Frag f = x.at(i);
+#pragma unroll
+        for (int e = 0; e < M::E; ++e) s += fabsf((float)f[e]);
+    }
+    return half_sum(s);
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(DA_THREADS) void k_diff_sizes(mep_diff_attn_bwd_desc bd, uint64_t sizes, int parts) {
+    typedef Mat<TYPE> M;
+    typedef typename M::T T;
+    const mep_diff_attn_desc& d = bd.f;
+    __shared__ float Part[3][DA_WAVES];
+    Job j;
+    const int bg = blockIdx.x / parts, part = blockIdx.x - bg * parts, chunks = (d.dv + M::E - 1) / M::E;
+    j.b = bg / d.G;
+    j.g = bg - j.b * d.G;
+    fill_job(d, j);
+    auto largest = [&](const MEP_G T* p) {
+        const typename M::Frag f = *reinterpret_cast<const MEP_G typename M::Frag*>(p);
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < M::E; ++e) m = fmaxf(m, fabsf((float)f[e]));
+        return m;
+    };
+    float z[3] = {0.f, 0.f, 1.f};
+    // this part's keys: those that are read; and rows
+    const int k0 = (int)((int64_t)j.len * part / parts), k1 = (int)((int64_t)j.len * (part + 1) / parts);
+    const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < (int64_t)(k1 - k0) * chunks; i += DA_THREADS) {
+        const int64_t key = k0 + i / chunks;
+        if (d.mask_form != 1 || mask_at(d, (int64_t)j.b * d.m_sB + key * d.m_sK)) z[0] = fmaxf(z[0], largest(vp + key * d.v_sT + i % chunks * M::E));
+    }
+    const int r0 = (int)((int64_t)j.rows * part / parts), r1 = (int)((int64_t)j.rows * (part + 1) / parts);
+    const MEP_G T* op = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
+    const MEP_G float* lp = G<const float>(d.lam) + (int64_t)j.b * d.lam_sB + (int64_t)j.g * j.n * d.lam_sH;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < (int64_t)(r1 - r0) * chunks; i += DA_THREADS) {
+        const int row = r0 + (int)(i / chunks), t = row / j.n, head = row - t * j.n;
+        const float w = fmaxf(1.f, fabsf(lp[(int64_t)t * d.lam_sT + (int64_t)head * d.lam_sH]));
+        z[1] = fmaxf(z[1], w * largest(op + (int64_t)t * bd.o_sT + (int64_t)head * bd.o_sH + i % chunks * M::E));
+        z[2] = fmaxf(z[2], w);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        for (int o = 32; o; o /= 2) z[i] = fmaxf(z[i], __shfl_xor(z[i], o));
+        if ((threadIdx.x & 63) == 0) Part[i][threadIdx.x >> 6] = z[i];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) z[i] = fmaxf(fmaxf(Part[i][0], Part[i][1]), fmaxf(Part[i][2], Part[i][3]));
+        G<f32x4>(sizes)[blockIdx.x] = f32x4{z[0], z[1], z[2], 0.f};
+    }
 }
 
 // The keys and values of a (batch, key head), tile by tile
@@ -980,7 +1077,7 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
 // at B 4, T 2048 152 -> 229, 128 / 128 there 282 -> 474.  (In fp32 the estimate is as good as the sum.)  The sums are also lam's
 // gradient and what dk needs.
 template <int TYPE, int DK, int DV, int KS>
-__global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks) {
+__global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks, uint64_t sizes, int parts) {
     typedef RowShape<TYPE, DK, DV, KS> Sh;
     typedef Geo<TYPE, DK, DV> Ge;
     typedef typename Ge::M M;
@@ -1041,6 +1138,13 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
     const f32x4 st = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * srow);      // m1, 1 / l1, m2, 1 / l2
 
     constexpr bool BESIDE = TYPE != MEP_F32 && DK == 32, CORR = TYPE != MEP_F32 && DK != 32;
+    float up = 1.f;                             // dS, and the estimates with it, times up (Fit)
+    if constexpr (Fit<TYPE>::ON) {
+        up = ldexpf(1.f, Fit<TYPE>::lift(2.f * size_sum<M, Operand<M, Ge::NV, HOLD>, Ge::NV>(g) * Fit<TYPE>(sizes, parts, d, j).all().v));
+        d1 *= up;
+        d2 *= up;
+    }
+    auto above = [&](float dp, float estimate) { return Fit<TYPE>::ON ? fmaf(dp, up, -estimate) : dp - estimate; };
     float sum1 = 0.f, sum2 = 0.f, sq1 = 0.f, sq2 = 0.f, top1 = 0.f, top2 = 0.f;
     floatx16 a1[DK / 32], a2[DK / 32], b1, b2;
     b1 = b2 = zero16();
@@ -1091,8 +1195,8 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
                     s1[r] = e1;
                     s2[r] = e2;
                 } else {
-                    s1[r] = e1 * (dp[r] - d1);
-                    s2[r] = e2 * (dp[r] - d2);
+                    s1[r] = e1 * above(dp[r], d1);
+                    s2[r] = e2 * above(dp[r], d2);
                 }
                 if constexpr (CORR) {
                     sq1 = fmaf(s1[r], s1[r], sq1);
@@ -1112,8 +1216,8 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s1[r] *= dp[r] - d1;
-                    s2[r] *= dp[r] - d2;
+                    s1[r] *= above(dp[r], d1);
+                    s2[r] *= above(dp[r], d2);
                 }
             }
 #pragma unroll
@@ -1164,7 +1268,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
             const float x = error == 0.f ? 0.f : fminf(fabsf(error) / r, 1e3f);
             return x * x;
         };
-        const float x = w.live ? fmaxf(off(d1 - sum1, u * st[1] * sqrtf(sq1)), off(d2 - sum2, u * st[3] * sqrtf(sq2))) : 0.f;
+        const float x = w.live ? fmaxf(off(above(-sum1, -d1), u * st[1] * sqrtf(sq1)), off(above(-sum2, -d2), u * st[3] * sqrtf(sq2))) : 0.f;
         if (__syncthreads_or(few || wave_sum(x) > 2 * 32 * 9.f)) {      // (a row is in two lanes)
             floatx16 k1[DK / 32], k2[DK / 32];
 #pragma unroll
@@ -1206,16 +1310,16 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
             for (int n = 0; n < DK / 32; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    a1[n][r] = fmaf(k1[n][r], d1 - sum1, a1[n][r]);
-                    a2[n][r] = fmaf(k2[n][r], d2 - sum2, a2[n][r]);
+                    a1[n][r] = fmaf(k1[n][r], above(-sum1, -d1), a1[n][r]);
+                    a2[n][r] = fmaf(k2[n][r], above(-sum2, -d2), a2[n][r]);
                 }
         }
     }
     if constexpr (BESIDE) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            a1[0][r] = fmaf(b1[r], d1 - sum1, a1[0][r]);
-            a2[0][r] = fmaf(b2[r], d2 - sum2, a2[0][r]);
+            a1[0][r] = fmaf(b1[r], above(-sum1, -d1), a1[0][r]);
+            a2[0][r] = fmaf(b2[r], above(-sum2, -d2), a2[0][r]);
         }
     }
     tile_sync();                             // the tiles are free
@@ -1233,8 +1337,9 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
     };
     const bool whole = d.d % M::E == 0;
     T* mine = Buf + wave * 32 * (da_piece(DK) + M::E);
-    write_rows<M>(mine, a1, st[1] * d.scale, d.d, whole, [&](int r) { return row_at(0, r); });
-    write_rows<M>(mine, a2, -lam * st[3] * d.scale, d.d, whole, [&](int r) { return row_at(1, r); });
+    const float f = Fit<TYPE>::ON ? d.scale / up : d.scale;
+    write_rows<M>(mine, a1, st[1] * f, d.d, whole, [&](int r) { return row_at(0, r); });
+    write_rows<M>(mine, a2, -lam * st[3] * f, d.d, whole, [&](int r) { return row_at(1, r); });
 }
 
 // ------------------------------------------------------------------ backward: dk and dv
@@ -1285,7 +1390,7 @@ MEP_DEV floatx16 row_values(const bf16x8_da* x) {
 }
 
 template <int KW, int TYPE, int DK, int DV>
-__global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1 : 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks, int splits) {
+__global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1 : 2) void k_diff_bwd_kv(mep_diff_attn_bwd_desc bd, int blocks, int splits, uint64_t sizes, int parts) {
     typedef Geo<TYPE, DK, DV> Ge;
     typedef KvShape<KW, TYPE, DK, DV> Sh;
     typedef typename Ge::M M;
@@ -1399,8 +1504,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
     const bool wave_on = __ballot(on) != 0, all_on = __ballot(on) == ~0ull;
     if (rbeg < rend) put_stats(0);
 
-    // A_1 and lam A_2 of the rows from rs on
-    auto maps = [&](int buf, int sub, int rs, floatx16& s1, floatx16& s2) {
+    // A_1 and lam A_2 of the rows from rs on, times 2^lift
+    auto maps = [&](int buf, int sub, int rs, float lift, floatx16& s1, floatx16& s2) {
         const T* qt = Buf + buf * Ge::TSZ;
         if constexpr (PARTS) {
             s1 = row_values(Xs[buf][X_LSE1] + 32 * sub);
@@ -1437,8 +1542,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
         if constexpr (PARTS) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s1[r] = exp2_fast(s1[r] * c);
-                s2[r] = exp2_fast(s2[r] * c);
+                s1[r] = exp2_fast(Fit<TYPE>::ON ? fmaf(s1[r], c, lift) : s1[r] * c);
+                s2[r] = exp2_fast(Fit<TYPE>::ON ? fmaf(s2[r], c, lift) : s2[r] * c);
             }
             if (Neg[buf]) {
                 const floatx16 sg = row_values(Xs[buf][X_SIGN] + 32 * sub);
@@ -1532,6 +1637,15 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
                 }
         }
     };
+    // the powers of two that P and dS are taken to float16 with (Fit)
+    int lift_v = 0, lift_k = 0;
+    auto fit = [&](const V* v) {
+        if constexpr (Fit<TYPE>::ON) {
+            const Sizes z = Fit<TYPE>(sizes, parts, d, j).all();
+            lift_v = Fit<TYPE>::lift(2.f * z.w);
+            if (v) lift_k = Fit<TYPE>::lift(2.f * size_sum<M, V, Ge::NV>(*v) * z.o);
+        }
+    };
     // with splits, a split's sums in fp32: [splits][B, Tk, G][2 d + dv]
     auto put_part = [&](const auto& acc, int at, int n, float f) {
         if (key >= d.Tk) return;
@@ -1546,17 +1660,19 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
             }
     };
     auto put_v = [&](T* mine) {
-        if (splits > 1) return put_part(av, 2 * d.d, d.dv, 1.f);
-        write_rows<M>(mine, av, 1.f, d.dv, d.dv % M::E == 0, [&](int r) { return key_at(bd.dv, r, d.dv); });
+        const float f = Fit<TYPE>::ON ? ldexpf(1.f, -lift_v) : 1.f;
+        if (splits > 1) return put_part(av, 2 * d.d, d.dv, f);
+        write_rows<M>(mine, av, f, d.dv, d.dv % M::E == 0, [&](int r) { return key_at(bd.dv, r, d.dv); });
     };
     auto put_k = [&](T* mine) {
+        const float f = Fit<TYPE>::ON ? ldexpf(d.scale, -lift_k) : d.scale;
         if (splits > 1) {
-            put_part(a1, 0, d.d, d.scale);
-            put_part(a2, d.d, d.d, -d.scale);
+            put_part(a1, 0, d.d, f);
+            put_part(a2, d.d, d.d, -f);
             return;
         }
-        write_rows<M>(mine, a1, d.scale, d.d, d.d % M::E == 0, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
-        write_rows<M>(mine, a2, -d.scale, d.d, d.d % M::E == 0, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
+        write_rows<M>(mine, a1, f, d.d, d.d % M::E == 0, [&](int r) { return key_at(bd.dk, r, 2 * d.d); });
+        write_rows<M>(mine, a2, -f, d.d, d.d % M::E == 0, [&](int r) { MEP_G T* p = key_at(bd.dk, r, 2 * d.d); return p ? p + d.d : p; });
     };
     T* vbuf = Buf + wave % KW * 32 * (da_piece(DV) + M::E);
     T* kbuf = Buf + KW * 32 * (da_piece(DV) + M::E) + wave % KW * 32 * (da_piece(DK) + M::E);
@@ -1564,12 +1680,18 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
         clear_v();
         clear_k();
         const V v(vp, d.dv, on);
+        fit(&v);
+        const float more = Fit<TYPE>::ON ? ldexpf(1.f, lift_k - lift_v) : 1.f;
         walk([&](int buf, int sub, int rs) {
             const T* qt = Buf + buf * Ge::TSZ;
             floatx16 s1, s2, p;
-            maps(buf, sub, rs, s1, s2);
+            maps(buf, sub, rs, lift_v, s1, s2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] = s1[r] - s2[r];
+            if constexpr (Fit<TYPE>::ON) {
+                s1 *= more;
+                s2 *= more;
+            }
             add_v(qt + Ge::KSZ, sub, p);
             add_k(v, qt, buf, sub, s1, s2);
         });
@@ -1577,9 +1699,10 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
         put_k(kbuf);
     } else if (for_v) {
         clear_v();
+        fit(nullptr);
         walk([&](int buf, int sub, int rs) {
             floatx16 s1, s2;
-            maps(buf, sub, rs, s1, s2);
+            maps(buf, sub, rs, lift_v, s1, s2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s1[r] -= s2[r];
             add_v(Buf + buf * Ge::TSZ + Ge::KSZ, sub, s1);
@@ -1588,9 +1711,10 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
     } else {
         clear_k();
         const V v(vp, d.dv, on);
+        fit(&v);
         walk([&](int buf, int sub, int rs) {
             floatx16 s1, s2;
-            maps(buf, sub, rs, s1, s2);
+            maps(buf, sub, rs, lift_k, s1, s2);
             add_k(v, Buf + buf * Ge::TSZ, buf, sub, s1, s2);
         });
         put_k(kbuf);
@@ -1602,18 +1726,18 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
 constexpr int da_kw(int type, int dk) { return dk >= 128 && type != MEP_F32 ? 2 : 4; }
 
 template <int TYPE, int DK, int DV>
-void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st) {      // splits: DA_FWD's parts, DA_SPLIT's groups
+void da_instance(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, uint64_t sizes, int parts) {      // splits: DA_FWD's parts, DA_SPLIT's groups
     constexpr int PV = da_piece(DV);
     if (what == DA_FWD) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, PV, 1>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
     else if (what == DA_FWD_TWO) {
         if constexpr (da_two(TYPE, DK, PV)) hipLaunchKernelGGL((k_diff_fwd<TYPE, DK, PV, 2>), dim3(grid), dim3(DA_THREADS), 0, st, d, blocks, splits);
     } else if (what == DA_BWD_Q_TWO) {
-        if constexpr (da_two(TYPE, DK, DV)) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV, 2>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+        if constexpr (da_two(TYPE, DK, DV)) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV, 2>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks, sizes, parts);
     }
     else if (what == DA_SPLIT) hipLaunchKernelGGL((k_diff_split<TYPE, DK, da_piece(DV)>), dim3(grid), dim3(DA_SPLIT_THREADS), 0, st, d, blocks, splits);
-    else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV, 1>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks);
+    else if (what == DA_BWD_Q) hipLaunchKernelGGL((k_diff_bwd_q<TYPE, DK, DV, 1>), dim3(grid), dim3(DA_THREADS), 0, st, *b, blocks, sizes, parts);
     else hipLaunchKernelGGL((k_diff_bwd_kv<da_kw(TYPE, DK), TYPE, DK, DV>), dim3(grid),
-                            dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks, splits);
+                            dim3(KvShape<da_kw(TYPE, DK), TYPE, DK, DV>::THREADS), 0, st, *b, blocks, splits, sizes, parts);
 }
 
 // the smallest instance that holds the head widths
@@ -1624,18 +1748,22 @@ inline int da_value_width(int d, int dv) {
     return dk == 32 ? (dv <= 32 ? 32 : 64) : dk == 64 ? (dv <= 64 ? 64 : 128) : (dv <= 128 ? 128 : 256);
 }
 template <int TYPE>
-void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all) {
+void da_run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all, uint64_t sizes, int parts) {
+    if (what == DA_SIZES) {
+        if constexpr (Fit<TYPE>::ON) hipLaunchKernelGGL(k_diff_sizes<TYPE>, dim3(grid), dim3(DA_THREADS), 0, st, *b, sizes, parts);
+        return;
+    }
     const int dk = da_width(d.d, all), dv = da_value_width(d.d, all);      // all: the values' whole width
-    if (dk == 32 && dv == 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, splits, st);
-    else if (dk == 32) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, splits, st);
-    else if (dk == 64 && dv == 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, splits, st);
-    else if (dk == 64) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, splits, st);
-    else if (dv == 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, splits, st);
-    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, splits, st);
+    if (dk == 32 && dv == 32) da_instance<TYPE, 32, 32>(what, d, b, grid, blocks, splits, st, sizes, parts);
+    else if (dk == 32) da_instance<TYPE, 32, 64>(what, d, b, grid, blocks, splits, st, sizes, parts);
+    else if (dk == 64 && dv == 64) da_instance<TYPE, 64, 64>(what, d, b, grid, blocks, splits, st, sizes, parts);
+    else if (dk == 64) da_instance<TYPE, 64, 128>(what, d, b, grid, blocks, splits, st, sizes, parts);
+    else if (dv == 128) da_instance<TYPE, 128, 128>(what, d, b, grid, blocks, splits, st, sizes, parts);
+    else da_instance<TYPE, 128, 256>(what, d, b, grid, blocks, splits, st, sizes, parts);
 }
 
-void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all);
-void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all);
-void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all);
+void da_run_f32(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all, uint64_t sizes, int parts);
+void da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all, uint64_t sizes, int parts);
+void da_run_f16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all, uint64_t sizes, int parts);
 
 }  // namespace mep

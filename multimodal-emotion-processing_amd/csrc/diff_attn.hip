@@ -176,10 +176,10 @@ int64_t split_bytes(const mep_diff_attn_desc& d, const Split& s) {
     return ((d.B + 4) / 4 * 4 + parts * 2 * split_floats((int)(rows < 32 ? rows : 32), da_piece(d.dv))) * 4;
 }
 
-void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, hipStream_t st, int dv) {
-    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, st, dv);
-    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, st, dv);
-    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, st, dv);
+void run(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, int64_t grid, int blocks, int splits, hipStream_t st, int dv, uint64_t sizes = 0, int parts = 0) {
+    if (d.type == MEP_F32) da_run_f32(what, d, b, (unsigned)grid, blocks, splits, st, dv, sizes, parts);
+    else if (d.type == MEP_BF16) da_run_bf16(what, d, b, (unsigned)grid, blocks, splits, st, dv, sizes, parts);
+    else da_run_f16(what, d, b, (unsigned)grid, blocks, splits, st, dv, sizes, parts);
 }
 
 // Into how many workgroups the rows of a block of keys are split: until there are two for every compute unit, 4 tiles of rows each at
@@ -192,6 +192,20 @@ int kv_splits(const mep_diff_attn_desc& d) {
     int64_t n = 512 / grid;
     n = n > tiles / 4 ? tiles / 4 : n;
     return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+
+// bytes of the splits' sums, and behind them of k_diff_sizes' parts: 32 keys or rows each, DA_SIZE_PARTS at most (a lane's worth)
+int64_t kv_bytes(const mep_diff_attn_desc& d) {
+    const int n = kv_splits(d);
+    return n > 1 ? ((int64_t)n * d.B * d.Tk * d.G * (2 * d.d + d.dv) * 4 + 15) / 16 * 16 : 0;
+}
+int size_parts(const mep_diff_attn_desc& d) {
+    const int64_t rows = (int64_t)d.Tq * (d.H / d.G), pairs = (int64_t)d.B * d.G;
+    if (d.type != MEP_F16 || pairs == 0) return 0;
+    int64_t n = ((rows > d.Tk ? rows : d.Tk) + 31) / 32;
+    n = n > DA_SIZE_PARTS ? DA_SIZE_PARTS : n;
+    if (n * pairs >= 1 << 23) n = ((1 << 23) - 1) / pairs;
+    return (int)(n < 1 ? 1 : n);
 }
 
 // Whether two waves share a row's keys (KS = 2) in a launch of `grid` workgroups of 128 rows, over dv channels of the values at a time:
@@ -296,8 +310,7 @@ extern "C" int mep_diff_attn_fwd(const mep_diff_attn_desc* desc, mep_stream_t st
 
 extern "C" int64_t mep_diff_attn_bwd_workspace(const mep_diff_attn_desc* desc) {
     if (!desc || !attn_shape_ok(*desc)) { mep_set_error("mep_diff_attn_bwd_workspace: invalid descriptor"); return MEP_EINVAL; }
-    const int n = kv_splits(*desc);
-    return n > 1 ? (int64_t)n * desc->B * desc->Tk * desc->G * (2 * desc->d + desc->dv) * 4 : 0;
+    return kv_bytes(*desc) + (int64_t)size_parts(*desc) * desc->B * desc->G * 16;
 }
 
 extern "C" int64_t mep_diff_attn_workspace(const mep_diff_attn_desc* desc) {
@@ -319,19 +332,26 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
         mep_set_error("mep_diff_attn_bwd: rows that cannot be read 16 bytes at a time");
         return MEP_EINVAL;
     }
+    const int parts = rows || keys ? size_parts(d) : 0;
+    if (parts && (!b.workspace || b.workspace % 16)) {
+        mep_set_error("mep_diff_attn_bwd: float16 without a workspace");
+        return MEP_EINVAL;
+    }
     hipStream_t st = (hipStream_t)stream;
     int qb, kb;
     const int64_t kg = plan(d, d.Tk, 32 * da_kw(d.type, da_width(d.d, d.dv)), kb);
     int64_t qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS, qb);
     if (qg < 0 || kg < 0) { mep_set_error("mep_diff_attn_bwd: too many rows for one launch"); return MEP_EINVAL; }
+    const uint64_t sizes = b.workspace + (uint64_t)kv_bytes(d);
+    if (parts) run(DA_SIZES, d, &b, (int64_t)d.B * d.G * parts, 0, 1, st, d.dv, sizes, parts);
     if (rows) {
         const bool two = two_waves(d, qg, 256);
         if (two) qg = plan(d, (int64_t)d.Tq * (d.H / d.G), DA_ROWS / 2, qb);
-        run(two ? DA_BWD_Q_TWO : DA_BWD_Q, d, &b, qg, qb, 1, st, d.dv);
+        run(two ? DA_BWD_Q_TWO : DA_BWD_Q, d, &b, qg, qb, 1, st, d.dv, sizes, parts);
     }
     if (keys && b.dk) {
         const int splits = b.workspace ? kv_splits(d) : 1;
-        run(DA_BWD_KV, d, &b, kg * splits, kb, splits, st, d.dv);
+        run(DA_BWD_KV, d, &b, kg * splits, kb, splits, st, d.dv, sizes, parts);
         if (splits > 1) {
             const int64_t want = ((int64_t)d.B * d.Tk * d.G * (2 * d.d + d.dv) + DA_THREADS - 1) / DA_THREADS;
             const dim3 grid((unsigned)(want < 4096 ? want : 4096)), block(DA_THREADS);

@@ -1,6 +1,6 @@
 // The differential-attention kernels in MEP_BF16.
 #include "diff_attn.h"
 
-void mep::da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all) {
-    da_run<MEP_BF16>(what, d, b, grid, blocks, splits, st, all);
+void mep::da_run_bf16(int what, const mep_diff_attn_desc& d, const mep_diff_attn_bwd_desc* b, unsigned grid, int blocks, int splits, hipStream_t st, int all, uint64_t sizes, int parts) {
+    da_run<MEP_BF16>(what, d, b, grid, blocks, splits, st, all, sizes, parts);
 }

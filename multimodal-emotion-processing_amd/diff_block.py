@@ -7,9 +7,9 @@
 
 They stand beside the residual-attention blocks of the reference (its Attention_Block takes position tables, one
 softmax map and a LayerNorm behind the block, cmu-mosei/run.py:206-262) and have no counterpart there.  Each call launches
-its kernels (one; more where column sums or splits are joined, an unaligned input is copied, or dq, dk and lam's gradient
-follow each other) on the current stream of its tensors' device, allocates nothing but its results and workspace, never
-synchronises, and may be captured into a graph.  float32, bfloat16 and float16
+its kernels (one; more where column sums or splits are joined, an unaligned input is copied, dq, dk and lam's gradient
+follow each other, or float16 gradients are scaled into range) on the current stream of its tensors' device, allocates nothing
+but its results and workspace, never synchronises, and may be captured into a graph.  float32, bfloat16 and float16
 activations; sums, statistics and angles in 32 bits or more; results do not depend on the order of atomics.
 
 Gradients come through torch.autograd.  To capture a backward pass into a graph, make the leaves it differentiates inside
@@ -426,7 +426,7 @@ class _DiffAttnFn(torch.autograd.Function):
         dlam = torch.empty(lam.shape, dtype=torch.float32, device=dev) if need[7] else None
         delta = torch.empty(B, H, Tq, 4, dtype=torch.float32, device=dev)
         shared = lam.dim() == 1
-        ws = _workspace('mep_diff_attn_bwd_workspace', d, dev) if dk is not None else None
+        ws = _workspace('mep_diff_attn_bwd_workspace', d, dev) if dk is not None or dout.dtype == torch.float16 else None
         bd = _lib.DiffAttnBwdDesc(f=d, dout=_ptr(dout), o_sB=dout.stride(0), o_sT=dout.stride(1), o_sH=dout.stride(2),
                                   dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlam=_ptr(dlam) if shared else 0,
                                   dlam_rows=0 if shared else _ptr(dlam), delta=_ptr(delta), workspace=_ptr(ws))

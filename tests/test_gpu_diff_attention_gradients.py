@@ -1,5 +1,5 @@
 """Gradients of mep_amd.diff_block.diff_attention by their whole error (the Frobenius norm), against the 64-bit form: keys and values
-that have a mean."""
+that have a mean, and float16 upstream gradients of any size."""
 import math
 
 import pytest
@@ -66,7 +66,7 @@ def check(q, k, v, lam, dout, causal=False):
         tol = half * (norm + 2 * t) + tiny * math.sqrt(e.numel())
         err = float((x - e).norm())
         report.append('%s %.2e of %.2e' % (name, err / norm, tol / norm))
-        if not err <= tol:
+        if not (bool(x.isfinite().all()) and err <= tol):
             report[-1] += ' OFF'
     report = '; '.join(report)
     print(report, flush=True)
@@ -88,3 +88,34 @@ def test_means(cuda, size, k_mean, v_mean, dtype):
 @pytest.mark.parametrize('dtype', HALVES)
 def test_means_causal(cuda, dtype):
     check(*case(2, 700, 700, 4, 2, 64, 128, dtype, 2.0, 2.0), rand((2, 700, 4, 128), dtype, 77, grad=False), causal=True)
+
+
+SIZES = [(1, 64, 4096, 1, 1, 64, 128), (1, 300, 700, 2, 1, 32, 64), (1, 70, 2, 2, 2, 64, 64), (1, 40, 1000, 2, 1, 128, 256),
+         (1, 600, 100, 1, 1, 16, 32)]
+
+
+@pytest.mark.parametrize('size', SIZES)
+@pytest.mark.parametrize('std,v_std', [(1e-6, 1.0), (1e-4, 1.0), (1.0, 1.0), (700.0, 1.0), (1500.0, 4.0), (4000.0, 1.0), (4000.0, 0.01)])
+def test_float16_upstream_gradients_of_any_size(cuda, size, std, v_std):
+    """dP past float16's largest number and below its smallest, where the gradients are inside (what a loss scale does)"""
+    a = case(*size, torch.float16, 0.0, 0.0, v_std)
+    if size[2] < 10:      # two keys share a row's weight: their scores are made small, or dq would pass 65504 with dP
+        with torch.no_grad():
+            a[1].mul_(0.05)
+    dout = rand((*size[:2], size[3], size[6]), torch.float16, 77, std, grad=False)
+    check(*a, dout.clamp(-30000, 30000))
+
+
+def test_float16_upstream_gradients_that_differ_by_rows(cuda):
+    """rows' sizes 2^-16 to 2^10 in one block, growing along the queries and falling"""
+    a = case(1, 256, 600, 2, 1, 64, 128, torch.float16, 0.0, 0.0)
+    size = 2.0 ** torch.linspace(-16, 10, 256, device='cuda')[:, None, None]
+    up = rand((1, 256, 2, 128), torch.float32, 77, grad=False)
+    for way in (size, size.flip(0)):
+        check(*a, (up * way).half())
+
+
+@pytest.mark.parametrize('values', [[1e-3, 0.5], [-30.0, 0.2], [900.0, -900.0]])
+def test_float16_lam_of_any_size(cuda, values):
+    q, k, v, _ = case(1, 150, 500, 2, 1, 64, 64, torch.float16, 0.0, 0.0)
+    check(q, k, v, torch.tensor(values, device='cuda', requires_grad=True), rand((1, 150, 2, 64), torch.float16, 77, grad=False))
