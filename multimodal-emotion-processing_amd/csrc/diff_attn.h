@@ -148,12 +148,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes a lane from the buffer `rs` at off + soff to LDS at `dst` + 16 lane (dst of the wave).  In inline assembly, since the
 // compiler would wait for every load in flight before the next LDS read, which is of the other tile; nothing but tile_sync
-// waits for these.  The loads return no registers; m0 is written, and said to be.
+// waits for these.  The loads return no registers; m0 has no other user in these kernels.
 MEP_DEV void dma16(const void* dst, unsigned off, i32x4 rs, unsigned soff) {
     const unsigned at = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const da_lds_char*)dst);
     soff = __builtin_amdgcn_readfirstlane((int)soff);
     // 5 wait states between a readfirstlane and a memory instruction that reads its result, 1 behind m0
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(off), "s"(rs), "s"(soff) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(off), "s"(rs), "s"(soff) : "memory");
 }
 // a raw buffer of DA_SPAN bytes from p on
 MEP_DEV i32x4 da_buffer(const MEP_G void* p) {
