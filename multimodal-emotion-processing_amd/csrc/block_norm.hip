@@ -195,9 +195,11 @@ __global__ __launch_bounds__(norm_threads<L>()) void k_block_norm_fwd(mep_block_
     }
 }
 
-// Column sums of a workgroup: partial[seq * gridDim.x + blockIdx.x][n_sums][D] = those wanted of dw, db, dnw, dnb, dgate, and
-// the scalar dscale behind all of them.  gridDim.y sequences of d.T rows under a sequence gate, else one of all rows.
-template <int TYPE, int V, int L, bool TAIL, bool BIAS>
+// Column sums of a workgroup: partial[blockIdx.y * gridDim.x + blockIdx.x][n_sums][D] = those wanted of dw, db, dnw, dnb, dgate, and
+// the scalar dscale behind all of them.  Under a sequence gate blockIdx.y is a sequence of d.T rows.  MANY: there are more sequences
+// than gridDim.y, and a workgroup takes every gridDim.y-th whole one and writes its gate's gradient itself, so that the partial sums do
+// not grow with the sequences (4096 of one row, 4096 channels in bf16: 8 MB and 60 us, 134 MB and 692 us with a sequence each).
+template <int TYPE, int V, int L, bool TAIL, bool BIAS, bool MANY>
 __global__ __launch_bounds__(norm_threads<L>(), L > 512 ? 4 : 2) void k_block_norm_bwd(mep_block_norm_bwd_desc bd) {
     typedef typename ElemOf<TYPE>::T T;
     constexpr int RPB = norm_threads<L>() / L;
@@ -214,13 +216,14 @@ __global__ __launch_bounds__(norm_threads<L>(), L > 512 ? 4 : 2) void k_block_no
     load_param<T, V, L, TAIL>(BIAS ? d.b : 0, 0, wide, 0.f, lane, D, bi);
     load_param<T, V, L, TAIL>(d.nw, 0, wide, 1.f, lane, D, nw);
     if (d.gate_form <= GATE_CHANNEL) load_param<T, V, L, TAIL>(d.gate, 0, gwide, 1.f, lane, D, gc);
-    else if (d.gate_form == GATE_SEQUENCE) load_param<T, V, L, TAIL>(d.gate, (int64_t)blockIdx.y * D, gwide, 1.f, lane, D, gc);
+    else if (!MANY && d.gate_form == GATE_SEQUENCE) load_param<T, V, L, TAIL>(d.gate, (int64_t)blockIdx.y * D, gwide, 1.f, lane, D, gc);
     const float sc = residual_scale(d);
     float aw[E], ab[E], anw[E], anb[E], ag[E], as = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) aw[i] = ab[i] = anw[i] = anb[i] = ag[i] = 0.f;
-    const int64_t first = d.gate_form == GATE_SEQUENCE ? (int64_t)blockIdx.y * d.T : 0;
-    const int64_t end = d.gate_form == GATE_SEQUENCE ? first + d.T : d.rows;
+    const bool by_seq = MANY || d.gate_form == GATE_SEQUENCE;
+    const int nseq = MANY ? (int)(d.rows / d.T) : 0;
+    int64_t first = by_seq ? (int64_t)blockIdx.y * d.T : 0, end = by_seq ? first + d.T : d.rows;
     int par = 0;
     const int64_t step = (int64_t)gridDim.x * RPB;
     RawRow<T, V> ry, rx, rg, rs, rn;
@@ -234,8 +237,27 @@ __global__ __launch_bounds__(norm_threads<L>(), L > 512 ? 4 : 2) void k_block_no
         if (next) fetch_row<T, V, L, TAIL>(G<const T>(bd.dnormed) + rr * bd.dn_ld, lane, D, rn);
         rst = *reinterpret_cast<const MEP_G f32x4*>(G<const float>(d.stats) + 4 * rr);
     };
-    const int64_t r00 = first + (int64_t)blockIdx.x * RPB;
+    // v's sums over the workgroup's row slots, in order, to to(column, sum)
+    auto join_slots = [&](const float (&v)[E], auto to) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i) slots[slot * L * E + ((i / V) * L + lane) * V + i % V] = v[i];
+        __syncthreads();
+        for (int col = threadIdx.x; col < D; col += norm_threads<L>()) {
+            float s = slots[col];
+#pragma unroll
+            for (int r = 1; r < RPB; ++r) s += slots[r * L * E + col];
+            to(col, s);
+        }
+    };
     constexpr bool AHEAD = L < 1024;                 // 1024 threads have 128 registers each: no room for a row ahead
+    for (int seq = blockIdx.y; !MANY || seq < nseq; seq += gridDim.y) {
+    if constexpr (MANY) {
+        load_param<T, V, L, TAIL>(d.gate, (int64_t)seq * D, gwide, 1.f, lane, D, gc);
+        first = (int64_t)seq * d.T;
+        end = first + d.T;
+    }
+    const int64_t r00 = first + (int64_t)blockIdx.x * RPB;
     if (AHEAD && r00 < end) fetch(r00);
     for (int64_t r0 = r00; r0 < end; r0 += step) {
         const int64_t row = r0 + slot;
@@ -303,6 +325,22 @@ __global__ __launch_bounds__(norm_threads<L>(), L > 512 ? 4 : 2) void k_block_no
         for (int i = 0; i < E; ++i) g[i] = st[1] * (g[i] - mu - y[i] * mq);
         if (live) store_row<T, V, L, TAIL>(G<T>(bd.dy) + row * D, lane, D, g);
     }
+    if constexpr (!MANY) break;
+    if (bd.dgate) {      // (gridDim.x is 1)
+        const int64_t at = (int64_t)seq * D;
+        if constexpr (RPB == 1) {
+            if (gwide) store_row<float, V, L, TAIL>(G<float>(bd.dgate) + at, lane, D, ag);
+            else store_row<T, V, L, TAIL>(G<T>(bd.dgate) + at, lane, D, ag);
+        } else {
+            join_slots(ag, [&](int col, float s) {
+                if (gwide) G<float>(bd.dgate)[at + col] = s;
+                else G<T>(bd.dgate)[at + col] = (T)s;
+            });
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) ag[i] = 0.f;
+    }
+    }
     if (!bd.partial) return;
     const int64_t p = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     gfloat* out = G<float>(bd.partial) + p * bd.n_sums * D;
@@ -310,26 +348,14 @@ __global__ __launch_bounds__(norm_threads<L>(), L > 512 ? 4 : 2) void k_block_no
     auto put = [&](bool on, const float (&v)[E]) {
         if (!on) return;
         gfloat* o = out + (int64_t)k++ * D;
-        if constexpr (RPB == 1) {
-            store_row<float, V, L, TAIL>(o, lane, D, v);
-        } else {      // the row slots' sums, in order
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < E; ++i) slots[slot * L * E + ((i / V) * L + lane) * V + i % V] = v[i];
-            __syncthreads();
-            for (int col = threadIdx.x; col < D; col += norm_threads<L>()) {
-                float s = slots[col];
-#pragma unroll
-                for (int r = 1; r < RPB; ++r) s += slots[r * L * E + col];
-                o[col] = s;
-            }
-        }
+        if constexpr (RPB == 1) store_row<float, V, L, TAIL>(o, lane, D, v);
+        else join_slots(v, [&](int col, float s) { o[col] = s; });
     };
     put(bd.dw != 0, aw);
     put(bd.db != 0, ab);
     put(bd.dnw != 0, anw);
     put(bd.dnb != 0, anb);
-    put(bd.dgate != 0, ag);
+    put(bd.dgate != 0 && !MANY, ag);
     if (bd.dscale) {
         float z = 0.f;
         row_sum2<L>(as, z, red, par);
@@ -418,15 +444,18 @@ int rows_per_block(int D) {
 }
 
 // workgroups per sequence of the backward: as many as the compute units hold over all sequences, at least 4 rows a slot
-// where there are so many (each workgroup's column sums cost 5 D floats), never more than its rows ask for
-int bwd_groups(const mep_block_norm_desc& d, int rpb) {
+// where there are so many (each workgroup's column sums cost 5 D floats), never more than its rows ask for; and how many
+// sequences are taken side by side
+dim3 bwd_grid(const mep_block_norm_desc& d, int rpb) {
     const int64_t nseq = d.gate_form == GATE_SEQUENCE ? d.rows / d.T : 1;
     const int64_t rows = d.rows / nseq;
     const int all = rpb == 1 && d.D > 2048 ? 256 : 512;      // of 512 threads and more, one fits a compute unit
     int64_t most = (all + nseq - 1) / nseq, want = (rows + 4 * rpb - 1) / (4 * rpb);
     const int64_t n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : n);
+    return dim3((unsigned)(n < 1 ? 1 : n), (unsigned)(nseq < all ? nseq : all));
 }
+
+bool many_sequences(const mep_block_norm_desc& d, const dim3& grid) { return d.gate_form == GATE_SEQUENCE && d.rows / d.T > grid.y; }
 
 template <int TYPE, int V, int L, bool TAIL>
 void run_norm(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hipStream_t st) {
@@ -435,9 +464,10 @@ void run_norm(const mep_block_norm_desc& d, const mep_block_norm_bwd_desc* b, hi
         const int64_t want = (d.rows + RPB - 1) / RPB, most = 2048;
         hipLaunchKernelGGL((k_block_norm_fwd<TYPE, V, L, TAIL>), dim3((unsigned)(want < most ? want : most)), dim3(TH), 0, st, d);
     } else {
-        const dim3 grid(bwd_groups(d, RPB), d.gate_form == GATE_SEQUENCE ? (int)(d.rows / d.T) : 1);
-        if (d.b || d.nb) hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, TAIL, true>), grid, dim3(TH), 0, st, *b);
-        else hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, TAIL, false>), grid, dim3(TH), 0, st, *b);
+        const dim3 grid = bwd_grid(d, RPB);
+        if (many_sequences(d, grid)) hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, true, true, true>), grid, dim3(TH), 0, st, *b);
+        else if (d.b || d.nb) hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, TAIL, true, false>), grid, dim3(TH), 0, st, *b);
+        else hipLaunchKernelGGL((k_block_norm_bwd<TYPE, V, L, TAIL, false, false>), grid, dim3(TH), 0, st, *b);
     }
 }
 
@@ -489,8 +519,8 @@ extern "C" int mep_block_norm_fwd(const mep_block_norm_desc* desc, mep_stream_t 
 extern "C" int mep_block_norm_partial(const mep_block_norm_desc* desc) {
     if (!desc || !norm_ok(*desc)) { mep_set_error("mep_block_norm_partial: invalid descriptor"); return MEP_EINVAL; }
     if (desc->rows == 0) return 0;
-    const int nseq = desc->gate_form == GATE_SEQUENCE ? (int)(desc->rows / desc->T) : 1;
-    return bwd_groups(*desc, rows_per_block(desc->D)) * nseq;
+    const dim3 grid = bwd_grid(*desc, rows_per_block(desc->D));
+    return (int)(grid.x * grid.y);
 }
 
 extern "C" int mep_block_norm_bwd(const mep_block_norm_bwd_desc* desc, mep_stream_t stream) {
@@ -510,10 +540,12 @@ extern "C" int mep_block_norm_bwd(const mep_block_norm_bwd_desc* desc, mep_strea
     run_type(b.f, &b, st);
     int rc = mep_check_launch("mep_block_norm_bwd");
     if (rc || !b.partial) return rc;
-    const int nseq = b.f.gate_form == GATE_SEQUENCE ? (int)(b.f.rows / b.f.T) : 1;
-    const int rows_seq = bwd_groups(b.f, rows_per_block(b.f.D));
-    const int ny = sums - !!b.dgate + (b.dgate ? nseq : 0) + !!b.dscale;
+    const dim3 grid = bwd_grid(b.f, rows_per_block(b.f.D));
+    mep_block_norm_bwd_desc s = b;
+    if (many_sequences(b.f, grid)) s.dgate = 0;      // written already
+    const int ny = sums - !!b.dgate + (s.dgate ? (int)grid.y : 0) + !!b.dscale;
+    if (ny == 0) return 0;
     hipLaunchKernelGGL(k_block_norm_sums, dim3((b.f.D + NORM_SUM_COLS - 1) / NORM_SUM_COLS, ny),
-                       dim3(NORM_SUM_COLS * NORM_SUM_SLICES), 0, st, b, rows_seq, nseq);
+                       dim3(NORM_SUM_COLS * NORM_SUM_SLICES), 0, st, s, (int)grid.x, (int)grid.y);
     return mep_check_launch("mep_block_norm_bwd");
 }
