@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "elem.h"
+#include "diff_order.h"
 
 namespace mep {
 
@@ -331,49 +332,12 @@ MEP_DEV void fill_job(const mep_diff_attn_desc& d, Job& j) {
     if (d.q_start) j.first = max(-(1 << 30), min(1 << 30, G<const int>(d.q_start)[j.b]));
     if (d.causal) j.len = max(0, min(j.len, j.first + d.Tq));     // what no query sees is never read
 }
-// Workgroups go round the 8 XCDs by their index; where the (batch, key head) pairs divide evenly over them, a pair's blocks
-// stay on one XCD (or on a few, in turn), so that its keys are read into one L2.
-// Causal calls: the blocks differ by up to their number in length, and all pairs' longest come first.  Where two workgroups share a
-// compute unit (`shared`) and both halves of the first 512 are there from the start, the second half goes the other way, so that
-// the longest shares its unit with the shortest (B 2, T 4096, 8 heads, 64 / 128, bf16: forward 199 us, 207 without that turn, 230 pair by
-// pair).
-enum Order { IN_TURN, FIRST_LONGEST, LAST_LONGEST };
 MEP_DEV Job make_job(const mep_diff_attn_desc& d, int blocks, Order order, bool shared) {
+    const Place p = place_of(blockIdx.x, d.B * d.G, blocks, order, shared);
     Job j;
-    const int x = blockIdx.x, bgs = d.B * d.G;
-    // position s of n on one XCD of 8, or in all; the 32 / 256 units' second ones the other way
-    auto turn = [&](int s, int n, int units) {
-        const int last = min(n, 2 * units) - 1;
-        return shared && s >= units && s <= last ? units + last - s : s;
-    };
-    int bg;
-    if (bgs % 8 == 0) {
-        const int q = bgs / 8;
-        bg = x & 7;
-        if (order == IN_TURN) {
-            const int s = x >> 3, p = s / blocks;
-            bg += p * 8;
-            j.block = s - p * blocks;
-        } else {
-            const int s = turn(x >> 3, blocks * q, 32);
-            j.block = s / q;
-            bg += (s - j.block * q) * 8;
-        }
-    } else if (8 % bgs == 0 && blocks % (8 / bgs) == 0) {
-        const int per = 8 / bgs, s = order == IN_TURN ? x >> 3 : turn(x >> 3, blocks / per, 32);
-        bg = (x & 7) / per;
-        j.block = s * per + (x & 7) % per;
-    } else if (order == IN_TURN) {
-        bg = x / blocks;
-        j.block = x - bg * blocks;
-    } else {
-        const int s = turn(x, blocks * bgs, 256);
-        j.block = s / bgs;
-        bg = s - j.block * bgs;
-    }
-    if (order == LAST_LONGEST) j.block = blocks - 1 - j.block;
-    j.b = bg / d.G;
-    j.g = bg - j.b * d.G;
+    j.block = p.block;
+    j.b = p.bg / d.G;
+    j.g = p.bg - j.b * d.G;
     fill_job(d, j);
     return j;
 }
@@ -897,7 +861,7 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) || (KS == 2 && DV >= 
 // at 4.3 TB/s: two tiles in flight in each of two workgroups on a compute unit.
 // workspace: the number of tiles before each batch row, int [B + 1]; then a part for each wave of each (workgroup, (batch row, key head,
 // 32 rows)) that meet, at workgroup + (batch row, key head, 32 rows): (m1, l1, m2, l2) [R], E_1 [R][dv], E_2 [R][dv], R = min(32, rows)
-constexpr int DA_SPLIT_THREADS = 128, DA_SPLIT_START = 3;
+constexpr int DA_SPLIT_THREADS = 128;
 constexpr bool da_split_full(int type, int dk, int dv) { return dv >= 128 || dk >= 128 || type == MEP_F32; }      // all registers of a SIMD
 constexpr int da_split_groups(int type, int dk, int dv) {      // that are on the chip at a time
     const int lds = (type == MEP_F32 ? 4 : 2) * 2 * da_split_keys(type, dk, dv) * (2 * dk + dv), fit = 160 * 1024 / lds, waves = da_split_full(type, dk, dv) ? 2 : 4;
@@ -905,15 +869,15 @@ constexpr int da_split_groups(int type, int dk, int dv) {      // that are on th
 }
 constexpr int64_t split_floats(int rows, int dv) { return (rows * (4 + 2 * (int64_t)dv) + 3) / 4 * 4; }
 struct Parts {
-    int64_t tiles, share, stride;      // in all; a workgroup's; floats of a part
+    Shares all;
+    int64_t stride;                    // floats of a part
     int per;                           // (key head, 32 rows) of a batch row
     gfloat* first;
 };
 MEP_DEV Parts parts_of(const mep_diff_attn_desc& d, int blocks, int groups, int before_end) {
     Parts p;
     p.per = d.G * blocks;
-    p.tiles = (int64_t)before_end * p.per;
-    p.share = max((p.tiles + groups - 1) / groups, (int64_t)4);      // 4 tiles at least: a part costs as much as one
+    p.all = shares_of(before_end, p.per, groups);
     p.stride = split_floats(min(32, d.Tq * (d.H / d.G)), d.dv);
     p.first = G<float>(d.workspace) + (d.B + 4) / 4 * 4;
     return p;
@@ -955,7 +919,7 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
     if (tid == DA_SPLIT_THREADS - 1) At[1] = upto;
     __syncthreads();
     const Parts parts = parts_of(d, blocks, groups, __builtin_amdgcn_readfirstlane(At[1]));
-    const int64_t start = self * parts.share, stop = min(start + parts.share, parts.tiles);
+    const int64_t start = self * parts.all.share, stop = min(start + parts.all.share, parts.all.tiles);
     const bool some = start < stop;
     const int first_tile = some ? (int)(start / parts.per) : 0;      // of the batch rows' tiles
     int before = upto - mine;
@@ -986,17 +950,17 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
             ++b;
             continue;
         }
-        const int item = (int)(in / n), from = (int)(in - (int64_t)item * n), to = (int)min((int64_t)n, from + (stop - at));
-        const int tile0 = max(0, from - DA_SPLIT_START), tile1 = to - DA_SPLIT_START;
-        at += to - from;
-        if (tile0 >= tile1) continue;
+        const Piece piece = piece_at(in, stop - at, n);
+        const int item = piece.item;
+        at += piece.taken;
+        if (piece.tile0 >= piece.tile1) continue;
         Job j;
         j.b = b;
         j.g = item / blocks;
         j.block = item - j.g * blocks;
         fill_job(d, j);
         const Rows32 w(d, j, j.block * 32);
-        const int begin = tile0 * KT, end = min(w.wend, tile1 * KT);
+        const int begin = piece.tile0 * KT, end = min(w.wend, piece.tile1 * KT);
         const MEP_G T* kp = G<const T>(d.k) + (int64_t)j.b * d.k_sB + (int64_t)j.g * d.k_sH;
         const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
         auto load = [&](T* tile, int k0, unsigned long long bits) {
@@ -1031,7 +995,7 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
         float n1, n2, g1, g2;
         o.maxima(n1, n2, g1, g2);
         const float l1 = half_sum(o.l1) * g1, l2 = half_sum(o.l2) * g2;
-        gfloat* part = parts.first + ((self + (int64_t)b * parts.per + item) * 2 + wave) * parts.stride;
+        gfloat* part = parts.first + (part_at(self, b, parts.per, item) * 2 + wave) * parts.stride;
         const int row = tid & 31, rows = min(32, j.rows);
         if (w.live && h == 0) *reinterpret_cast<MEP_G f32x4*>(part + 4 * row) = f32x4{n1, l1, n2, l2};
         if (w.live && (l1 != 0.f || l2 != 0.f)) {      // without a key of this row here the join reads no further
@@ -1418,8 +1382,8 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
     const int wfull = d.causal ? max(0, min(d.Tq, key0 + 31 - j.first)) * j.n : 0;
     const int rmin = d.causal ? max(0, min(d.Tq, key - j.first)) * j.n : 0;
     // the split's share of the tiles of rows that see a key of the block
-    const int all0 = bstart / RT * RT, all1 = j.block * Sh::KEYS < j.len ? j.rows : 0, share = ((all1 - all0 + RT - 1) / RT + splits - 1) / splits * RT;
-    const int rbeg = all0 + split * share, rend = min(all1, rbeg + share);
+    const Range mine = split_rows(bstart / RT * RT, j.block * Sh::KEYS < j.len ? j.rows : 0, RT, split, splits);
+    const int rbeg = mine.begin, rend = mine.end;
 
     const MEP_G T* qb = G<const T>(d.q) + (int64_t)j.b * d.q_sB + (int64_t)j.g * j.n * d.q_sH;
     const MEP_G T* ob = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;

@@ -49,10 +49,10 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_join(mep_diff_attn_desc d, 
     const Parts ps = parts_of(d, blocks, groups, before[d.B]);
     // the row's tiles are tile .. tile + tiles - 1 of all
     const int item = g * blocks + row / 32, tiles = before[b + 1] - before[b];
-    const int64_t tile = (int64_t)before[b] * ps.per + (int64_t)item * tiles, w0 = (tile + DA_SPLIT_START) / ps.share;
-    const int parts = tiles ? 2 * (int)((tile + tiles - 1) / ps.share - w0 + 1) : 0;
+    const Meet meet = meet_of((int64_t)before[b] * ps.per + (int64_t)item * tiles, tiles, ps.all.share);
+    const int parts = 2 * meet.count;
     const int64_t stride = ps.stride;
-    const gfloat* part = ps.first + (w0 + (int64_t)b * ps.per + item) * 2 * stride;
+    const gfloat* part = ps.first + part_at(meet.first, b, ps.per, item) * 2 * stride;
     const int lr = row & 31;
     auto stats = [&](int p) { return *reinterpret_cast<const MEP_G f32x4*>(part + p * stride + 4 * lr); };
     float m1 = -FLT_MAX, m2 = -FLT_MAX;      // (without keys the backward gets finite ones)
