@@ -73,14 +73,16 @@ def check(q, k, v, lam, dout, causal=False):
     assert 'OFF' not in report, report
 
 
+MEANS = [(0.0, 0.0), (1.0, 1.0), (1.0, 3.0), (3.0, 3.0), (0.0, 3.0)]
+MEAN_SIZES = [(1, 128, 4096, 1, 1, 64, 128), (1, 1024, 1024, 2, 1, 64, 64), (1, 200, 1500, 2, 1, 128, 128), (1, 130, 1000, 1, 1, 128, 256),
+              (1, 200, 1500, 2, 1, 32, 64)]
+
+
 @pytest.mark.parametrize('dtype', HALVES)
-@pytest.mark.parametrize('k_mean,v_mean', [(0.0, 0.0), (1.0, 1.0), (1.0, 3.0), (3.0, 3.0), (0.0, 3.0)])
-@pytest.mark.parametrize('size', [(1, 128, 4096, 1, 1, 64, 128), (1, 1024, 1024, 2, 1, 64, 64), (1, 200, 1500, 2, 1, 128, 128),
-                                  (1, 130, 1000, 1, 1, 128, 256), (1, 200, 1500, 2, 1, 32, 64), (16, 160, 1024, 8, 8, 64, 128)])
+@pytest.mark.parametrize('size,k_mean,v_mean', [(s, *m) for s in MEAN_SIZES for m in MEANS] +
+                         [((16, 160, 1024, 8, 8, 64, 128), *m) for m in (MEANS[1], MEANS[3])])
 def test_means(cuda, size, k_mean, v_mean, dtype):
     """whole rows, shared heads, a row's keys shared by two waves (few workgroups) and not (the last: 256)"""
-    if size[0] > 1 and (k_mean, v_mean) not in ((1.0, 1.0), (3.0, 3.0)):
-        pytest.skip('the large case, at two means')
     a = case(*size, dtype, k_mean, v_mean)
     check(*a, rand((*size[:2], size[3], size[6]), dtype, 77, grad=False))
 
