@@ -402,23 +402,30 @@ MEP_DEV int thread_again() {
 //   |dP - D| <= 2 sum|dO_t| max|v| (dq, by row),  2 max|dO_t| sum|v_k| (dk, by key),  A_1, |lam| A_2 <= w = max(1, |lam|),  |P| <= 2 w
 // no value passes 2^15, and where bound and typical value are 2^6 apart (128 channels of either sign), what is 2^-19 of the
 // typical value is still above 2^-24.  The maxima over a (batch row, key head) come from this kernel, a pass over the values and the
-// upstream gradient: B 4, T 2048, 8 heads, 64 / 128 11 us (B 2, T 1024 7), dq 155 us and dk and dv 277, unscaled 155 and 260.  (Found
+// upstream gradient: B 4, T 2048, 8 heads, 64 / 128 13 us (B 2, T 1024 7), dq 155 us and dk and dv 277, unscaled 155 and 260.  (Found
 // beside the products instead, with the accumulators scaled down whenever a value passes the range: 172 and 298; at 128 / 128 437 and
 // 715, with this kernel 287 and 610.)
-// part p of a (batch row, key head): max |v|, max |dO| w, max w
+// part p of a (batch row, key head), an n-th of its keys and of its rows: max |v|, max |dO| w, max w.  Rows that see no key are left out
+// (their upstream gradient may be anything), and for dk and dv those that are too early for the keys: the last keys' gradients
+// are of the size of the last rows'.
 constexpr int DA_SIZE_PARTS = 64;
 struct Sizes { float v, o, w; };
 template <int TYPE>
 struct Fit {
     static constexpr bool ON = TYPE == MEP_F16;
-    const MEP_G f32x4* parts;
-    int n;
-    MEP_DEV Fit(uint64_t sizes, int count, const mep_diff_attn_desc& d, const Job& j) : parts(G<const f32x4>(sizes) + ((int64_t)j.b * d.G + j.g) * count), n(count) {}
-    MEP_DEV Sizes all() const {
+    // part p's first of `all` keys or rows
+    static MEP_DEV int begin(int all, int p, int n) { return (int)((int64_t)all * p / n); }
+    // over the keys, and the rows from `row` on
+    static MEP_DEV Sizes of(uint64_t sizes, int n, const mep_diff_attn_desc& d, const Job& j, int row) {
         Sizes z = {0.f, 0.f, 1.f};
-        if ((int)(threadIdx.x & 63) < n) {
-            const f32x4 x = parts[threadIdx.x & 63];
-            z = {x[0], x[1], x[2]};
+        const int p = threadIdx.x & 63;
+        if (p < n) {
+            const f32x4 x = G<const f32x4>(sizes)[((int64_t)j.b * d.G + j.g) * n + p];
+            z.v = x[0];
+            if (begin(j.rows, p + 1, n) > row) {
+                z.o = x[1];
+                z.w = x[2];
+            }
         }
         for (int o = 32; o; o /= 2) {
             z.v = fmaxf(z.v, __shfl_xor(z.v, o));
@@ -463,19 +470,20 @@ __global__ __launch_bounds__(DA_THREADS) void k_diff_sizes(mep_diff_attn_bwd_des
     };
     float z[3] = {0.f, 0.f, 1.f};
     // this part's keys: those that are read; and rows
-    const int k0 = (int)((int64_t)j.len * part / parts), k1 = (int)((int64_t)j.len * (part + 1) / parts);
+    const int k0 = Fit<TYPE>::begin(j.len, part, parts), k1 = Fit<TYPE>::begin(j.len, part + 1, parts);
     const MEP_G T* vp = G<const T>(d.v) + (int64_t)j.b * d.v_sB + (int64_t)j.g * d.v_sH;
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < (int64_t)(k1 - k0) * chunks; i += DA_THREADS) {
         const int64_t key = k0 + i / chunks;
         if (d.mask_form != 1 || mask_at(d, (int64_t)j.b * d.m_sB + key * d.m_sK)) z[0] = fmaxf(z[0], largest(vp + key * d.v_sT + i % chunks * M::E));
     }
-    const int r0 = (int)((int64_t)j.rows * part / parts), r1 = (int)((int64_t)j.rows * (part + 1) / parts);
+    const int r0 = Fit<TYPE>::begin(j.rows, part, parts), r1 = Fit<TYPE>::begin(j.rows, part + 1, parts);
     const MEP_G T* op = G<const T>(bd.dout) + (int64_t)j.b * bd.o_sB + (int64_t)j.g * j.n * bd.o_sH;
     const MEP_G float* lp = G<const float>(d.lam) + (int64_t)j.b * d.lam_sB + (int64_t)j.g * j.n * d.lam_sH;
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < (int64_t)(r1 - r0) * chunks; i += DA_THREADS) {
         const int row = r0 + (int)(i / chunks), t = row / j.n, head = row - t * j.n;
+        if (G<const float>(d.stats)[4 * (((int64_t)j.b * d.H + j.g * j.n + head) * d.Tq + t) + 1] == 0.f) continue;      // 1 / l
         const float w = fmaxf(1.f, fabsf(lp[(int64_t)t * d.lam_sT + (int64_t)head * d.lam_sH]));
         z[1] = fmaxf(z[1], w * largest(op + (int64_t)t * bd.o_sT + (int64_t)head * bd.o_sH + i % chunks * M::E));
         z[2] = fmaxf(z[2], w);
@@ -1104,7 +1112,7 @@ __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 
     constexpr bool BESIDE = TYPE != MEP_F32 && DK == 32, CORR = TYPE != MEP_F32 && DK != 32;
     float up = 1.f;                             // dS, and the estimates with it, times up (Fit)
     if constexpr (Fit<TYPE>::ON) {
-        up = ldexpf(1.f, Fit<TYPE>::lift(2.f * size_sum<M, Operand<M, Ge::NV, HOLD>, Ge::NV>(g) * Fit<TYPE>(sizes, parts, d, j).all().v));
+        up = ldexpf(1.f, Fit<TYPE>::lift(2.f * size_sum<M, Operand<M, Ge::NV, HOLD>, Ge::NV>(g) * Fit<TYPE>::of(sizes, parts, d, j, 0).v));
         d1 *= up;
         d2 *= up;
     }
@@ -1605,7 +1613,7 @@ __global__ __launch_bounds__(64 * KW * da_roles(TYPE, DK), da_wide(TYPE, DK) ? 1
     int lift_v = 0, lift_k = 0;
     auto fit = [&](const V* v) {
         if constexpr (Fit<TYPE>::ON) {
-            const Sizes z = Fit<TYPE>(sizes, parts, d, j).all();
+            const Sizes z = Fit<TYPE>::of(sizes, parts, d, j, wstart);
             lift_v = Fit<TYPE>::lift(2.f * z.w);
             if (v) lift_k = Fit<TYPE>::lift(2.f * size_sum<M, V, Ge::NV>(*v) * z.o);
         }

@@ -25,7 +25,7 @@ def case(B, Tq, Tk, H, G, d, dv, dtype, k_mean, v_mean, v_std=1.0, seed=1):
     return q, k, v, lam
 
 
-def check(q, k, v, lam, dout, causal=False):
+def check(q, k, v, lam, dout, by=None, **masks):
     """The error of a whole gradient.  With half = half a step of the type, dS = A (dP - D):
 
     dq   rounding dS adds at most half sqrt(sum dS^2 |k|^2) / sqrt(3) on average, independent from key to key.  A row's D may be off
@@ -34,21 +34,22 @@ def check(q, k, v, lam, dout, causal=False):
          S = sqrt(sum over rows of (sum dS^2) (sum A |k|^2)) plus sqrt(sum dS^2 |k|^2).
     dk   sums dS^T q of rows with their D as summed: 2 half sqrt(sum dS^2 |q|^2) for its 0.6.
     dv   sums P^T dO: likewise.
-    Each is rounded once more (half, and half a subnormal step of every element).  float32's own sums are far below."""
+    Each is rounded once more (half, and half a subnormal step of every element).  float32's own sums are far below.
+    by: dk and dv by that many keys at a time."""
     from mep_amd import diff_block as db
     B, Tq, H, _, d = q.shape
     Tk, G = k.shape[1], k.shape[2]
     n, sc = H // G, d ** -0.5
     half = ref.half_step(q.dtype)
     tiny = torch.finfo(q.dtype).smallest_normal * half
-    got = torch.autograd.grad(db.diff_attention(q, k, v, lam, causal=causal), (q, k, v, lam), dout)
+    got = torch.autograd.grad(db.diff_attention(q, k, v, lam, **masks), (q, k, v, lam), dout)
     w = [ref.wide(t) for t in (q, k, v, lam)]
-    ok = ref.allowed(B, Tq, Tk, None, None, causal, None)
+    ok = ref.allowed(B, Tq, Tk, masks.get('mask'), masks.get('lengths'), masks.get('causal', False), masks.get('q_start'))
     exact = torch.autograd.grad(ref.diff_attention(*w, ok), w, dout.cpu().double())
     with torch.no_grad():
         kk, vv, do = w[1].repeat_interleave(n, 2), w[2].repeat_interleave(n, 2), dout.cpu().double()
         s = torch.einsum('bthmd,bshmd->bhmts', w[0], kk) * sc
-        a = torch.softmax(s.masked_fill(~ok[:, None, None], -1e300), -1)
+        a = torch.softmax(s.masked_fill(~ok[:, None, None], -1e300), -1) * ok.any(-1)[:, None, None, :, None]
         l = w[3].reshape(1, H, 1, 1)
         dp = torch.einsum('bthe,bshe->bhts', do, vv)
         ds = a * (dp[:, :, None] - (a * dp[:, :, None]).sum(-1, keepdim=True)) * torch.stack([torch.ones_like(l), l], 2) * sc
@@ -56,16 +57,20 @@ def check(q, k, v, lam, dout, causal=False):
         q2 = (w[0] * w[0]).sum(-1).permute(0, 2, 3, 1)[..., None]
         ds2 = ds * ds
         tq = math.sqrt(float((ds2 * k2).sum())) + math.sqrt(float((ds2.sum(-1) * (a * k2).sum(-1)).sum()))
-        tk = math.sqrt(float((ds2 * q2).sum()))
+        tk = (ds2 * q2).sum((0, 1, 2, 3))                                 # by key
         p = a[:, :, 0] - l * a[:, :, 1]
-        tv = math.sqrt(float((p * p * (do * do).sum(-1).permute(0, 2, 1)[..., None]).sum()))
+        tv = (p * p * (do * do).sum(-1).permute(0, 2, 1)[..., None]).sum((0, 1, 2))
     report = []
-    for name, x, e, t in zip(('dq', 'dk', 'dv'), got, exact, (tq, tk, tv)):
+    parts = [('dq', got[0], exact[0], tq)]
+    for i in range(0, Tk, by or Tk):
+        at = slice(i, i + (by or Tk))
+        parts += [('dk', got[1][:, at], exact[1][:, at], math.sqrt(float(tk[at].sum()))), ('dv', got[2][:, at], exact[2][:, at], math.sqrt(float(tv[at].sum())))]
+    for name, x, e, t in parts:
         x = x.cpu().double()
         norm = float(e.norm())
         tol = half * (norm + 2 * t) + tiny * math.sqrt(e.numel())
         err = float((x - e).norm())
-        report.append('%s %.2e of %.2e' % (name, err / norm, tol / norm))
+        report.append('%s %.2e of %.2e' % (name, err / (norm or 1.0), tol / (norm or 1.0)))
         if not (bool(x.isfinite().all()) and err <= tol):
             report[-1] += ' OFF'
     report = '; '.join(report)
@@ -121,3 +126,23 @@ def test_float16_upstream_gradients_that_differ_by_rows(cuda):
 def test_float16_lam_of_any_size(cuda, values):
     q, k, v, _ = case(1, 150, 500, 2, 1, 64, 64, torch.float16, 0.0, 0.0)
     check(q, k, v, torch.tensor(values, device='cuda', requires_grad=True), rand((1, 150, 2, 64), torch.float16, 77, grad=False))
+
+
+@pytest.mark.parametrize('size', [(1, 600, 600, 2, 1, 64, 128), (1, 600, 600, 1, 1, 16, 32), (2, 300, 900, 2, 2, 128, 128)])
+def test_float16_upstream_gradients_that_fall_along_a_causal_row(cuda, size):
+    """the last keys' gradients come from rows that are 2^-24 of the first's"""
+    a = case(*size, torch.float16, 0.0, 0.0)
+    fall = 2.0 ** torch.linspace(9, -15, size[1], device='cuda')[:, None, None]
+    up = rand((*size[:2], size[3], size[6]), torch.float32, 77, grad=False)
+    check(*a, (up * fall).half(), by=100, causal=True)
+
+
+def test_float16_rows_that_see_nothing(cuda):
+    """whatever upstream gradients they have"""
+    a = case(2, 200, 300, 2, 1, 64, 64, torch.float16, 0.0, 0.0)
+    up = rand((2, 200, 2, 64), torch.float16, 77, 1e-3, grad=False)
+    up[:, :50] = 60000.0
+    check(*a, up, by=100, causal=True, q_start=torch.full((2,), -50, dtype=torch.int32, device='cuda'))
+    mask = torch.ones(2, 200, 300, dtype=torch.bool, device='cuda')
+    mask[:, :50] = False
+    check(*a, up, by=100, mask=mask)
