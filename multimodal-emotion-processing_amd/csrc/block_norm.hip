@@ -11,9 +11,11 @@
 // Bound by memory: every row is read and written once, held in registers in between: 8 elements in each of L lanes, L = 16
 // of a wave to 1024 of a workgroup by the row's width, in 16-byte accesses at any address (TAIL: widths that end inside one).
 // A workgroup walks many rows with the parameters, and in the backward the column sums, in registers; the sums of its row
-// slots are joined in LDS, those of the workgroups by a second kernel, in a fixed order.  8 elements a lane leave the
-// backward's registers (parameters, up to 5 sums and 4 rows) room for 4 waves on a SIMD: at 16384 rows of 4096 in bf16, both
-// norms and a gate, 211 us (4.1 TB/s), 455 with 16 elements; the forward 131 us.
+// slots are joined in LDS, those of the workgroups by a second kernel, in a fixed order.  With 8
+// elements a lane the backward (parameters, up to 5 sums and 4 rows) holds everything in about 200 registers, two waves on a SIMD: at
+// 16384 rows of 4096 in bf16, both norms and a gate, 196 us (4.1 TB/s), 455 with 16 elements; the forward 119 us (4.5 TB/s).
+// Rows of more than 4096 channels have 1024 lanes of 128 registers each, which does not hold the backward: it spills 93 to 441 of them, and
+// 8192 rows of 8192 take 531 us (1.5 TB/s; forward 125 us, 4.3).
 #include "elem.h"
 
 namespace {

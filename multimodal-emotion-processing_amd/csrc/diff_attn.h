@@ -9,7 +9,9 @@
 //
 // The difference is formed before anything is rounded to 16 bits: two nearly equal maps cancel, and rounding each of them
 // first would leave an error of 2^-9 of the parts in a difference of a few hundredths.  See k_diff_fwd for how one pass over the
-// keys does that.  Scores, statistics and accumulators are fp32; P and dS are rounded once, as operands of the second products.
+// keys does that.  Scores, statistics and accumulators are fp32; P and dS are rounded once, as operands of the second products, because
+// the matrix instructions take no wider ones.  In 16 bits results are so off by 1.4 times what rounding them alone would leave (whole
+// errors of 2.3e-3 and 1.7e-3 in bf16, 2.9e-4 and 2.1e-4 in float16).
 //
 // Products on v_mfma_f32_32x32x16 (fp32: 32x32x2).  Scores are formed transposed (keys x rows): a lane holds one row and 16
 // keys, the row statistics are lane-local, and the accumulator registers are the second product's operand as they are
@@ -149,7 +151,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes a lane from the buffer `rs` at off + soff to LDS at `dst` + 16 lane (dst of the wave).  In inline assembly, since the
 // compiler would wait for every load in flight before the next LDS read, which is of the other tile; nothing but tile_sync
-// waits for these.  The loads return no registers; m0 has no other user in these kernels.
+// waits for these.  The loads return no registers.  m0 is a reserved register, which the compiler keeps nothing in (it cannot be named
+// as clobbered), and no other instruction of these kernels uses it.
 MEP_DEV void dma16(const void* dst, unsigned off, i32x4 rs, unsigned soff) {
     const unsigned at = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const da_lds_char*)dst);
     soff = __builtin_amdgcn_readfirstlane((int)soff);
@@ -276,6 +279,7 @@ MEP_DEV typename M::Frag acc_frag(const floatx16& p, int i) {
     return f;
 }
 
+// (the instruction: off by 2^-23 of its result, as much as a score's own rounding)
 MEP_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 2^(s c - m), c = scale log2 e.  In fp32 the rounding of c is put right (it would shift every exponent the same way, by up to
@@ -595,7 +599,7 @@ MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, i
 // the sums l_m stay lane-local to the end.
 // Bound by vector operations beside the products: a step of 32 keys x 32 rows has 24 matrix instructions (64 / 128; 768 cycles) and about
 // 240 others, 32 of them exponentials (1350 cycles), and two waves on a SIMD overlap them in part; s_setprio lets the wave whose products
-// are ready go first (254 us -> 230).  B 2, T 4096, 8 heads, causal: 199 us; B 1, T 8192, 16 heads on 4 key heads: 490 us, 560 TFLOP/s
+// are ready go first (254 us -> 230).  B 2, T 4096, 8 heads, causal: 178 us; B 1, T 8192, 16 heads on 4 key heads: 466 us, 590 TFLOP/s
 // of the 512 operations that a pair takes by the formula.
 template <int TYPE, int DK, int DV>
 struct Online {
@@ -863,8 +867,9 @@ __global__ __launch_bounds__(DA_THREADS, da_wide(TYPE, DK) || (KS == 2 && DV >= 
 // Few rows against many keys (single tokens against a cache).  The tiles of keys of all (batch row, key head, 32 rows) stand in one
 // row, those behind a batch row's length left out, and each of `groups` workgroups takes an equal share of it: equal work whatever
 // the lengths (B 32 of up to 8192 keys, 4 key heads: 81 us, against 105 with as many tiles to a workgroup in each batch row's own
-// splits), neighbouring shares on one XCD; to begin with the next rows counts as DA_SPLIT_START tiles (87 us without).  A workgroup has
-// two waves; of a tile of 64 keys (32 where two of 64 do not fit LDS: of every other tile) a wave takes 32, and for each batch row it
+// splits), neighbouring shares on one XCD; to begin with the next rows counts as DA_SPLIT_START tiles (87 us without).  (Causal calls of
+// many rows: the tiles that an item's rows do not see are dealt out too and passed over, so that a call takes as long as without the
+// order of time, and less than whole: T 4096, one head, 64 / 128, bf16 80 us, 84 and 137.)  A workgroup has two waves; of a tile of 64 keys (32 where two of 64 do not fit LDS: of every other tile) a wave takes 32, and for each batch row it
 // comes to it leaves its rows' maxima, sums, E_1 and E_2 in fp32; k_diff_join joins them.  Bound by reading the keys and values once,
 // at 4.3 TB/s: two tiles in flight in each of two workgroups on a compute unit.
 // workspace: the number of tiles before each batch row, int [B + 1]; then a part for each wave of each (workgroup, (batch row, key head,
@@ -1046,8 +1051,9 @@ __global__ __launch_bounds__(DA_SPLIT_THREADS, da_split_full(TYPE, DK, DV) ? 1 :
 // keys (a weight over 1 / 4).  (Without a mean that is 1.3 r, 2.5 r at most in 4096 waves.  Single rows reach 8 r, and one pass
 // taken twice keeps its whole launch waiting: asked of each row, B 4, T 2048, 8 heads, 64 / 128 took 185 us instead of 143.)  What the
 // second pass costs where keys and values have a mean (as large as the deviation, bf16): 64 / 128 at B 2, T 4096, causal 208 -> 313 us,
-// at B 4, T 2048 152 -> 229, 128 / 128 there 282 -> 474.  (In fp32 the estimate is as good as the sum.)  The sums are also lam's
-// gradient and what dk needs.
+// at B 4, T 2048 152 -> 229, 128 / 128 there 282 -> 474.  (In fp32 the estimate is left as it is: its error is that of the forward's
+// sums over keys, 4e-7 of the terms.  Without a mean that is below dq's own; with means as large as the deviations, 2048 keys, it makes
+// 9e-6 of dq, where elementary operations in 32 bits leave 2e-6.)  The sums are also lam's gradient and what dk needs.
 template <int TYPE, int DK, int DV, int KS>
 __global__ __launch_bounds__(DA_THREADS, DK >= 128 || (KS == 2 && DK >= 64) ? 1 : 2) void k_diff_bwd_q(mep_diff_attn_bwd_desc bd, int blocks, uint64_t sizes, int parts) {
     typedef RowShape<TYPE, DK, DV, KS> Sh;

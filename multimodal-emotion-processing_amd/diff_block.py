@@ -290,6 +290,7 @@ def norm_residual(y, residual, weight=None, bias=None, *, kind='rms', gate=None,
     [B, D] or [B, 1, D] for y [B, T, D] (one row per sequence), or y's shape; float32 or y's type, y's type for the last.
     scale: a number, or a one-element float32 tensor that is learned.  Returns stream, or (stream, normed).
     Under torch.autocast, where a block's output is of 16 bits and the residual stream float32, all are widened to float32.
+    With both kinds 'none', small rows are slower than the torch operations they stand for.
     """
     _type_of(y, 'y')
     if residual is not None and residual.dtype != y.dtype and residual.dtype in TYPES and torch.is_autocast_enabled('cuda'):
@@ -449,7 +450,10 @@ def diff_attention(q, k, v, lam, *, mask=None, lengths=None, causal=False, q_sta
       lengths   int32 [B]: the keys at and behind it are not there (a padded batch, a cache)
       causal    query t of row b sees the keys up to q_start[b] + t; q_start int32 [B], Tk - Tq without it
     Keys past the lengths, past every query's causal reach or of a zero in a [B, Tk] mask never enter a result, whatever they
-    hold; the keys that only some queries may see must be finite.
+    hold; the keys that only some queries may see must be finite, and so must scores be: they are formed in float32, where scores over
+    2^24 lie more than 1 apart.
+    q, k, v and upstream gradients whose rows are not whole and aligned 16 bytes are copied first, a cache whole at every call.
+    float32 with gradients is slower than elementary torch operations where heads are wider than 64.
     """
     _type_of(q, 'q')
     if q.dim() != 5 or k.dim() != 5 or v.dim() != 4 or q.shape[3] != 2 or k.shape[3] != 2 or q.shape[4] != k.shape[4] or \
