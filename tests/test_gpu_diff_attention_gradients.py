@@ -122,6 +122,34 @@ def test_float16_upstream_gradients_that_differ_by_rows(cuda):
         check(*a, (up * way).half())
 
 
+def test_float16_captured_and_replayed(cuda):
+    """a float16 training pass in a graph, on upstream gradients and values of other sizes at each replay, against the eager pass"""
+    from mep_amd import diff_block as db
+    a = [t.detach() for t in case(2, 150, 300, 4, 2, 64, 128, torch.float16, 0.0, 0.0)]
+    up = rand((2, 150, 4, 128), torch.float16, 9, grad=False)
+
+    def train():
+        leaves = [t.detach().requires_grad_() for t in a]
+        out = db.diff_attention(*leaves)
+        return (out,) + torch.autograd.grad(out, leaves, up)
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        train()
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = train()
+    for std, v_std in ((1.0, 1.0), (3000.0, 0.01), (1e-4, 4.0), (1000.0, 1.0)):
+        up.copy_(rand(up.shape, torch.float16, 11, std, grad=False))
+        a[2].copy_(rand(a[2].shape, torch.float16, 12, v_std, grad=False))
+        g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, train()):
+            assert torch.equal(x, y) and bool(x.isfinite().all())
+
+
 @pytest.mark.parametrize('values', [[1e-3, 0.5], [-30.0, 0.2], [900.0, -900.0]])
 def test_float16_lam_of_any_size(cuda, values):
     q, k, v, _ = case(1, 150, 500, 2, 1, 64, 64, torch.float16, 0.0, 0.0)
