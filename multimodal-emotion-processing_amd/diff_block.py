@@ -289,11 +289,11 @@ def norm_residual(y, residual, weight=None, bias=None, *, kind='rms', gate=None,
     next_weight, next_bias [D] in float32 or y's type (all the same).  gate: None, [D] (learned per channel),
     [B, D] or [B, 1, D] for y [B, T, D] (one row per sequence), or y's shape; float32 or y's type, y's type for the last.
     scale: a number, or a one-element float32 tensor that is learned.  Returns stream, or (stream, normed).
-    Under torch.autocast, where a block's output is of 16 bits and the residual stream float32, all are widened to float32.
+    Under torch.autocast, where products are of 16 bits, all are widened to float32 if y or the residual is.
     With both kinds 'none', small rows are slower than the torch operations they stand for.
     """
     _type_of(y, 'y')
-    if residual is not None and residual.dtype != y.dtype and residual.dtype in TYPES and torch.is_autocast_enabled('cuda'):
+    if torch.is_autocast_enabled('cuda') and (y.dtype == torch.float32 or (residual is not None and residual.dtype == torch.float32)):
         y, residual, weight, bias, gate, next_weight, next_bias = (
             t.float() if t is not None and t.dtype in TYPES else t for t in (y, residual, weight, bias, gate, next_weight, next_bias))
     if y.dim() < 1 or not 1 <= y.shape[-1] <= _lib.BLOCK_NORM_MAX_D:

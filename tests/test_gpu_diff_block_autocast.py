@@ -74,3 +74,16 @@ def test_other_types_are_still_refused(cuda):
             db.norm_residual(y, x.double())
         with pytest.raises(ValueError, match='gate'):
             db.norm_residual(y, x, gate=torch.ones(8, dtype=torch.int32, device='cuda'))
+
+
+def test_gate_of_a_product_on_a_float32_block(cuda):
+    """y and the stream are float32, the gate comes out of a product; and all of 16 bits with a float32 gate stay in 16"""
+    from mep_amd import diff_block as db
+    y, x, g = (rand((3, 5, 16), torch.float32, i) for i in range(3))
+    with pytest.raises(ValueError, match='gate'):
+        db.norm_residual(y, x, gate=g.bfloat16())
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        for gate in (g.bfloat16(), g.bfloat16()[0, 0], g.bfloat16()[:, 0]):
+            assert torch.equal(db.norm_residual(y, x, gate=gate), db.norm_residual(y, x, gate=gate.float()))
+        assert torch.equal(db.norm_residual(y, None, gate=g.bfloat16()), db.norm_residual(y, None, gate=g.bfloat16().float()))
+        assert db.norm_residual(y.bfloat16(), x.bfloat16(), gate=g[0, 0]).dtype == torch.bfloat16
