@@ -594,7 +594,8 @@ MEP_DEV void write_rows(typename M::T* buf, const floatx16 (&acc)[N], float f, i
 // What is rounded is the difference itself, up to the estimate's error: where the maps cancel, l_1 / l_2 hardly changes along the
 // keys and Y's factor vanishes.  rho is renewed, by X' = f1' (X + f2 Y) / f1 - f2' Y, at every rescaling and whenever it is
 // off the sums so far (these keys' own among them) by a quarter: a few times a row, and neither operand is ever of a size
-// that the row's weights do not have.
+// that the row's weights do not have.  (A weight of the second map that a larger one has since replaced was rounded in both operands, and
+// leaves the difference behind: up to a step of rho times its value.)
 // The maxima m_m are renewed only when a score exceeds one by 8 (e <= 256: the sums are as exact), the lanes of a row agree on them, and
 // the sums l_m stay lane-local to the end.
 // Bound by vector operations beside the products: a step of 32 keys x 32 rows has 24 matrix instructions (64 / 128; 768 cycles) and about

@@ -450,8 +450,8 @@ def diff_attention(q, k, v, lam, *, mask=None, lengths=None, causal=False, q_sta
       lengths   int32 [B]: the keys at and behind it are not there (a padded batch, a cache)
       causal    query t of row b sees the keys up to q_start[b] + t; q_start int32 [B], Tk - Tq without it
     Keys past the lengths, past every query's causal reach or of a zero in a [B, Tk] mask never enter a result, whatever they
-    hold; the keys that only some queries may see must be finite, and so must scores be: they are formed in float32, where scores over
-    2^24 lie more than 1 apart.
+    hold; the keys that only some queries may see must be finite.  Scores, scale q_m k_m^T, must lie within 2^22: they are formed in
+    float32, and past that the rounding of an exponent alone can pass a type's range.
     q, k, v and upstream gradients whose rows are not whole and aligned 16 bytes are copied first, a cache whole at every call.
     float32 with gradients is slower than elementary torch operations where heads are wider than 64.
     """

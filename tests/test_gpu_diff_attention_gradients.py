@@ -122,6 +122,39 @@ def test_float16_upstream_gradients_that_differ_by_rows(cuda):
         check(*a, (up * way).half())
 
 
+@pytest.mark.parametrize('dtype', [torch.float32] + HALVES)
+@pytest.mark.parametrize('size', [(1, 70, 200, 2, 1, 64, 128), (1, 200, 200, 2, 2, 16, 32), (1, 2, 1500, 4, 1, 64, 64), (1, 40, 100, 1, 1, 128, 256)])
+def test_scores_up_to_their_limit(cuda, size, dtype):
+    """Scores of up to 2^22: finite, and rows whose largest scores are alone by 64 or more (their roundings are 1 at most) give those keys'
+    values, by the whole error.  Four operands and the result are rounded (2 half of |v_1| + |v_2|, independent), and each time that
+    a larger score of the second map came up the one before it left half a step of at most 1.25 lam of its own value: H_47 = 4.4
+    times in 47 tiles of keys, independent: sqrt(4.4) 1.25 0.8 = 2.1 half.  Together under 4."""
+    from mep_amd import diff_block as db
+    q, k, v, lam = case(*size, dtype, 0.0, 0.0)
+    B, Tq, H, _, d = q.shape
+    n = H // k.shape[2]
+    score = lambda: torch.einsum('bthmd,bshmd->bhmts', q.detach().cpu().double(), k.detach().cpu().double().repeat_interleave(n, 2)) * d ** -0.5  # noqa: E731
+    with torch.no_grad():
+        f = math.sqrt(2.0 ** 22 / float(score().abs().max())) * 0.99
+        q.mul_(f)
+        k.mul_(f)
+    s = score()
+    assert 2.0 ** 21 < float(s.abs().max()) < 2.0 ** 22
+    out = db.diff_attention(q, k, v, lam)
+    got = torch.autograd.grad(out, (q, k, v, lam), rand(out.shape, dtype, 77, grad=False))
+    assert all(bool(x.isfinite().all()) for x in (out, *got))
+    top = s.topk(2, -1)
+    alone = (top.values[..., 0] - top.values[..., 1] > 64).all(2)                  # [B, H, Tq], in both maps
+    assert float(alone.double().mean()) > 0.9
+    vv = v.detach().cpu().double().repeat_interleave(n, 2)
+    pick = [torch.gather(vv.transpose(1, 2), 2, top.indices[:, :, m, :, :1].expand(-1, -1, -1, v.shape[-1])) for m in (0, 1)]
+    want = pick[0] - lam.detach().cpu().double()[:, None, None] * pick[1]
+    err = (out.detach().cpu().double().transpose(1, 2) - want)[alone]
+    tol = 4 * (ref.half_step(dtype) + 16 * ref.U) * float((pick[0].abs() + pick[1].abs())[alone].norm())
+    print('%.2e of %.2e' % (float(err.norm()), tol), flush=True)
+    assert float(err.norm()) <= tol
+
+
 def test_float16_captured_and_replayed(cuda):
     """a float16 training pass in a graph, on upstream gradients and values of other sizes at each replay, against the eager pass"""
     from mep_amd import diff_block as db
