@@ -123,10 +123,10 @@ bool rows_ok(const mep_diff_attn_desc& d, uint64_t p, int64_t sB, int64_t sT, in
     return p % 16 == 0 && sB % V == 0 && sT % V == 0 && sH % V == 0 && sM % V == 0 && sT >= 0 && sT < 1 << 23 && sM >= 0 && sM < 1 << 28 &&
            (!heads || (sH >= 0 && sH * h < 1 << 28)) && 64 * sT + sM + sH * h < (V << 27) - 512;
 }
-bool inputs_ok(const mep_diff_attn_desc& d) {
-    return rows_ok(d, d.q, d.q_sB, d.q_sT, d.q_sH, d.q_sM, true) && rows_ok(d, d.k, d.k_sB, d.k_sT, d.k_sH, d.k_sM, false) &&
-           rows_ok(d, d.v, d.v_sB, d.v_sT, d.v_sH, 0, false);
+bool keys_ok(const mep_diff_attn_desc& d) {
+    return rows_ok(d, d.k, d.k_sB, d.k_sT, d.k_sH, d.k_sM, false) && rows_ok(d, d.v, d.v_sB, d.v_sT, d.v_sH, 0, false);
 }
+bool inputs_ok(const mep_diff_attn_desc& d) { return rows_ok(d, d.q, d.q_sB, d.q_sT, d.q_sH, d.q_sM, true) && keys_ok(d); }
 
 // the workgroups of a launch over `items` rows or keys per (batch, key head), `per` each, or -1 (too many)
 int64_t plan(const mep_diff_attn_desc& d, int64_t items, int per, int& blocks) {
@@ -324,11 +324,11 @@ extern "C" int mep_diff_attn_bwd(const mep_diff_attn_bwd_desc* desc, mep_stream_
     const mep_diff_attn_bwd_desc& b = *desc;
     const mep_diff_attn_desc& d = b.f;
     const bool rows = d.B > 0 && d.Tq > 0, keys = d.B > 0 && d.Tk > 0;
-    if ((rows && (!d.stats || !d.second || !b.dout || !b.delta)) || (keys && (!b.dk != !b.dv))) {
+    if ((rows && (!d.stats || !d.second || !b.dout || !b.delta)) || (keys && (!b.dk != !b.dv || !d.k || !d.v))) {
         mep_set_error("mep_diff_attn_bwd: a missing operand");
         return MEP_EINVAL;
     }
-    if (rows && (!inputs_ok(d) || !rows_ok(d, b.dout, b.o_sB, b.o_sT, b.o_sH, 0, true))) {
+    if ((rows && (!inputs_ok(d) || !rows_ok(d, b.dout, b.o_sB, b.o_sT, b.o_sH, 0, true))) || (keys && !keys_ok(d))) {
         mep_set_error("mep_diff_attn_bwd: rows that cannot be read 16 bytes at a time");
         return MEP_EINVAL;
     }

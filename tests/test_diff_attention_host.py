@@ -30,6 +30,16 @@ def test_float16_backward_needs_its_workspace(workspace):
     assert b'workspace' in buf.value
 
 
+@pytest.mark.parametrize('type', [F32, BF16, F16])
+@pytest.mark.parametrize('wrong', [dict(k=0), dict(v=0), dict(k=(1 << 20) + 4), dict(v_sT=7), dict(k_sM=3)])
+def test_backward_without_queries_still_reads_keys(type, wrong):
+    """dk and dv of no queries are zeros, formed by the kernel that loads the keys: their addresses have to be there"""
+    f = forward(type, Tq=0)
+    for n, x in wrong.items():
+        setattr(f, n, x)
+    assert _lib.lib().mep_diff_attn_bwd(ctypes.byref(backward(f, workspace=1 << 20)), None) == -1000
+
+
 @pytest.mark.parametrize('size', [dict(), dict(B=1, Tq=1, Tk=1, H=1, G=1), dict(B=1, Tq=4096, Tk=64, H=8, G=1), dict(B=3000, G=1, H=1), dict(Tq=0), dict(Tk=0)])
 def test_workspace_bytes(size):
     """room for the float16 backward's sizes whatever is split, and none in the other types where nothing is"""
